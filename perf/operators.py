@@ -187,11 +187,16 @@ _compute = None
 
 
 class _View:
-    """The CUDA array interface of a framework buffer."""
+    """The CUDA array interface of a framework buffer that lives as long as the tensors over it."""
 
-    def __init__(self, address, like):
+    def __init__(self, label, like):
         kind = {torch.float32: "<f4", torch.float16: "<f2", torch.float64: "<f8", torch.int32: "<i4"}[like.dtype]
-        self.__cuda_array_interface__ = {"data": (address, False), "shape": tuple(like.shape), "typestr": kind, "version": 3}
+        self.buffer = _compute.buffer(like.numel() * like.element_size(), label)
+        self.__cuda_array_interface__ = {"data": (_compute.address(self.buffer), False), "shape": tuple(like.shape), "typestr": kind,
+                                         "version": 3}
+
+    def __del__(self):
+        _compute.destroy(self.buffer)
 
 
 class _Buffers:
@@ -202,27 +207,22 @@ class _Buffers:
         if _compute is None:
             from webgpu_amd.gpu import Compute
             _compute = Compute().init()
-        c, self.held, self.at, self.tensor = _compute, [], {}, {}
+        self.at, self.tensor = {}, {}
         for name, t in inputs.items():
             if name in ("sees", "depth") or t is None:
                 continue
-            pairs = [self.place(c, name, x) for x in (t.unbind(0) if name == "rings" else [t])]
+            pairs = [self.place(name, x) for x in (t.unbind(0) if name == "rings" else [t])]
             self.at[name], self.tensor[name] = ([p[i] for p in pairs] for i in range(2))
             if name != "rings":
                 self.at[name], self.tensor[name] = self.at[name][0], self.tensor[name][0]
         torch.cuda.synchronize()
 
-    def place(self, c, name, t):
-        b = c.buffer(t.numel() * t.element_size(), name)
-        self.held.append(b)
-        c.done()
-        view = torch.as_tensor(_View(c.address(b), t), device="cuda")
-        view.copy_(t)
-        return b, view
-
-    def __del__(self):
-        for b in self.held:
-            _compute.destroy(b)
+    def place(self, name, t):
+        view = _View(name, t)
+        _compute.done()  # the new buffer's zeros come before its values
+        tensor = torch.as_tensor(view, device="cuda")
+        tensor.copy_(t)
+        return view.buffer, tensor
 
 
 # ------------------------------------------------------------------------------- the plain forms
