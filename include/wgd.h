@@ -69,6 +69,10 @@ int wgd_buffer_create(wgd_context *ctx, uint64_t size, const char *label, wgd_bu
 /* Compute.destroy (gpu.ts:31). */
 int wgd_buffer_destroy(wgd_context *ctx, wgd_buffer *buf);
 uint64_t wgd_buffer_size(const wgd_buffer *buf);
+/* The device address of a buffer, for hosts that fill or read it with their own device code
+ * ordered against wgd_stream(). It stays valid until the buffer is destroyed (NULL for a NULL
+ * handle). Buffers of wgd_upload_weights hold this library's own layout. */
+void *wgd_buffer_address(const wgd_buffer *buf);
 /* WeightPager.page (pager.ts:25-44) with paging collapsed: upload a whole rows x cols weight
  * matrix of GGUF `type` once, in the layout the kernels read fastest. Q4_K, Q5_K and Q6_K
  * (and Q8_0 / Q4_0 of a width that is a multiple of 64) are rearranged on the device into a
@@ -211,6 +215,76 @@ int wgd_sample(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, double te
  * in f64 (scale = sqrt(hidden) for Gemma 3, else 1). ids is int32[n]. */
 int wgd_embed(wgd_context *ctx, int32_t type, const wgd_buffer *table, const wgd_buffer *ids,
               wgd_buffer *out, uint32_t hidden, uint32_t n, double scale);
+
+/* ---------------------------------------------------------------- drafted trees
+ * One decode step over a tree of drafted tokens (no reference counterpart): a host drafts
+ * `nodes` tokens after the `start` cached ones, runs the model over all of them as one batch,
+ * and keeps the path that the model's own draws confirm. Node i has the position start + its
+ * depth and its K/V in ring slot (start + i) % capacity. parents (int32[nodes], on the device)
+ * holds the node that i follows, in [0, i), or -1 where it follows the last cached token; node 0
+ * is the token that the step before picked. Any other value makes i and every node below it
+ * padding: attention writes zeros for it and no path takes it, so trees of several sizes can
+ * share one launch shape. The launches allocate nothing once a call of the same sizes has run,
+ * so they can be captured into HIP graphs; where their scratch would have to grow during a
+ * capture they fail with WGD_E_STATE and the capture stays valid. Graphs keep using the
+ * context's scratch: replay them in order with its other work. */
+#define WGD_TREE_MAX 256 /* most nodes of a tree */
+
+/* Rotary embedding at given positions, in place: for token t < batch and head h < heads, x at
+ * t * stride + offset + h * head_dim (floats; stride 0: heads * head_dim) has its first
+ * rotary_dim dims (0 = head_dim) rotated pairwise, (j, j + rot/2) or with `adjacent` (2j, 2j+1):
+ *   (l, r) -> magnitude * (l cos a - r sin a, l sin a + r cos a),
+ *   a = positions[t] * scale * theta^(-2j/rot) / factors[j].
+ * positions is int32[batch], factors f32[rot/2] or NULL for ones; linear, NTK, by-parts (YaRN)
+ * and Llama 3 scaling are factors and a magnitude (webgpu_amd/rope.py makes them). Angles are
+ * formed and reduced in f64, and the tail of a head is left as it is. Query and key heads that
+ * lie side by side in a row are one call. For models with Q/K norm run wgd_norm with n =
+ * head_dim first. */
+int wgd_rope_at(wgd_context *ctx, wgd_buffer *x, const wgd_buffer *positions, const wgd_buffer *factors,
+                uint32_t heads, uint32_t head_dim, float theta, float scale, float magnitude, uint32_t rotary_dim,
+                uint32_t stride, uint64_t offset, int32_t adjacent, uint32_t batch);
+/* Attention of every node of a drafted tree: query q[i][h] over the cached keys t in
+ * (position_i - window, start), at ring slot t % capacity as in wgd_attention, and over i itself
+ * and its ancestors within the window; y[i][h] = softmax(scale * q.k) V, zeros for padding. A
+ * node outside i's ancestors never reaches y[i], whatever its K/V hold. Needs nodes <=
+ * WGD_TREE_MAX, head_dim <= 512, start < 2^31 and a ring that holds every key that some node sees,
+ * min(start, window - 1) + nodes <= capacity. */
+int wgd_attention_tree(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *y,
+                       const wgd_buffer *parents, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t start,
+                       float scale, uint32_t window, uint32_t capacity, uint32_t nodes);
+/* The same over f16 rings (wgd_attention_f16kv's): scores, softmax and sums stay f32. */
+int wgd_attention_tree_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v,
+                             wgd_buffer *y, const wgd_buffer *parents, uint32_t heads, uint32_t kv_heads,
+                             uint32_t head_dim, uint32_t start, float scale, uint32_t window, uint32_t capacity,
+                             uint32_t nodes);
+/* One token for each of `rows` rows of n logits, `stride` floats apart (0: n), drawn with the
+ * caller's uniforms (f64[rows] in [0, 1)) into tokens (int32[rows]) on the device, without
+ * waiting. The finite logits in descending order, ties to the lower index, have weights
+ * exp((l - best) / temperature); kept are the top_k first (0: all of them), of these the
+ * shortest prefix whose share of their weight reaches top_p, and of these the ones with a weight
+ * of min_p or more; the token is the first whose running sum reaches uniform * (the kept
+ * weight). With min_p 0 that is wgd_sample's rule. Weights and sums are integers of
+ * 2^-(62 - ceil(log2 n)) of the largest weight, so a draw does not depend on the order of the sums.
+ * Temperature 0 takes the best; so does a uniform outside [0, 1). A row without a finite logit
+ * gets -1. temperature <= 2, 0 < top_p <= 1, 0 <= min_p <= 1 (WGD_E_INVALID otherwise). */
+int wgd_sample_rows(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, uint32_t rows, uint32_t stride,
+                    const wgd_buffer *uniforms, wgd_buffer *tokens, double temperature, uint32_t top_k, double top_p,
+                    double min_p);
+/* The drafted path that the model confirms: from node 0, the lowest child i of the node c reached
+ * with drafted[i] == picked[c] (the token drawn at c), until none is. path (int32[nodes + 2])
+ * becomes the count of nodes on it, the token picked at the last one, their indices in
+ * order, and -1 behind them; count 0 and token -1 where node 0 is padding. A negative picked
+ * token ends the path. */
+int wgd_tree_accept(wgd_context *ctx, const wgd_buffer *parents, const wgd_buffer *drafted, const wgd_buffer *picked,
+                    wgd_buffer *path, uint32_t nodes);
+/* Moves the K/V rows of an accepted path (as wgd_tree_accept writes it) to the slots that its
+ * tokens keep: row (start + path[2 + j]) % capacity of every ring to row (start + j) % capacity,
+ * for j < path[0]; the other rows stay. `rings` is a host array of `count` distinct buffers of
+ * [capacity][row_bytes] (K and V of any number of layers; row_bytes = kv_heads * head_dim * 4, or
+ * * 2 for f16 rings, a multiple of 2); nodes <= capacity. Entries of the path that do not lie
+ * beyond their own place and below `nodes` move nothing. */
+int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, const wgd_buffer *path,
+                  uint64_t row_bytes, uint32_t start, uint32_t capacity, uint32_t nodes);
 
 /* ---------------------------------------------------------------- measurement
  * No reference counterpart: `launches` back-to-back plain streaming reads of `bytes`

@@ -1349,3 +1349,5 @@ hipError_t decode_attention(hipStream_t s, const DecodeAttnArgs &in) {
 }
 
 }  // namespace wgd
+
+#include "attention_tree.h"

@@ -208,6 +208,36 @@ hipError_t attention(hipStream_t s, const AttnArgs &a);
 // not limit the split count (0: one split, no scratch used).
 uint64_t attention_partial_need(const AttnArgs &a);
 uint64_t attention_scratch_floats(uint32_t heads, uint32_t hd, uint32_t batch, uint32_t max_keys);
+// ---------------------------------------------------------------- drafted trees (include/wgd.h)
+// x[t * stride + h * hd ..]: rotary embedding at positions[t]; rot even, rot <= hd.
+struct RopeAtArgs {
+  float *x; const int32_t *positions; const float *factors;  // factors may be null
+  uint32_t heads, hd, rot, stride, batch;
+  float theta, scale, magnitude;
+  bool adjacent;
+};
+hipError_t rope_at(hipStream_t s, const RopeAtArgs &a);
+struct TreeAttnArgs {
+  const float *q; const void *k, *v; float *y; const int32_t *parents;
+  uint32_t heads, kv_heads, hd, start, window, capacity, nodes;
+  float scale;
+  bool kv16 = false;
+  float *partial = nullptr; uint64_t partial_floats = 0;  // at least attention_tree_scratch_floats()
+};
+uint64_t attention_tree_scratch_floats(const TreeAttnArgs &a);
+hipError_t attention_tree(hipStream_t s, const TreeAttnArgs &a);
+struct SampleRowsArgs {
+  const float *logits; uint32_t n, rows; uint64_t stride;
+  const double *uniforms; int32_t *tokens;
+  double temperature, top_p, min_p; uint32_t top_k;
+  void *scratch = nullptr;  // sample_rows_scratch_bytes()
+};
+uint64_t sample_rows_scratch_bytes(const SampleRowsArgs &a);
+hipError_t sample_rows(hipStream_t s, const SampleRowsArgs &a);
+hipError_t tree_accept(hipStream_t s, const int32_t *parents, const int32_t *drafted, const int32_t *picked, int32_t *path,
+                       uint32_t nodes);
+hipError_t kv_commit(hipStream_t s, void *const *rings, uint32_t count, const int32_t *path, uint64_t row_bytes,
+                     uint32_t start, uint32_t capacity, uint32_t nodes);
 hipError_t add(hipStream_t s, const float *delta, float *state, uint32_t n);
 hipError_t glu(hipStream_t s, const float *gate, const float *up, float *y, uint32_t n, int act);
 // glu() over [batch][cols] that also writes y in the prompt GEMM's split form (cols % 64 == 0).

@@ -494,6 +494,136 @@ hipError_t rope(hipStream_t s, float *x, const float *w, uint32_t heads, uint32_
   return hipGetLastError();
 }
 
+// ------------------------------------------------------------------ drafted trees: rotary positions
+// A workgroup per (token, group of heads): the token's rotations, formed once in LDS with the f64
+// angles of k_rope, then every pair of its heads.
+__global__ __launch_bounds__(256) void k_rope_at(RopeAtArgs a, uint32_t per) {
+  __shared__ float2 cs[256];
+  const uint32_t t = blockIdx.x, h0 = blockIdx.y * per, nh = min(per, a.heads - h0), half = a.rot / 2;
+  float *x = a.x + (uint64_t)t * a.stride + (uint64_t)h0 * a.hd;
+  const double pos = (double)a.positions[t] * (double)a.scale;
+  for (uint32_t p0 = 0; p0 < half; p0 += 256) {
+    const uint32_t np = min(256u, half - p0);
+    __syncthreads();
+    if (threadIdx.x < np) {
+      const uint32_t j = p0 + threadIdx.x;
+      double angle = pos * pow((double)a.theta, -(double)(2 * j) / (double)a.rot);
+      if (a.factors) angle /= (double)a.factors[j];
+      double sn, c;
+      sincos(angle, &sn, &c);
+      cs[threadIdx.x] = make_float2((float)(c * (double)a.magnitude), (float)(sn * (double)a.magnitude));
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < nh * np; i += 256) {
+      const uint32_t h = i / np, j = i % np;
+      float *v = x + (uint64_t)h * a.hd;
+      const uint32_t ia = a.adjacent ? 2 * (p0 + j) : p0 + j, ib = a.adjacent ? ia + 1 : ia + half;
+      const float l = v[ia], r = v[ib], c = cs[j].x, sn = cs[j].y;
+      v[ia] = l * c - r * sn;
+      v[ib] = l * sn + r * c;
+    }
+  }
+}
+
+hipError_t rope_at(hipStream_t s, const RopeAtArgs &a) {
+  if (!a.batch || !a.heads) return hipSuccess;
+  if (!a.rot || a.rot % 2 || a.rot > a.hd) return hipErrorInvalidValue;
+  const uint32_t per = a.heads;
+  hipLaunchKernelGGL(k_rope_at, dim3(a.batch, (a.heads + per - 1) / per), dim3(256), 0, s, a, per);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ drafted trees: the accepted path
+// One wavefront, four nodes per lane: a step of the walk is four ballots for the lowest child of
+// the node reached that drafted its picked token. Children come after their parent, so the walk ends.
+__global__ __launch_bounds__(64) void k_tree_accept(const int32_t *parents, const int32_t *drafted, const int32_t *picked,
+                                                    int32_t *path, int32_t n) {
+  __shared__ int32_t pick[WGD_TREE_MAX];
+  constexpr int PER = WGD_TREE_MAX / 64;
+  const int lane = (int)threadIdx.x;
+  int32_t par[PER], dr[PER];
+#pragma unroll
+  for (int r = 0; r < PER; r++) {
+    const int i = 64 * r + lane;
+    par[r] = i < n ? parents[i] : -2;
+    dr[r] = i < n ? drafted[i] : -1;
+    pick[i] = i < n ? picked[i] : -1;
+  }
+  __syncthreads();
+  int32_t count = 0, next = -1;
+  if (__builtin_amdgcn_readfirstlane(par[0]) == -1) {
+    int cur = 0;
+    for (;;) {
+      if (lane == 0) path[2 + count] = cur;
+      count++;
+      next = pick[cur];
+      int child = n;
+#pragma unroll
+      for (int r = PER - 1; r >= 0; r--) {
+        const uint64_t m = __ballot(par[r] == cur && dr[r] == next && 64 * r + lane > cur);
+        if (m) child = 64 * r + (int)__ffsll((unsigned long long)m) - 1;
+      }
+      if (next < 0 || child >= n) break;
+      cur = child;
+    }
+  }
+  if (lane == 0) { path[0] = count; path[1] = next; }
+  for (int i = count + lane; i < n; i += 64) path[2 + i] = -1;
+}
+
+hipError_t tree_accept(hipStream_t s, const int32_t *parents, const int32_t *drafted, const int32_t *picked, int32_t *path,
+                       uint32_t nodes) {
+  if (!nodes || nodes > WGD_TREE_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k_tree_accept, dim3(1), dim3(64), 0, s, parents, drafted, picked, path, (int32_t)nodes);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ drafted trees: the accepted rows
+// Row (start + path[2 + j]) % capacity of each ring to row (start + j) % capacity. A thread owns one
+// unit of U bytes of the rows of one ring and moves the path's rows in order, eight loads ahead of
+// their stores: a row lies beyond its place, so no store reaches a row that is read later.
+constexpr uint32_t COMMIT_RINGS = 64;
+struct CommitRings { void *p[COMMIT_RINGS]; };
+
+template <class U>
+__global__ __launch_bounds__(256) void k_kv_commit(CommitRings rings, const int32_t *path, uint32_t units, uint32_t start,
+                                                   uint32_t capacity, int32_t n) {
+  const uint32_t u = blockIdx.x * 256 + threadIdx.x;
+  if (u >= units) return;
+  U *ring = (U *)rings.p[blockIdx.y];
+  const int32_t count = min(path[0], n);
+  for (int32_t j0 = 0; j0 < count; j0 += 8) {
+    U v[8];
+    bool move[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int32_t j = j0 + e, node = j < count ? path[2 + j] : -1;
+      move[e] = node > j && node < n;
+      if (move[e]) v[e] = ring[(uint64_t)((start + (uint32_t)node) % capacity) * units + u];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (move[e]) ring[(uint64_t)((start + (uint32_t)(j0 + e)) % capacity) * units + u] = v[e];
+  }
+}
+
+hipError_t kv_commit(hipStream_t s, void *const *rings, uint32_t count, const int32_t *path, uint64_t row_bytes,
+                     uint32_t start, uint32_t capacity, uint32_t nodes) {
+  if (!nodes || nodes > capacity || !row_bytes || row_bytes % 2) return hipErrorInvalidValue;
+  const uint32_t unit = row_bytes % 16 == 0 ? 16 : row_bytes % 4 == 0 ? 4 : 2, units = (uint32_t)(row_bytes / unit);
+  for (uint32_t r0 = 0; r0 < count; r0 += COMMIT_RINGS) {
+    const uint32_t nr = count - r0 < COMMIT_RINGS ? count - r0 : COMMIT_RINGS;
+    CommitRings c{};
+    for (uint32_t i = 0; i < nr; i++) c.p[i] = rings[r0 + i];
+    const dim3 grid((units + 255) / 256, nr);
+    if (unit == 16) hipLaunchKernelGGL(k_kv_commit<uint4>, grid, dim3(256), 0, s, c, path, units, start, capacity, (int32_t)nodes);
+    else if (unit == 4) hipLaunchKernelGGL(k_kv_commit<uint32_t>, grid, dim3(256), 0, s, c, path, units, start, capacity, (int32_t)nodes);
+    else hipLaunchKernelGGL(k_kv_commit<uint16_t>, grid, dim3(256), 0, s, c, path, units, start, capacity, (int32_t)nodes);
+    WGD_HIP(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
 // ------------------------------------------------------------------ elementwise
 __global__ void k_add(const float *d, float *state, uint32_t n) {
   for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) state[i] += d[i];

@@ -10,6 +10,8 @@
 #include <mutex>
 #include <set>
 #include <string>
+#include <vector>
+#include <cmath>
 
 #include "internal.h"
 #include "matvec.h"
@@ -186,6 +188,8 @@ int wgd_buffer_destroy(wgd_context *ctx, wgd_buffer *b) {
 }
 
 uint64_t wgd_buffer_size(const wgd_buffer *b) { return b ? b->size : 0; }
+
+void *wgd_buffer_address(const wgd_buffer *b) { return b ? b->ptr : nullptr; }
 
 void *wgd_stream(const wgd_context *ctx) { return ctx ? (void *)ctx->stream : nullptr; }
 
@@ -670,6 +674,155 @@ int wgd_sample(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, double te
   *token = id;
   if (id < 0) return fail(ctx, WGD_E_NONFINITE, "Inference produced non-finite logits. Stop and report this model/runtime combination.");
   return WGD_OK;
+}
+
+// ---------------------------------------------------------------- drafted trees
+
+// Scratch of the drafted-tree launchers, grown by doubling and kept with the context. A captured
+// graph keeps its address: nothing is allocated during a capture, and a block that a graph may
+// hold is kept until the context ends when a larger one takes its place.
+static int tree_workspace(wgd_context *ctx, uint64_t need, const char *what, void **out) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  hipError_t e = hipStreamIsCapturing(ctx->stream, &st);
+  if (e != hipSuccess) return hip_fail(ctx, e, what);
+  const bool capturing = st != hipStreamCaptureStatusNone;
+  if (need > ctx->tree_scratch_bytes) {
+    if (capturing)
+      return fail(ctx, WGD_E_STATE, "%s: its scratch would have to grow during a stream capture; run a call of these sizes once before", what);
+    if (!ctx->tree_scratch_captured) ctx_free(ctx, ctx->tree_scratch);
+    uint64_t size = std::max(need, 2 * ctx->tree_scratch_bytes);
+    ctx->tree_scratch = nullptr; ctx->tree_scratch_bytes = 0;
+    if (ctx->allocated + size > ctx->limit) size = need;
+    int rc = ctx_alloc(ctx, size, "drafted-tree scratch", &ctx->tree_scratch);
+    if (rc) return rc;
+    ctx->tree_scratch_bytes = size;
+    ctx->tree_scratch_captured = false;
+  }
+  if (capturing) ctx->tree_scratch_captured = true;
+  *out = ctx->tree_scratch;
+  return WGD_OK;
+}
+
+int wgd_rope_at(wgd_context *ctx, wgd_buffer *x, const wgd_buffer *positions, const wgd_buffer *factors, uint32_t heads,
+                uint32_t hd, float theta, float scale, float magnitude, uint32_t rot, uint32_t stride, uint64_t offset,
+                int32_t adjacent, uint32_t batch) {
+  NEED_CTX(ctx); NEED_BUF(ctx, x, "rope_at"); NEED_BUF(ctx, positions, "rope_at");
+  if (hd == 0 || hd % 2 || rot % 2 || rot > hd) return fail(ctx, WGD_E_INVALID, "rope_at: head_dim %u / rotary_dim %u invalid", hd, rot);
+  if (!(theta > 0.f) || !std::isfinite(theta)) return fail(ctx, WGD_E_INVALID, "rope_at: theta %g is not a positive number", (double)theta);
+  if (!heads || !batch) return WGD_OK;
+  const uint64_t row = (uint64_t)heads * hd;
+  if (row > 0xFFFFFFFFull || (stride && stride < row)) return fail(ctx, WGD_E_INVALID, "rope_at: stride %u < %u heads of %u", stride, heads, hd);
+  RopeAtArgs a{};
+  a.heads = heads; a.hd = hd; a.rot = rot ? rot : hd; a.stride = stride ? stride : (uint32_t)row; a.batch = batch;
+  a.theta = theta; a.scale = scale; a.magnitude = magnitude; a.adjacent = adjacent != 0;
+  if (offset > x->size / 4) return fail(ctx, WGD_E_INVALID, "rope_at: offset %llu outside buffer %s", (unsigned long long)offset, x->label.c_str());
+  NEED_FIT(ctx, x, (offset + (uint64_t)(batch - 1) * a.stride + row) * 4, "rope_at input");
+  NEED_FIT(ctx, positions, (uint64_t)batch * 4, "rope_at positions");
+  if (factors) { NEED_BUF(ctx, factors, "rope_at"); NEED_FIT(ctx, factors, (uint64_t)a.rot / 2 * 4, "rope_at factors"); }
+  if (x == positions || x == factors) return fail(ctx, WGD_E_INVALID, "rope_at: positions and factors need buffers of their own");
+  a.x = (float *)x->ptr + offset; a.positions = (const int32_t *)positions->ptr;
+  a.factors = factors ? (const float *)factors->ptr : nullptr;
+  return ctx_check(ctx, rope_at(ctx->stream, a), "rope_at");
+}
+
+static int attention_tree_common(wgd_context *ctx, const char *what, const wgd_buffer *q, const wgd_buffer *k,
+                                 const wgd_buffer *v, wgd_buffer *y, const wgd_buffer *parents, uint32_t heads,
+                                 uint32_t kv_heads, uint32_t hd, uint32_t start, float scale, uint32_t window,
+                                 uint32_t capacity, uint32_t nodes, bool kv16) {
+  NEED_CTX(ctx);
+  NEED_BUF(ctx, q, what); NEED_BUF(ctx, k, what); NEED_BUF(ctx, v, what); NEED_BUF(ctx, y, what); NEED_BUF(ctx, parents, what);
+  const uint64_t esz = kv16 ? 2 : 4;
+  if (!kv_heads || !heads || heads % kv_heads || !hd || hd > 512 || !capacity || !window)
+    return fail(ctx, WGD_E_INVALID, "%s: invalid heads %u/%u, head_dim %u, capacity %u or window %u", what, heads, kv_heads, hd, capacity, window);
+  if (nodes > WGD_TREE_MAX) return fail(ctx, WGD_E_INVALID, "%s: %u nodes, a tree has at most %u", what, nodes, WGD_TREE_MAX);
+  if (start > 0x7FFFFFFFu) return fail(ctx, WGD_E_INVALID, "%s: start %u is beyond 2^31 - 1", what, start);
+  if (heads > (1u << 20)) return fail(ctx, WGD_E_INVALID, "%s: %u heads", what, heads);
+  if ((uint64_t)std::min(start, window - 1) + nodes > capacity)
+    return fail(ctx, WGD_E_INVALID, "%s: %u cached keys and %u nodes do not fit a ring of %u slots", what, std::min(start, window - 1), nodes, capacity);
+  if (y == q || y == k || y == v || y == parents) return fail(ctx, WGD_E_INVALID, "%s: the output needs a buffer of its own", what);
+  if (!nodes) return WGD_OK;
+  NEED_FIT(ctx, q, (uint64_t)nodes * heads * hd * 4, "attention queries");
+  NEED_FIT(ctx, k, (uint64_t)capacity * kv_heads * hd * esz, "attention keys");
+  NEED_FIT(ctx, v, (uint64_t)capacity * kv_heads * hd * esz, "attention values");
+  NEED_FIT(ctx, y, (uint64_t)nodes * heads * hd * 4, "attention output");
+  NEED_FIT(ctx, parents, (uint64_t)nodes * 4, "tree parents");
+  TreeAttnArgs a{};
+  a.q = (const float *)q->ptr; a.k = k->ptr; a.v = v->ptr; a.y = (float *)y->ptr; a.parents = (const int32_t *)parents->ptr;
+  a.heads = heads; a.kv_heads = kv_heads; a.hd = hd; a.start = start; a.window = window; a.capacity = capacity; a.nodes = nodes;
+  a.scale = scale; a.kv16 = kv16;
+  a.partial_floats = attention_tree_scratch_floats(a);
+  int rc = tree_workspace(ctx, a.partial_floats * 4, what, (void **)&a.partial);
+  if (rc) return rc;
+  return ctx_check(ctx, attention_tree(ctx->stream, a), what);
+}
+
+int wgd_attention_tree(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *y,
+                       const wgd_buffer *parents, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t start,
+                       float scale, uint32_t window, uint32_t capacity, uint32_t nodes) {
+  return attention_tree_common(ctx, "attention_tree", q, k, v, y, parents, heads, kv_heads, hd, start, scale, window,
+                               capacity, nodes, false);
+}
+
+int wgd_attention_tree_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v,
+                             wgd_buffer *y, const wgd_buffer *parents, uint32_t heads, uint32_t kv_heads, uint32_t hd,
+                             uint32_t start, float scale, uint32_t window, uint32_t capacity, uint32_t nodes) {
+  return attention_tree_common(ctx, "attention_tree_f16kv", q, k, v, y, parents, heads, kv_heads, hd, start, scale, window,
+                               capacity, nodes, true);
+}
+
+int wgd_sample_rows(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, uint32_t rows, uint32_t stride,
+                    const wgd_buffer *uniforms, wgd_buffer *tokens, double temperature, uint32_t top_k, double top_p,
+                    double min_p) {
+  NEED_CTX(ctx); NEED_BUF(ctx, logits, "sample_rows"); NEED_BUF(ctx, uniforms, "sample_rows"); NEED_BUF(ctx, tokens, "sample_rows");
+  if (!n || n > 0x7FFFFFFFu || (stride && stride < n)) return fail(ctx, WGD_E_INVALID, "sample_rows: rows of %u logits, %u apart", n, stride);
+  if (!(temperature >= 0.0 && temperature <= 2.0) || !(top_p > 0.0 && top_p <= 1.0) || !(min_p >= 0.0 && min_p <= 1.0))
+    return fail(ctx, WGD_E_INVALID, "Invalid sampling settings.");
+  if (tokens == logits || tokens == uniforms) return fail(ctx, WGD_E_INVALID, "sample_rows: the tokens need a buffer of their own");
+  if (!rows) return WGD_OK;
+  SampleRowsArgs a{};
+  a.n = n; a.rows = rows; a.stride = stride ? stride : n;
+  NEED_FIT(ctx, logits, ((uint64_t)(rows - 1) * a.stride + n) * 4, "sample_rows logits");
+  NEED_FIT(ctx, uniforms, (uint64_t)rows * 8, "sample_rows uniforms");
+  NEED_FIT(ctx, tokens, (uint64_t)rows * 4, "sample_rows tokens");
+  a.logits = (const float *)logits->ptr; a.uniforms = (const double *)uniforms->ptr; a.tokens = (int32_t *)tokens->ptr;
+  a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
+  int rc = tree_workspace(ctx, sample_rows_scratch_bytes(a), "sample_rows", &a.scratch);
+  if (rc) return rc;
+  return ctx_check(ctx, sample_rows(ctx->stream, a), "sample_rows");
+}
+
+int wgd_tree_accept(wgd_context *ctx, const wgd_buffer *parents, const wgd_buffer *drafted, const wgd_buffer *picked,
+                    wgd_buffer *path, uint32_t nodes) {
+  NEED_CTX(ctx);
+  NEED_BUF(ctx, parents, "tree_accept"); NEED_BUF(ctx, drafted, "tree_accept"); NEED_BUF(ctx, picked, "tree_accept"); NEED_BUF(ctx, path, "tree_accept");
+  if (!nodes || nodes > WGD_TREE_MAX) return fail(ctx, WGD_E_INVALID, "tree_accept: %u nodes, a tree has 1 to %u", nodes, WGD_TREE_MAX);
+  NEED_FIT(ctx, parents, (uint64_t)nodes * 4, "tree parents");
+  NEED_FIT(ctx, drafted, (uint64_t)nodes * 4, "drafted tokens");
+  NEED_FIT(ctx, picked, (uint64_t)nodes * 4, "picked tokens");
+  NEED_FIT(ctx, path, (uint64_t)(nodes + 2) * 4, "accepted path");
+  if (path == parents || path == drafted || path == picked) return fail(ctx, WGD_E_INVALID, "tree_accept: the path cannot be one of the inputs");
+  return ctx_check(ctx, tree_accept(ctx->stream, (const int32_t *)parents->ptr, (const int32_t *)drafted->ptr,
+                                    (const int32_t *)picked->ptr, (int32_t *)path->ptr, nodes), "tree_accept");
+}
+
+int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, const wgd_buffer *path, uint64_t row_bytes,
+                  uint32_t start, uint32_t capacity, uint32_t nodes) {
+  NEED_CTX(ctx); NEED_BUF(ctx, path, "kv_commit");
+  if (!nodes || nodes > WGD_TREE_MAX) return fail(ctx, WGD_E_INVALID, "kv_commit: %u nodes, a tree has 1 to %u", nodes, WGD_TREE_MAX);
+  if (nodes > capacity || start > 0x7FFFFFFFu || !row_bytes || row_bytes % 2 || row_bytes > (1u << 30))
+    return fail(ctx, WGD_E_INVALID, "kv_commit: %u nodes at %u in a ring of %u rows of %llu bytes", nodes, start, capacity, (unsigned long long)row_bytes);
+  NEED_FIT(ctx, path, (uint64_t)(nodes + 2) * 4, "accepted path");
+  if (!count) return WGD_OK;
+  if (!rings) return fail(ctx, WGD_E_INVALID, "kv_commit: NULL rings");
+  std::vector<void *> at(count);
+  std::set<const wgd_buffer *> seen;
+  for (uint32_t i = 0; i < count; i++) {
+    NEED_BUF(ctx, rings[i], "kv_commit");
+    NEED_FIT(ctx, rings[i], (uint64_t)capacity * row_bytes, "kv_commit ring");
+    if (rings[i] == path || !seen.insert(rings[i]).second) return fail(ctx, WGD_E_INVALID, "kv_commit: ring %u (%s) is given twice or is the path", i, rings[i]->label.c_str());
+    at[i] = rings[i]->ptr;
+  }
+  return ctx_check(ctx, kv_commit(ctx->stream, at.data(), count, (const int32_t *)path->ptr, row_bytes, start, capacity, nodes), "kv_commit");
 }
 
 int wgd_embed(wgd_context *ctx, int32_t type, const wgd_buffer *table, const wgd_buffer *ids, wgd_buffer *out,

@@ -32,6 +32,9 @@
 //     probabilities, their running sum (one thread, in order) and the draw.
 //     It is a chain of latencies in one workgroup, not of bytes: 128256 logits, k = 40, took
 //     19.9 us by the histogram and serial sums with a division per step, 12.1 us so.
+#include <algorithm>
+#include <cmath>
+
 #include "internal.h"
 #include "decode.h"
 
@@ -450,6 +453,391 @@ hipError_t sample(hipStream_t s, const float *logits, uint32_t n, const SamplePa
   hipLaunchKernelGGL(k_sample, dim3(1), dim3(SMP_T), 0, s, (const uint64_t *)cand, (const SliceOut *)so, ns, sl, params,
                      value, index, st, out, tokens, cap, advance ? 1 : 0);
   return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ rows with given uniforms
+//
+// wgd_sample_rows: for every row the finite logits in descending order (composites, as above)
+// have the weights w = exp((l - best) / T) in f64, rounded to integers of 2^-shift with shift = 62 -
+// ceil(log2 n): their sums fit 64 bits, are exact, and do not depend on the order of the adds,
+// so atomics give the same token every time. A top-k, top-p or min-p cut and the draw itself are all
+// "the first token whose running count reaches A or whose running sum reaches X". Three launches:
+//   * k_rows_best (slices x rows): the slices' best composites and finite counts;
+//   * k_rows_hist (slices x rows): counts and weights over RS_BINS bins of (best - l) / T, which is
+//     monotonic in l, and the weight that min-p keeps;
+//   * k_rows_pick (a workgroup a row): the bin of each cut from the running histogram, then its tokens
+//     gathered, sorted and summed in LDS. A bin with more tokens than LDS holds (ties, logits far below the
+//     temperature's scale) is refined by 12 bits of the composite at a time.
+constexpr uint32_t RS_T = 1024, RS_BINS = 4096, RS_CAP = 2048;
+constexpr uint32_t RS_HT = 256, RS_SLICES = 64, RS_MIN = 2048;  // slice kernels: threads, slices, slice floor
+constexpr uint32_t RS_ROWS = 256;  // rows per launch: the histograms of more would only fill memory
+constexpr float RS_SPAN = 48.f;    // bins cover exp(0) to exp(-48) < 2^-62; the last one all below
+
+struct RowSlice { uint64_t best; uint32_t finite, pad; };
+struct RowHist {
+  uint64_t mass[RS_BINS];
+  uint32_t count[RS_BINS];
+  uint64_t minp;
+  RowSlice slice[RS_SLICES];
+};
+struct RowsK {
+  const float *logits; uint32_t n, slice, nslices; uint64_t stride;
+  const double *uniforms; int32_t *tokens; RowHist *hist;
+  double temperature, top_p, min_p, unit;  // unit: 2^shift
+  float bins;                              // bins per unit of logit
+  uint32_t top_k;
+};
+
+__device__ __forceinline__ uint32_t row_bin(const RowsK &a, float best, float l) {
+  return (uint32_t)fminf((best - l) * a.bins, (float)(RS_BINS - 1));
+}
+__device__ __forceinline__ double row_weight(const RowsK &a, float best, float l) {
+  return exp(((double)l - (double)best) / a.temperature);
+}
+__device__ __forceinline__ uint64_t row_mass(const RowsK &a, double w) { return (uint64_t)(w * a.unit + 0.5); }
+__device__ __forceinline__ uint64_t composite(float l, uint32_t i) { return ((uint64_t)order_key(l) << 32) | (0xFFFFFFFFu - i); }
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+__global__ __launch_bounds__(RS_HT) void k_rows_best(RowsK a) {
+  __shared__ uint64_t wmax[RS_HT / 64];
+  __shared__ uint32_t wsum[RS_HT / 64];
+  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const float *row = a.logits + blockIdx.y * a.stride;
+  RowHist &h = a.hist[blockIdx.y];
+  uint64_t best = 0;
+  uint32_t cnt = 0;
+  for (uint32_t i = lo + tid; i < hi; i += RS_HT) {
+    const float v = row[i];
+    if (!finite_f(v)) continue;
+    const uint64_t c = composite(v, i);
+    best = c > best ? c : best;
+    cnt++;
+  }
+  best = wave_max_u64(best);
+  cnt = wave_sum_u32(cnt);
+  if ((tid & 63) == 0) { wmax[tid >> 6] = best; wsum[tid >> 6] = cnt; }
+  // this slice's share of the histogram, which k_rows_hist adds to
+  for (uint32_t b = blockIdx.x * RS_HT + tid; b < RS_BINS; b += a.nslices * RS_HT) { h.mass[b] = 0; h.count[b] = 0; }
+  if (blockIdx.x == 0 && tid == 0) h.minp = 0;
+  __syncthreads();
+  if (tid != 0) return;
+  for (uint32_t w = 1; w < RS_HT / 64; w++) { best = wmax[w] > best ? wmax[w] : best; cnt += wsum[w]; }
+  h.slice[blockIdx.x] = RowSlice{best, cnt, 0};
+}
+
+// The row's best composite and finite count, in every thread of a wavefront.
+__device__ __forceinline__ void row_best(const RowsK &a, const RowHist &h, uint64_t *best, uint32_t *finite) {
+  const uint32_t lane = threadIdx.x & 63;
+  const RowSlice s = lane < a.nslices ? h.slice[lane] : RowSlice{0, 0, 0};
+  *best = wave_max_u64(s.best);
+  *finite = wave_sum_u32(s.finite);
+}
+
+// One token's weight into a histogram in LDS: a wavefront whose tokens all share a key adds once.
+__device__ __forceinline__ void hist_add(uint64_t *mass, uint32_t *count, bool ok, uint32_t bin, uint32_t key, uint64_t m) {
+  const uint64_t on = __ballot(ok);
+  if (!on) return;
+  const int first = (int)__ffsll((unsigned long long)on) - 1;
+  const uint32_t bin0 = __shfl(bin, first), key0 = __shfl(key, first);
+  if (__ballot(ok && (bin != bin0 || key != key0)) == 0) {
+    const uint32_t c = (uint32_t)__popcll(on);
+    if ((int)(threadIdx.x & 63) == first) { atomicAdd(&count[bin], c); atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)(m * c)); }
+  } else if (ok) {
+    atomicAdd(&count[bin], 1u);
+    if (m) atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)m);
+  }
+}
+
+__global__ __launch_bounds__(RS_HT) void k_rows_hist(RowsK a) {
+  __shared__ uint64_t mass[RS_BINS];
+  __shared__ uint32_t count[RS_BINS];
+  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const float *row = a.logits + blockIdx.y * a.stride;
+  RowHist &h = a.hist[blockIdx.y];
+  uint64_t best;
+  uint32_t finite;
+  row_best(a, h, &best, &finite);
+  if (!finite) return;
+  const float bv = comp_value(best);
+  for (uint32_t b = tid; b < RS_BINS; b += RS_HT) { mass[b] = 0; count[b] = 0; }
+  __syncthreads();
+  uint64_t minp = 0;
+  for (uint32_t i0 = lo; i0 < hi; i0 += RS_HT) {
+    const uint32_t i = i0 + tid;
+    const float v = i < hi ? row[i] : __uint_as_float(0x7FC00000u);
+    const bool ok = finite_f(v);
+    const double w = ok ? row_weight(a, bv, v) : 0.0;
+    const uint64_t m = row_mass(a, w);
+    if (ok && w >= a.min_p) minp += m;
+    hist_add(mass, count, ok, ok ? row_bin(a, bv, v) : 0, ok ? order_key(v) : 0, m);
+  }
+  __syncthreads();
+  for (uint32_t b = tid; b < RS_BINS; b += RS_HT)
+    if (count[b]) {
+      atomicAdd(&h.count[b], count[b]);
+      atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)mass[b]);
+    }
+  minp = wave_sum_u64(minp);
+  if ((tid & 63) == 0) atomicAdd((unsigned long long *)&h.minp, (unsigned long long)minp);
+}
+
+struct PickLds {
+  uint64_t mass[RS_BINS];
+  uint32_t count[RS_BINS];
+  uint64_t list[RS_CAP], cum[RS_CAP];
+  uint64_t wmass[RS_T / 64];
+  uint32_t wcount[RS_T / 64];
+  uint64_t x_mass;                 // of find_cross: the weight and count before the bin
+  uint32_t x_bin, x_count, nlist, at;
+};
+
+// The first bin at which the running count reaches A or the running weight X, added to count0 and
+// mass0, and both before that bin; bins run from 0, or with `down` from the last. Callers ask only for
+// what the bins hold; without such a bin x_bin stays RS_BINS.
+__device__ __forceinline__ void find_cross(PickLds &L, bool down, uint32_t count0, uint64_t mass0, uint64_t A, uint64_t X) {
+  constexpr uint32_t PER = RS_BINS / RS_T;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  uint32_t c = 0;
+  uint64_t m = 0;
+  auto at = [&](uint32_t e) { return down ? RS_BINS - 1 - (PER * tid + e) : PER * tid + e; };
+  for (uint32_t e = 0; e < PER; e++) { c += L.count[at(e)]; m += L.mass[at(e)]; }
+  uint32_t ci = c;
+  uint64_t mi = m;
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t cw = __shfl_up(ci, o);
+    const uint64_t mw = __shfl_up(mi, o);
+    if ((int)lane >= o) { ci += cw; mi += mw; }
+  }
+  __syncthreads();
+  if (lane == 63) { L.wcount[wv] = ci; L.wmass[wv] = mi; }
+  if (tid == 0) L.x_bin = RS_BINS;
+  __syncthreads();
+  uint64_t cb = (uint64_t)count0 + ci - c, mb = mass0 + mi - m;
+  for (uint32_t w = 0; w < wv; w++) { cb += L.wcount[w]; mb += L.wmass[w]; }
+  for (uint32_t e = 0; e < PER; e++) {
+    const uint64_t c1 = cb + L.count[at(e)], m1 = mb + L.mass[at(e)];
+    if (cb < A && mb < X && (c1 >= A || m1 >= X)) { L.x_bin = at(e); L.x_count = (uint32_t)cb; L.x_mass = mb; }
+    cb = c1; mb = m1;
+  }
+  __syncthreads();
+}
+
+// f(valid, logit, index) over the row, for every thread alike.
+template <class F>
+__device__ __forceinline__ void each_logit(const float *row, uint32_t n, F f) {
+  constexpr uint32_t E = 8;
+  for (uint32_t i0 = 0; i0 < n; i0 += RS_T * E) {
+    float v[E];
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) {
+      const uint32_t i = i0 + e * RS_T + threadIdx.x;
+      v[e] = i < n ? row[i] : __uint_as_float(0x7FC00000u);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) f(finite_f(v[e]), v[e], i0 + e * RS_T + threadIdx.x);
+  }
+}
+
+// The tokens for which pick(logit, index) holds, at most RS_CAP, in descending order in L.list, with
+// their running weights in L.cum.
+template <class Pick>
+__device__ __forceinline__ void gather(const RowsK &a, PickLds &L, const float *row, float bv, Pick pick) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  if (tid == 0) L.nlist = 0;
+  __syncthreads();
+  each_logit(row, a.n, [&](bool ok, float v, uint32_t i) {
+    const bool take = ok && pick(v, i);
+    const uint64_t m = __ballot(take);
+    if (!m) return;
+    uint32_t base = 0;
+    if (lane == 0) base = atomicAdd(&L.nlist, (uint32_t)__popcll(m));
+    base = __shfl(base, 0) + (uint32_t)__popcll(m & ((1ull << lane) - 1));
+    if (take && base < RS_CAP) L.list[base] = composite(v, i);
+  });
+  __syncthreads();
+  const uint32_t nl = min(L.nlist, RS_CAP);
+  uint32_t size = 2;
+  while (size < nl) size <<= 1;
+  for (uint32_t j = nl + tid; j < size; j += RS_T) L.list[j] = 0;
+  for (uint32_t k = 2; k <= size; k <<= 1)  // bitonic, descending
+    for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      for (uint32_t t = tid; t < size / 2; t += RS_T) {
+        const uint32_t i = 2 * t - (t & (j - 1)), p = i + j;
+        const uint64_t x = L.list[i], y = L.list[p];
+        if ((x < y) == ((i & k) == 0)) { L.list[i] = y; L.list[p] = x; }
+      }
+    }
+  __syncthreads();
+  // running weights, two tokens a thread
+  uint64_t m0 = 2 * tid < nl ? row_mass(a, row_weight(a, bv, comp_value(L.list[2 * tid]))) : 0;
+  const uint64_t m1 = 2 * tid + 1 < nl ? row_mass(a, row_weight(a, bv, comp_value(L.list[2 * tid + 1]))) : 0;
+  uint64_t incl = m0 + m1;
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t w = __shfl_up(incl, o);
+    if ((int)lane >= o) incl += w;
+  }
+  if (lane == 63) L.wmass[wv] = incl;
+  __syncthreads();
+  for (uint32_t w = 0; w < wv; w++) incl += L.wmass[w];
+  L.cum[2 * tid] = incl - m1;
+  L.cum[2 * tid + 1] = incl;
+  __syncthreads();
+}
+
+// The place in L.list at which the running count (1 for the first) reaches A or mass0 and the running
+// weight reach X; the last place if none does.
+__device__ __forceinline__ uint32_t find_place(PickLds &L, uint64_t mass0, uint64_t A, uint64_t X) {
+  const uint32_t nl = min(L.nlist, RS_CAP);
+  __syncthreads();
+  if (threadIdx.x == 0) L.at = nl - 1;
+  __syncthreads();
+  for (uint32_t j = threadIdx.x; j < nl; j += RS_T)
+    if (j + 1 >= A || mass0 + L.cum[j] >= X) { atomicMin(&L.at, j); break; }
+  __syncthreads();
+  return L.at;
+}
+
+__device__ __forceinline__ void load_hist(PickLds &L, const RowHist &h) {
+  __syncthreads();
+  for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) { L.mass[b] = h.mass[b]; L.count[b] = h.count[b]; }
+  __syncthreads();
+}
+
+// The first token of the row whose running count reaches A or whose running weight reaches X: its
+// composite, and the weight up to and with it.
+__device__ __forceinline__ uint64_t first_token(const RowsK &a, PickLds &L, const RowHist &h, const float *row, float bv,
+                                                uint64_t A, uint64_t X, uint64_t *mass) {
+  load_hist(L, h);
+  find_cross(L, false, 0, 0, A, X);
+  const uint32_t bin = L.x_bin;
+  uint32_t before = L.x_count, inside = L.count[bin < RS_BINS ? bin : 0];
+  uint64_t mbefore = L.x_mass, prefix = 0, hi_mask = 0;
+  uint32_t shift = 64;
+  while (inside > RS_CAP && shift > 0) {
+    const uint32_t next = shift >= 12 ? shift - 12 : 0, fmask = (1u << (shift - next)) - 1;
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) { L.mass[b] = 0; L.count[b] = 0; }
+    __syncthreads();
+    each_logit(row, a.n, [&](bool ok, float v, uint32_t i) {
+      const uint64_t c = composite(v, i);
+      ok = ok && row_bin(a, bv, v) == bin && (c & hi_mask) == prefix;
+      hist_add(L.mass, L.count, ok, (uint32_t)(c >> next) & fmask, order_key(v), ok ? row_mass(a, row_weight(a, bv, v)) : 0);
+    });
+    __syncthreads();
+    find_cross(L, true, before, mbefore, A, X);
+    before = L.x_count;
+    mbefore = L.x_mass;
+    inside = L.count[L.x_bin < RS_BINS ? L.x_bin : 0];
+    prefix |= (uint64_t)L.x_bin << next;
+    hi_mask = ~((1ull << next) - 1);
+    shift = next;
+    __syncthreads();
+  }
+  gather(a, L, row, bv, [&](float v, uint32_t i) {
+    return row_bin(a, bv, v) == bin && (composite(v, i) & hi_mask) == prefix;
+  });
+  const uint32_t at = find_place(L, mbefore, A > before ? A - before : 1, X);
+  *mass = mbefore + L.cum[at];
+  return L.list[at];
+}
+
+__global__ __launch_bounds__(RS_T) void k_rows_pick(RowsK a) {
+  extern __shared__ uint64_t pick_lds[];
+  PickLds &L = *(PickLds *)pick_lds;
+  const float *row = a.logits + blockIdx.x * a.stride;
+  const RowHist &h = a.hist[blockIdx.x];
+  constexpr uint64_t ALL = ~0ull;
+  uint64_t best;
+  uint32_t finite;
+  row_best(a, h, &best, &finite);
+  const double u = a.uniforms[blockIdx.x];
+  if (!finite || a.temperature == 0.0 || a.top_k == 1 || !(u > 0.0 && u < 1.0)) {
+    if (threadIdx.x == 0) a.tokens[blockIdx.x] = finite ? (int32_t)comp_index(best) : -1;
+    return;
+  }
+  const float bv = comp_value(best);
+  const uint32_t K = a.top_k && a.top_k < finite ? a.top_k : finite;
+  auto at_least = [](double x, uint64_t most) { return min(max((uint64_t)ceil(x), (uint64_t)1), most); };
+  load_hist(L, h);
+  uint64_t S = 0;  // the weight of the first K
+  bool listed = false;
+  if (K < finite) {
+    find_cross(L, false, 0, 0, K, ALL);
+    const uint32_t bin = L.x_bin;
+    if (L.x_count + L.count[bin] <= RS_CAP) {
+      gather(a, L, row, bv, [&](float v, uint32_t) { return row_bin(a, bv, v) <= bin; });
+      listed = true;
+      S = L.cum[K - 1];
+    } else {
+      first_token(a, L, h, row, bv, K, ALL, &S);
+    }
+  } else {
+    uint64_t m = 0;
+    for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) m += L.mass[b];
+    m = wave_sum_u64(m);
+    if ((threadIdx.x & 63) == 0) L.wmass[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (uint32_t w = 0; w < RS_T / 64; w++) S += L.wmass[w];
+    __syncthreads();
+  }
+  const uint64_t X = a.top_p < 1.0 ? at_least(a.top_p * (double)S, S) : S;
+  if (!listed && a.top_p < 1.0) {
+    load_hist(L, h);
+    find_cross(L, false, 0, 0, ALL, X);
+    const uint32_t bin = L.x_bin;
+    if (bin < RS_BINS && L.x_count + L.count[bin] <= RS_CAP) {
+      gather(a, L, row, bv, [&](float v, uint32_t) { return row_bin(a, bv, v) <= bin; });
+      listed = true;
+    }
+  }
+  uint64_t R = S, token;
+  if (listed) {
+    if (a.top_p < 1.0) R = L.cum[find_place(L, 0, ALL, X)];
+    R = min(R, h.minp);
+    token = L.list[find_place(L, 0, ALL, at_least(u * (double)R, R))];
+  } else {
+    if (a.top_p < 1.0) first_token(a, L, h, row, bv, ALL, X, &R);
+    R = min(R, h.minp);
+    uint64_t unused;
+    token = first_token(a, L, h, row, bv, ALL, at_least(u * (double)R, R), &unused);
+  }
+  if (threadIdx.x == 0) a.tokens[blockIdx.x] = (int32_t)comp_index(token);
+}
+
+uint64_t sample_rows_scratch_bytes(const SampleRowsArgs &a) { return (uint64_t)std::min(a.rows, RS_ROWS) * sizeof(RowHist); }
+
+hipError_t sample_rows(hipStream_t s, const SampleRowsArgs &in) {
+  if (!in.rows) return hipSuccess;
+  if (!in.n || !in.scratch || in.stride < in.n) return hipErrorInvalidValue;
+  RowsK a{};
+  a.n = in.n; a.stride = in.stride;
+  a.slice = std::max(RS_MIN, (in.n + RS_SLICES - 1) / RS_SLICES);
+  a.nslices = (in.n + a.slice - 1) / a.slice;
+  a.hist = (RowHist *)in.scratch;
+  a.temperature = in.temperature; a.top_p = in.top_p; a.min_p = in.min_p; a.top_k = in.top_k;
+  int log2n = 0;
+  while (log2n < 32 && (1ull << log2n) < in.n) log2n++;
+  a.unit = std::ldexp(1.0, 62 - log2n);
+  // a temperature near 0 has no finite scale: any large one keeps the bins monotonic
+  a.bins = in.temperature > 0.0 ? (float)std::min(1e30, RS_BINS / (RS_SPAN * in.temperature)) : 0.f;
+  lds_opt_in((const void *)k_rows_pick);
+  for (uint32_t r0 = 0; r0 < in.rows; r0 += RS_ROWS) {
+    const uint32_t nr = std::min(RS_ROWS, in.rows - r0);
+    a.logits = in.logits + (uint64_t)r0 * in.stride; a.uniforms = in.uniforms + r0; a.tokens = in.tokens + r0;
+    hipLaunchKernelGGL(k_rows_best, dim3(a.nslices, nr), dim3(RS_HT), 0, s, a);
+    WGD_HIP(hipGetLastError());
+    if (in.temperature != 0.0 && in.top_k != 1) {
+      hipLaunchKernelGGL(k_rows_hist, dim3(a.nslices, nr), dim3(RS_HT), 0, s, a);
+      WGD_HIP(hipGetLastError());
+    }
+    hipLaunchKernelGGL(k_rows_pick, dim3(nr), dim3(RS_T), sizeof(PickLds), s, a);
+    WGD_HIP(hipGetLastError());
+  }
+  return hipSuccess;
 }
 
 }  // namespace wgd

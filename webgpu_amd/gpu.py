@@ -31,6 +31,7 @@ SIGNATURES = {
     "wgd_buffer_create": (C.c_int, [_P, _U64, C.c_char_p, C.POINTER(_P)]),
     "wgd_buffer_destroy": (C.c_int, [_P, _P]),
     "wgd_buffer_size": (_U64, [_P]),
+    "wgd_buffer_address": (_P, [_P]),
     "wgd_upload_weights": (C.c_int, [_P, _I32, _U32, _U32, _P, _U64, C.c_char_p, C.POINTER(_P)]),
     "wgd_stream": (_P, [_P]),
     "wgd_write": (C.c_int, [_P, _P, _U64, _P, _U64]),
@@ -53,6 +54,12 @@ SIGNATURES = {
     "wgd_attention_noalloc_limit": (_U64, []),
     "wgd_attention_f16kv": (C.c_int, [_P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _F, _U32, _U32, _U32, _U32]),
     "wgd_kv_store_f16": (C.c_int, [_P, _P, _P, _U64, _U64, _U64]),
+    "wgd_rope_at": (C.c_int, [_P, _P, _P, _P, _U32, _U32, _F, _F, _F, _U32, _U32, _U64, _I32, _U32]),
+    "wgd_attention_tree": (C.c_int, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _F, _U32, _U32, _U32]),
+    "wgd_attention_tree_f16kv": (C.c_int, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _F, _U32, _U32, _U32]),
+    "wgd_sample_rows": (C.c_int, [_P, _P, _U32, _U32, _U32, _P, _P, _D, _U32, _D, _D]),
+    "wgd_tree_accept": (C.c_int, [_P, _P, _P, _P, _P, _U32]),
+    "wgd_kv_commit": (C.c_int, [_P, C.POINTER(_P), _U32, _P, _U64, _U32, _U32, _U32]),
     "wgd_probe_read": (C.c_int, [_P, _P, _U64, _U32, _U32, _U32, _U32, _U32, _P, _U32]),
     "wgd_add": (C.c_int, [_P, _P, _P, _U32]),
     "wgd_silu": (C.c_int, [_P, _P, _P, _P, _U32]),
@@ -185,6 +192,11 @@ class Compute:
                                             C.byref(out)))
         return Buffer(out.value, lib().wgd_buffer_size(out.value), label)
 
+    def address(self, b: Buffer) -> int:
+        """The device address of a buffer, for device code of the host's own (ordered against
+        ``stream``) that fills or reads it."""
+        return lib().wgd_buffer_address(b.ptr) or 0
+
     @property
     def stream(self) -> int:
         return lib().wgd_stream(self.ctx)
@@ -309,6 +321,43 @@ class Compute:
         self.check(lib().wgd_sample(self.ctx, logits.ptr, n, float(temperature), int(top_k), float(top_p),
                                     int(seed) & (2 ** 64 - 1), int(index), C.byref(tok)))
         return tok.value
+
+    # -- drafted trees (include/wgd.h) ------------------------------------------------
+    def rope_at(self, x: Buffer, positions: Buffer, heads: int, hd: int, theta: float, scale: float, rotary_dim: int,
+                batch: int = 1, adjacent: bool = False, factors: Optional[Buffer] = None, magnitude: float = 1.0,
+                stride: int = 0, offset: int = 0) -> None:
+        """Rotary embedding in place at positions[t] (int32) per token; ``factors`` divide the
+        frequencies pair by pair (``webgpu_amd.rope``)."""
+        self.check(lib().wgd_rope_at(self.ctx, x.ptr, positions.ptr, factors.ptr if factors is not None else None, heads,
+                                     hd, theta, scale, magnitude, rotary_dim, stride, offset, int(adjacent), batch))
+
+    def attention_tree(self, q: Buffer, k: Buffer, v: Buffer, y: Buffer, parents: Buffer, heads: int, kv_heads: int,
+                       hd: int, start: int, scale: float, window: int, capacity: int, nodes: int) -> None:
+        """Attention of a tree of drafted nodes over the cached keys and their own ancestors."""
+        self.check(lib().wgd_attention_tree(self.ctx, q.ptr, k.ptr, v.ptr, y.ptr, parents.ptr, heads, kv_heads, hd,
+                                            start, scale, window, capacity, nodes))
+
+    def attention_tree_f16kv(self, q: Buffer, k: Buffer, v: Buffer, y: Buffer, parents: Buffer, heads: int,
+                             kv_heads: int, hd: int, start: int, scale: float, window: int, capacity: int,
+                             nodes: int) -> None:
+        """attention_tree() over K/V rings of f16 elements."""
+        self.check(lib().wgd_attention_tree_f16kv(self.ctx, q.ptr, k.ptr, v.ptr, y.ptr, parents.ptr, heads, kv_heads,
+                                                  hd, start, scale, window, capacity, nodes))
+
+    def sample_rows(self, logits: Buffer, n: int, rows: int, uniforms: Buffer, tokens: Buffer, temperature: float,
+                    top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, stride: int = 0) -> None:
+        """One token per row of logits with the caller's uniforms (f64), into tokens (int32)."""
+        self.check(lib().wgd_sample_rows(self.ctx, logits.ptr, n, rows, stride, uniforms.ptr, tokens.ptr,
+                                         float(temperature), int(top_k), float(top_p), float(min_p)))
+
+    def tree_accept(self, parents: Buffer, drafted: Buffer, picked: Buffer, path: Buffer, nodes: int) -> None:
+        """The drafted path that the picked tokens confirm: path = [count, next token, nodes..., -1...]."""
+        self.check(lib().wgd_tree_accept(self.ctx, parents.ptr, drafted.ptr, picked.ptr, path.ptr, nodes))
+
+    def kv_commit(self, rings, path: Buffer, row_bytes: int, start: int, capacity: int, nodes: int) -> None:
+        """Moves the path's rows of every ring (K and V of any layers) to the slots they keep."""
+        ptrs = (C.c_void_p * max(1, len(rings)))(*[r.ptr for r in rings])
+        self.check(lib().wgd_kv_commit(self.ctx, ptrs, len(rings), path.ptr, row_bytes, start, capacity, nodes))
 
     def embed(self, type_: int, table: Buffer, ids: Buffer, out: Buffer, hidden: int, n: int, scale: float = 1.0) -> None:
         self.check(lib().wgd_embed(self.ctx, type_, table.ptr, ids.ptr, out.ptr, hidden, n, scale))
