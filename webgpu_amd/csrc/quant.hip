@@ -338,12 +338,13 @@ int device_cu_count() {
   return g_cus;
 }
 
-void lds_opt_in(const void *kernel) {
+void lds_opt_in(const void *kernel) { lds_opt_in_bytes(kernel, LDS_MAX); }
+void lds_opt_in_bytes(const void *kernel, uint32_t bytes) {
   static std::mutex mu;
   static std::unordered_set<const void *> done;
   std::lock_guard<std::mutex> lock(mu);
   if (done.insert(kernel).second)
-    (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS_MAX);
+    (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
 hipError_t matmul(hipStream_t s, const Matrix &w, const float *x, float *y, uint32_t stride,
