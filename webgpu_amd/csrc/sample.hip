@@ -457,74 +457,124 @@ hipError_t sample(hipStream_t s, const float *logits, uint32_t n, const SamplePa
 
 // ------------------------------------------------------------------ rows with given uniforms
 //
-// wgd_sample_rows: for every row the finite logits in descending order (composites, as above)
-// have the weights w = exp((l - best) / T) in f64, rounded to integers of 2^-shift with shift = 62 -
-// ceil(log2 n): their sums fit 64 bits, are exact, and do not depend on the order of the adds,
-// so atomics give the same token every time. A top-k, top-p or min-p cut and the draw itself are all
-// "the first token whose running count reaches A or whose running sum reaches X". Three launches:
-//   * k_rows_best (slices x rows): the slices' best composites and finite counts;
-//   * k_rows_hist (slices x rows): counts and weights over RS_BINS bins of (best - l) / T, which is
-//     monotonic in l, and the weight that min-p keeps;
-//   * k_rows_pick (a workgroup a row): the bin of each cut from the running histogram, then its tokens
-//     gathered, sorted and summed in LDS. A bin with more tokens than LDS holds (ties, logits far below the
-//     temperature's scale) is refined by 12 bits of the composite at a time.
-constexpr uint32_t RS_T = 1024, RS_BINS = 4096, RS_CAP = 2048;
-constexpr uint32_t RS_HT = 256, RS_SLICES = 64, RS_MIN = 2048;  // slice kernels: threads, slices, slice floor
+// wgd_sample_rows: for every row the finite logits in descending order (composites, as above) have the
+// weights w = exp((l - best) / T) in f64, rounded to integers of 2^-shift with shift = 62 - ceil(log2 n): their sums fit
+// 64 bits, are exact, and do not depend on the order of the adds, so atomics give the same token every time.
+// A top-k, top-p or min-p cut and the draw itself are all "the first token whose running count reaches A or whose
+// running weight reaches X". Two ways, by top_k alone:
+//
+// Few (2 <= top_k <= RS_FEW and half the row's groups, or a row that fits a list), two launches or one:
+//   * k_rows_groups reads the row once and leaves the largest key of every group of 16 to 128 logits;
+//   * k_rows_few, a workgroup a row: the bin (below) that holds the top_k-th largest of those keys bounds the bin of the
+//     top_k-th largest logit (top_k logits reach it). Only groups that reach it are read again; of their
+//     logits little more than top_k do, which are sorted and summed in LDS. A row of at most RS_CAP logits is one list.
+// Many (top_k 0 or above), four to six launches, each a pass over the rows by all CUs:
+//   * k_rows_best: the best composite and the count of finite logits, by slices;
+//   * k_rows_hist: counts and weights over RS_BINS bins of (best - l) / T, which is monotonic in l;
+//   * k_rows_stage for each of the cuts that there are (top-k, top-p) and the draw: the bin that holds the cut's token,
+//     from the running histogram, and that bin's tokens into a list; the cut before it, from its list;
+//   * k_rows_last: the token from the draw's list.
+// A cut's token is found in its list by a histogram of RS_SUB parts of the bin and a sort of the one part
+// that holds it (a sort of the whole list took four times as long).
+// A bin or bound with more tokens than a list holds (ties, logits close together for the temperature) goes through
+// pick_row, which refines by 12 bits of the composite at a time, in one workgroup.
+constexpr uint32_t RS_T = 512, RS_BINS = 2048, RS_CAP = 2048, RS_SUB = 1024;
 constexpr uint32_t RS_ROWS = 256;  // rows per launch: the histograms of more would only fill memory
 constexpr float RS_SPAN = 48.f;    // bins cover exp(0) to exp(-48) < 2^-62; the last one all below
+constexpr uint32_t RS_SLICES = 64, RS_SLICE = 16384;  // most slices of a row, least logits of one
+constexpr uint32_t RS_FEW = 512, RS_GROUPS = 2048;   // top_k by groups; most groups of a row
+constexpr uint32_t RG_T = 256, RG_STEP = 256;        // k_rows_groups: threads; logits of a wavefront's step
+enum RowCut : uint32_t { CUT_K = 0, CUT_P = 1, CUT_DRAW = 2, CUT_NONE = 3 };
 
 struct RowSlice { uint64_t best; uint32_t finite, pad; };
 struct RowHist {
   uint64_t mass[RS_BINS];
   uint32_t count[RS_BINS];
-  uint64_t minp;
+  uint64_t list[3][RS_CAP];
+  uint32_t nlist[3], slow[3];  // slow: a cut's bin holds more than its list
+  uint64_t minp, s, target;
   RowSlice slice[RS_SLICES];
 };
+struct RowGroups { uint32_t key[RS_GROUPS]; };
+
 struct RowsK {
   const float *logits; uint32_t n, slice, nslices; uint64_t stride;
-  const double *uniforms; int32_t *tokens; RowHist *hist;
-  double temperature, top_p, min_p, unit;  // unit: 2^shift
-  float bins;                              // bins per unit of logit
-  uint32_t top_k;
+  const double *uniforms; int32_t *tokens; RowHist *hist; RowGroups *groups;
+  double inv_t, top_p, min_p, unit;  // 1 / temperature; unit: 2^shift
+  float bins;                        // bins per unit of logit
+  uint32_t top_k, steps, ngroups, aligned;
 };
 
 __device__ __forceinline__ uint32_t row_bin(const RowsK &a, float best, float l) {
   return (uint32_t)fminf((best - l) * a.bins, (float)(RS_BINS - 1));
 }
-__device__ __forceinline__ double row_weight(const RowsK &a, float best, float l) {
-  return exp(((double)l - (double)best) / a.temperature);
-}
+__device__ __forceinline__ double row_weight(const RowsK &a, float best, float l) { return exp(((double)l - (double)best) * a.inv_t); }
 __device__ __forceinline__ uint64_t row_mass(const RowsK &a, double w) { return (uint64_t)(w * a.unit + 0.5); }
 __device__ __forceinline__ uint64_t composite(float l, uint32_t i) { return ((uint64_t)order_key(l) << 32) | (0xFFFFFFFFu - i); }
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
+__device__ __forceinline__ float wave_max_f(float v) {
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+// At least x and 1, at most `most`.
+__device__ __forceinline__ uint64_t at_least(double x, uint64_t most) { return min(max((uint64_t)ceil(x), (uint64_t)1), most); }
 
-__global__ __launch_bounds__(RS_HT) void k_rows_best(RowsK a) {
-  __shared__ uint64_t wmax[RS_HT / 64];
-  __shared__ uint32_t wsum[RS_HT / 64];
-  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
-  const float *row = a.logits + blockIdx.y * a.stride;
-  RowHist &h = a.hist[blockIdx.y];
-  uint64_t best = 0;
-  uint32_t cnt = 0;
-  for (uint32_t i = lo + tid; i < hi; i += RS_HT) {
-    const float v = row[i];
-    if (!finite_f(v)) continue;
-    const uint64_t c = composite(v, i);
-    best = c > best ? c : best;
-    cnt++;
+// Logits i .. i + 4 of a row of n, NaN past its end; 16 bytes at once where every row starts on 16.
+__device__ __forceinline__ float4 row_load4(const RowsK &a, const float *row, uint32_t i) {
+  const float none = __uint_as_float(0x7FC00000u);
+  if (a.aligned && i + 4 <= a.n) return *(const float4 *)(row + i);
+  return make_float4(i < a.n ? row[i] : none, i + 1 < a.n ? row[i + 1] : none, i + 2 < a.n ? row[i + 2] : none,
+                     i + 3 < a.n ? row[i + 3] : none);
+}
+// f(finite, logit, index) over the logits [lo, hi) (lo a multiple of 4), for every thread of T alike.
+template <uint32_t T, class F>
+__device__ __forceinline__ void each_logit(const RowsK &a, const float *row, uint32_t lo, uint32_t hi, F f) {
+  constexpr uint32_t E = 4;
+  for (uint32_t i0 = lo; i0 < hi; i0 += 4 * T * E) {
+    float4 v[E];
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) {
+      const uint32_t i = i0 + 4 * (e * T + threadIdx.x);
+      v[e] = i < hi ? row_load4(a, row, i) : make_float4(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) {
+      const uint32_t i = i0 + 4 * (e * T + threadIdx.x);
+      f(finite_f(v[e].x) && i < hi, v[e].x, i);
+      f(finite_f(v[e].y) && i + 1 < hi, v[e].y, i + 1);
+      f(finite_f(v[e].z) && i + 2 < hi, v[e].z, i + 2);
+      f(finite_f(v[e].w) && i + 3 < hi, v[e].w, i + 3);
+    }
   }
-  best = wave_max_u64(best);
+}
+
+__global__ __launch_bounds__(256) void k_rows_best(RowsK a) {
+  __shared__ uint64_t wmax[4];
+  __shared__ uint32_t wsum[4];
+  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  RowHist &h = a.hist[blockIdx.y];
+  float top = -INFINITY;
+  uint32_t at = 0, cnt = 0;
+  // a thread meets its logits in order: the first of equal ones stays
+  each_logit<256>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t i) {
+    cnt += ok;
+    if (ok && (v > top || cnt == 1)) { top = v; at = i; }
+  });
+  uint64_t best = wave_max_u64(cnt ? composite(top, at) : 0);
   cnt = wave_sum_u32(cnt);
   if ((tid & 63) == 0) { wmax[tid >> 6] = best; wsum[tid >> 6] = cnt; }
-  // this slice's share of the histogram, which k_rows_hist adds to
-  for (uint32_t b = blockIdx.x * RS_HT + tid; b < RS_BINS; b += a.nslices * RS_HT) { h.mass[b] = 0; h.count[b] = 0; }
-  if (blockIdx.x == 0 && tid == 0) h.minp = 0;
+  // this slice's share of what the launches behind it add to
+  for (uint32_t b = blockIdx.x * 256 + tid; b < RS_BINS; b += a.nslices * 256) { h.mass[b] = 0; h.count[b] = 0; }
+  if (blockIdx.x == 0 && tid == 0) {
+    h.minp = 0;
+    for (int e = 0; e < 3; e++) h.nlist[e] = h.slow[e] = 0;
+  }
   __syncthreads();
   if (tid != 0) return;
-  for (uint32_t w = 1; w < RS_HT / 64; w++) { best = wmax[w] > best ? wmax[w] : best; cnt += wsum[w]; }
+  for (uint32_t w = 1; w < 4; w++) { best = wmax[w] > best ? wmax[w] : best; cnt += wsum[w]; }
   h.slice[blockIdx.x] = RowSlice{best, cnt, 0};
 }
 
@@ -537,6 +587,8 @@ __device__ __forceinline__ void row_best(const RowsK &a, const RowHist &h, uint6
 }
 
 // One token's weight into a histogram in LDS: a wavefront whose tokens all share a key adds once.
+// COUNT: counts too.
+template <bool COUNT>
 __device__ __forceinline__ void hist_add(uint64_t *mass, uint32_t *count, bool ok, uint32_t bin, uint32_t key, uint64_t m) {
   const uint64_t on = __ballot(ok);
   if (!on) return;
@@ -544,50 +596,53 @@ __device__ __forceinline__ void hist_add(uint64_t *mass, uint32_t *count, bool o
   const uint32_t bin0 = __shfl(bin, first), key0 = __shfl(key, first);
   if (__ballot(ok && (bin != bin0 || key != key0)) == 0) {
     const uint32_t c = (uint32_t)__popcll(on);
-    if ((int)(threadIdx.x & 63) == first) { atomicAdd(&count[bin], c); atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)(m * c)); }
+    if ((int)(threadIdx.x & 63) == first) {
+      if (COUNT) atomicAdd(&count[bin], c);
+      atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)(m * c));
+    }
   } else if (ok) {
-    atomicAdd(&count[bin], 1u);
+    if (COUNT) atomicAdd(&count[bin], 1u);
     if (m) atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)m);
   }
 }
 
-__global__ __launch_bounds__(RS_HT) void k_rows_hist(RowsK a) {
+template <bool COUNT>
+__global__ __launch_bounds__(RS_T) void k_rows_hist(RowsK a) {
   __shared__ uint64_t mass[RS_BINS];
-  __shared__ uint32_t count[RS_BINS];
+  __shared__ uint32_t count[COUNT ? RS_BINS : 1];
   const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
-  const float *row = a.logits + blockIdx.y * a.stride;
   RowHist &h = a.hist[blockIdx.y];
   uint64_t best;
   uint32_t finite;
   row_best(a, h, &best, &finite);
   if (!finite) return;
   const float bv = comp_value(best);
-  for (uint32_t b = tid; b < RS_BINS; b += RS_HT) { mass[b] = 0; count[b] = 0; }
+  for (uint32_t b = tid; b < RS_BINS; b += RS_T) {
+    mass[b] = 0;
+    if (COUNT) count[b] = 0;
+  }
   __syncthreads();
   uint64_t minp = 0;
-  for (uint32_t i0 = lo; i0 < hi; i0 += RS_HT) {
-    const uint32_t i = i0 + tid;
-    const float v = i < hi ? row[i] : __uint_as_float(0x7FC00000u);
-    const bool ok = finite_f(v);
+  each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t) {
     const double w = ok ? row_weight(a, bv, v) : 0.0;
     const uint64_t m = row_mass(a, w);
     if (ok && w >= a.min_p) minp += m;
-    hist_add(mass, count, ok, ok ? row_bin(a, bv, v) : 0, ok ? order_key(v) : 0, m);
-  }
+    hist_add<COUNT>(mass, count, ok, ok ? row_bin(a, bv, v) : 0, ok ? order_key(v) : 0, m);
+  });
   __syncthreads();
-  for (uint32_t b = tid; b < RS_BINS; b += RS_HT)
-    if (count[b]) {
-      atomicAdd(&h.count[b], count[b]);
-      atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)mass[b]);
-    }
+  for (uint32_t b = tid; b < RS_BINS; b += RS_T) {
+    if (COUNT && count[b]) atomicAdd(&h.count[b], count[b]);
+    if (mass[b]) atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)mass[b]);
+  }
   minp = wave_sum_u64(minp);
-  if ((tid & 63) == 0) atomicAdd((unsigned long long *)&h.minp, (unsigned long long)minp);
+  if ((tid & 63) == 0 && minp) atomicAdd((unsigned long long *)&h.minp, (unsigned long long)minp);
 }
 
 struct PickLds {
   uint64_t mass[RS_BINS];
   uint32_t count[RS_BINS];
   uint64_t list[RS_CAP], cum[RS_CAP];
+  uint64_t part[RS_CAP];           // one part of a bin's tokens; tokens on their way to a list
   uint64_t wmass[RS_T / 64];
   uint32_t wcount[RS_T / 64];
   uint64_t x_mass;                 // of find_cross: the weight and count before the bin
@@ -597,12 +652,13 @@ struct PickLds {
 // The first bin at which the running count reaches A or the running weight X, added to count0 and
 // mass0, and both before that bin; bins run from 0, or with `down` from the last. Callers ask only for
 // what the bins hold; without such a bin x_bin stays RS_BINS.
+template <uint32_t BINS = RS_BINS>
 __device__ __forceinline__ void find_cross(PickLds &L, bool down, uint32_t count0, uint64_t mass0, uint64_t A, uint64_t X) {
-  constexpr uint32_t PER = RS_BINS / RS_T;
+  constexpr uint32_t PER = BINS / RS_T;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   uint32_t c = 0;
   uint64_t m = 0;
-  auto at = [&](uint32_t e) { return down ? RS_BINS - 1 - (PER * tid + e) : PER * tid + e; };
+  auto at = [&](uint32_t e) { return down ? BINS - 1 - (PER * tid + e) : PER * tid + e; };
   for (uint32_t e = 0; e < PER; e++) { c += L.count[at(e)]; m += L.mass[at(e)]; }
   uint32_t ci = c;
   uint64_t mi = m;
@@ -625,57 +681,44 @@ __device__ __forceinline__ void find_cross(PickLds &L, bool down, uint32_t count
   __syncthreads();
 }
 
-// f(valid, logit, index) over the row, for every thread alike.
-template <class F>
-__device__ __forceinline__ void each_logit(const float *row, uint32_t n, F f) {
-  constexpr uint32_t E = 8;
-  for (uint32_t i0 = 0; i0 < n; i0 += RS_T * E) {
-    float v[E];
-#pragma unroll
-    for (uint32_t e = 0; e < E; e++) {
-      const uint32_t i = i0 + e * RS_T + threadIdx.x;
-      v[e] = i < n ? row[i] : __uint_as_float(0x7FC00000u);
+// L.list[0 .. L.nlist) (at most RS_CAP) in descending order, and its running weights in L.cum. Up to RS_RANK tokens are
+// placed by the count of larger ones, without a barrier per step.
+constexpr uint32_t RS_RANK = 256;
+__device__ __forceinline__ void sort_list(const RowsK &a, PickLds &L, float bv) {
+  constexpr uint32_t PER = RS_CAP / RS_T;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, nl = min(L.nlist, RS_CAP);
+  if (nl <= RS_RANK) {
+    uint64_t mine = 0;
+    uint32_t rank = 0;
+    if (tid < nl) {
+      mine = L.list[tid];
+#pragma unroll 8
+      for (uint32_t j = 0; j < nl; j++) rank += L.list[j] > mine ? 1u : 0u;
     }
-#pragma unroll
-    for (uint32_t e = 0; e < E; e++) f(finite_f(v[e]), v[e], i0 + e * RS_T + threadIdx.x);
-  }
-}
-
-// The tokens for which pick(logit, index) holds, at most RS_CAP, in descending order in L.list, with
-// their running weights in L.cum.
-template <class Pick>
-__device__ __forceinline__ void gather(const RowsK &a, PickLds &L, const float *row, float bv, Pick pick) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  if (tid == 0) L.nlist = 0;
-  __syncthreads();
-  each_logit(row, a.n, [&](bool ok, float v, uint32_t i) {
-    const bool take = ok && pick(v, i);
-    const uint64_t m = __ballot(take);
-    if (!m) return;
-    uint32_t base = 0;
-    if (lane == 0) base = atomicAdd(&L.nlist, (uint32_t)__popcll(m));
-    base = __shfl(base, 0) + (uint32_t)__popcll(m & ((1ull << lane) - 1));
-    if (take && base < RS_CAP) L.list[base] = composite(v, i);
-  });
-  __syncthreads();
-  const uint32_t nl = min(L.nlist, RS_CAP);
-  uint32_t size = 2;
-  while (size < nl) size <<= 1;
-  for (uint32_t j = nl + tid; j < size; j += RS_T) L.list[j] = 0;
-  for (uint32_t k = 2; k <= size; k <<= 1)  // bitonic, descending
-    for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      for (uint32_t t = tid; t < size / 2; t += RS_T) {
-        const uint32_t i = 2 * t - (t & (j - 1)), p = i + j;
-        const uint64_t x = L.list[i], y = L.list[p];
-        if ((x < y) == ((i & k) == 0)) { L.list[i] = y; L.list[p] = x; }
+    __syncthreads();
+    if (tid < nl) L.list[rank] = mine;
+  } else {
+    uint32_t size = 2;
+    while (size < nl) size <<= 1;
+    for (uint32_t j = nl + tid; j < size; j += RS_T) L.list[j] = 0;
+    for (uint32_t k = 2; k <= size; k <<= 1)  // bitonic
+      for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+        __syncthreads();
+        for (uint32_t t = tid; t < size / 2; t += RS_T) {
+          const uint32_t i = 2 * t - (t & (j - 1)), p = i + j;
+          const uint64_t x = L.list[i], y = L.list[p];
+          if ((x < y) == ((i & k) == 0)) { L.list[i] = y; L.list[p] = x; }
+        }
       }
-    }
+  }
   __syncthreads();
-  // running weights, two tokens a thread
-  uint64_t m0 = 2 * tid < nl ? row_mass(a, row_weight(a, bv, comp_value(L.list[2 * tid]))) : 0;
-  const uint64_t m1 = 2 * tid + 1 < nl ? row_mass(a, row_weight(a, bv, comp_value(L.list[2 * tid + 1]))) : 0;
-  uint64_t incl = m0 + m1;
+  uint64_t m[PER], incl = 0;
+#pragma unroll
+  for (uint32_t e = 0; e < PER; e++) {
+    const uint32_t j = PER * tid + e;
+    m[e] = j < nl ? row_mass(a, row_weight(a, bv, comp_value(L.list[j]))) : 0;
+    incl += m[e];
+  }
   for (int o = 1; o < 64; o <<= 1) {
     const uint64_t w = __shfl_up(incl, o);
     if ((int)lane >= o) incl += w;
@@ -683,8 +726,11 @@ __device__ __forceinline__ void gather(const RowsK &a, PickLds &L, const float *
   if (lane == 63) L.wmass[wv] = incl;
   __syncthreads();
   for (uint32_t w = 0; w < wv; w++) incl += L.wmass[w];
-  L.cum[2 * tid] = incl - m1;
-  L.cum[2 * tid + 1] = incl;
+#pragma unroll
+  for (int e = (int)PER - 1; e >= 0; e--) {
+    L.cum[PER * tid + e] = incl;
+    incl -= m[e];
+  }
   __syncthreads();
 }
 
@@ -706,6 +752,66 @@ __device__ __forceinline__ void load_hist(PickLds &L, const RowHist &h) {
   for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) { L.mass[b] = h.mass[b]; L.count[b] = h.count[b]; }
   __syncthreads();
 }
+// The sum of the histogram's weights.
+__device__ __forceinline__ uint64_t hist_mass(PickLds &L) {
+  uint64_t m = 0, s = 0;
+  for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) m += L.mass[b];
+  m = wave_sum_u64(m);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) L.wmass[threadIdx.x >> 6] = m;
+  __syncthreads();
+  for (uint32_t w = 0; w < RS_T / 64; w++) s += L.wmass[w];
+  __syncthreads();
+  return s;
+}
+
+// Appends the wavefront's tokens for which `take` holds to a list with room for RS_CAP; the count goes on past it.
+__device__ __forceinline__ void append(uint64_t *list, uint32_t *nlist, bool take, uint64_t c) {
+  const uint64_t m = __ballot(take);
+  if (!m) return;
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t base = 0;
+  if (lane == 0) base = atomicAdd(nlist, (uint32_t)__popcll(m));
+  base = __shfl(base, 0) + (uint32_t)__popcll(m & ((1ull << lane) - 1));
+  if (take && base < RS_CAP) list[base] = c;
+}
+
+// The first of the n tokens in L.part (one bin's, in any order) whose running count, from `before` on, reaches A or whose
+// running weight, from mbefore on, reaches X (the last if none does): its composite, and the weight up to and with it.
+__device__ __forceinline__ uint64_t cut_list(const RowsK &a, PickLds &L, float bv, uint32_t bin, uint32_t n, uint32_t before, uint64_t mbefore,
+                                             uint64_t A, uint64_t X, uint64_t *mass) {
+  auto part = [&](uint64_t c) {  // monotonic within the bin, as row_bin is
+    const float x = (bv - comp_value(c)) * a.bins - (float)bin;
+    return (uint32_t)fminf(fmaxf(x, 0.f) * (float)RS_SUB, (float)(RS_SUB - 1));
+  };
+  __syncthreads();
+  for (uint32_t b = threadIdx.x; b < RS_SUB; b += RS_T) { L.mass[b] = 0; L.count[b] = 0; }
+  if (threadIdx.x == 0) L.nlist = 0;
+  __syncthreads();
+  for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {
+    const uint32_t j = j0 + threadIdx.x;
+    const uint64_t c = j < n ? L.part[j] : 0;
+    hist_add<true>(L.mass, L.count, j < n, j < n ? part(c) : 0, (uint32_t)(c >> 32), j < n ? row_mass(a, row_weight(a, bv, comp_value(c))) : 0);
+  }
+  __syncthreads();
+  find_cross<RS_SUB>(L, false, before, mbefore, A, X);
+  const uint32_t sub = L.x_bin < RS_SUB ? L.x_bin : RS_SUB - 1;
+  const bool found = L.x_bin < RS_SUB;
+  for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {
+    const uint32_t j = j0 + threadIdx.x;
+    const uint64_t c = j < n ? L.part[j] : 0;
+    append(L.list, &L.nlist, j < n && (!found || part(c) == sub), c);
+  }
+  __syncthreads();
+  sort_list(a, L, bv);
+  const uint32_t b0 = found ? L.x_count : before;
+  const uint64_t m0 = found ? L.x_mass : mbefore;
+  const uint32_t at = find_place(L, m0, A > b0 ? A - b0 : 1, X);
+  *mass = m0 + L.cum[at];
+  return L.list[at];
+}
+
+// ------------------------------------------------------------------ rows: one workgroup, any bins
 
 // The first token of the row whose running count reaches A or whose running weight reaches X: its
 // composite, and the weight up to and with it.
@@ -718,14 +824,14 @@ __device__ __forceinline__ uint64_t first_token(const RowsK &a, PickLds &L, cons
   uint64_t mbefore = L.x_mass, prefix = 0, hi_mask = 0;
   uint32_t shift = 64;
   while (inside > RS_CAP && shift > 0) {
-    const uint32_t next = shift >= 12 ? shift - 12 : 0, fmask = (1u << (shift - next)) - 1;
+    const uint32_t next = shift >= 11 ? shift - 11 : 0, fmask = (1u << (shift - next)) - 1;
     __syncthreads();
     for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) { L.mass[b] = 0; L.count[b] = 0; }
     __syncthreads();
-    each_logit(row, a.n, [&](bool ok, float v, uint32_t i) {
+    each_logit<RS_T>(a, row, 0, a.n, [&](bool ok, float v, uint32_t i) {
       const uint64_t c = composite(v, i);
       ok = ok && row_bin(a, bv, v) == bin && (c & hi_mask) == prefix;
-      hist_add(L.mass, L.count, ok, (uint32_t)(c >> next) & fmask, order_key(v), ok ? row_mass(a, row_weight(a, bv, v)) : 0);
+      hist_add<true>(L.mass, L.count, ok, (uint32_t)(c >> next) & fmask, order_key(v), ok ? row_mass(a, row_weight(a, bv, v)) : 0);
     });
     __syncthreads();
     find_cross(L, true, before, mbefore, A, X);
@@ -737,104 +843,352 @@ __device__ __forceinline__ uint64_t first_token(const RowsK &a, PickLds &L, cons
     shift = next;
     __syncthreads();
   }
-  gather(a, L, row, bv, [&](float v, uint32_t i) {
-    return row_bin(a, bv, v) == bin && (composite(v, i) & hi_mask) == prefix;
+  if (threadIdx.x == 0) L.nlist = 0;
+  __syncthreads();
+  each_logit<RS_T>(a, row, 0, a.n, [&](bool ok, float v, uint32_t i) {
+    const uint64_t c = composite(v, i);
+    append(L.list, &L.nlist, ok && row_bin(a, bv, v) == bin && (c & hi_mask) == prefix, c);
   });
+  __syncthreads();
+  sort_list(a, L, bv);
   const uint32_t at = find_place(L, mbefore, A > before ? A - before : 1, X);
   *mass = mbefore + L.cum[at];
   return L.list[at];
 }
 
-__global__ __launch_bounds__(RS_T) void k_rows_pick(RowsK a) {
+// The row's histogram, and the weight that min-p keeps, by this workgroup alone, into h.
+__device__ __forceinline__ void row_hist(const RowsK &a, PickLds &L, RowHist &h, const float *row, float bv) {
+  __syncthreads();
+  for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) { L.mass[b] = 0; L.count[b] = 0; }
+  if (threadIdx.x == 0) L.x_mass = 0;
+  __syncthreads();
+  uint64_t minp = 0;
+  each_logit<RS_T>(a, row, 0, a.n, [&](bool ok, float v, uint32_t) {
+    const double w = ok ? row_weight(a, bv, v) : 0.0;
+    if (ok && w >= a.min_p) minp += row_mass(a, w);
+    hist_add<true>(L.mass, L.count, ok, ok ? row_bin(a, bv, v) : 0, ok ? order_key(v) : 0, row_mass(a, w));
+  });
+  minp = wave_sum_u64(minp);
+  if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long *)&L.x_mass, (unsigned long long)minp);
+  __syncthreads();
+  for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) { h.mass[b] = L.mass[b]; h.count[b] = L.count[b]; }
+  if (threadIdx.x == 0) h.minp = L.x_mass;
+  __syncthreads();
+}
+
+// The row's token from its histogram (row_hist's), cut after cut.
+__device__ __forceinline__ int32_t pick_row(const RowsK &a, PickLds &L, const RowHist &h, const float *row, float bv, uint32_t finite,
+                                            double u) {
+  constexpr uint64_t ALL = ~0ull;
+  uint64_t S, R, unused;
+  if (a.top_k && a.top_k < finite) {
+    first_token(a, L, h, row, bv, a.top_k, ALL, &S);
+  } else {
+    load_hist(L, h);
+    S = hist_mass(L);
+  }
+  R = S;
+  if (a.top_p < 1.0) first_token(a, L, h, row, bv, ALL, at_least(a.top_p * (double)S, S), &R);
+  R = min(R, h.minp);
+  return (int32_t)comp_index(first_token(a, L, h, row, bv, ALL, at_least(u * (double)R, R), &unused));
+}
+
+// ------------------------------------------------------------------ rows: many
+
+// Resolves the cut `done` from its list (CUT_NONE: there is none yet) and gathers the list of `next` over this
+// workgroup's slice.
+__global__ __launch_bounds__(RS_T) void k_rows_stage(RowsK a, uint32_t done, uint32_t next) {
   extern __shared__ uint64_t pick_lds[];
   PickLds &L = *(PickLds *)pick_lds;
-  const float *row = a.logits + blockIdx.x * a.stride;
-  const RowHist &h = a.hist[blockIdx.x];
   constexpr uint64_t ALL = ~0ull;
+  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  RowHist &h = a.hist[blockIdx.y];
+  uint64_t best;
+  uint32_t finite;
+  row_best(a, h, &best, &finite);
+  if (!finite) return;
+  for (uint32_t e = 0; e < next; e++)  // launches before this one
+    if (h.slow[e]) return;
+  const float bv = comp_value(best);
+  const bool cut_k = a.top_k && a.top_k < finite;
+  load_hist(L, h);
+  const uint64_t total = hist_mass(L);
+  // the weight that the cut `done` leaves: up to and with its token
+  auto resolve = [&](uint32_t cut, uint64_t A, uint64_t X) -> uint64_t {
+    uint64_t m;
+    find_cross(L, false, 0, 0, A, X);
+    const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[cut], RS_CAP);
+    const uint64_t mbefore = L.x_mass;
+    for (uint32_t j = tid; j < n; j += RS_T) L.part[j] = h.list[cut][j];
+    cut_list(a, L, bv, bin, n, before, mbefore, A, X, &m);
+    load_hist(L, h);  // cut_list used its place
+    return m;
+  };
+  uint64_t S = done == CUT_P ? h.s : total, R = 0;
+  if (done == CUT_K && cut_k) S = resolve(CUT_K, a.top_k, ALL);
+  const uint64_t X = at_least(a.top_p * (double)S, S);
+  if (done == CUT_P) R = resolve(CUT_P, ALL, X);
+  else R = S;
+  uint64_t A = ALL, to = ALL;
+  if (next == CUT_K) {
+    if (!cut_k) return;
+    A = a.top_k;
+  } else if (next == CUT_P) {
+    to = X;
+    if (blockIdx.x == 0 && tid == 0) h.s = S;
+  } else {
+    R = min(R, h.minp);
+    to = at_least(a.uniforms[blockIdx.y] * (double)R, R);
+    if (blockIdx.x == 0 && tid == 0) h.target = to;
+  }
+  find_cross(L, false, 0, 0, A, to);
+  const uint32_t bin = L.x_bin;
+  // this slice's tokens of the bin, in LDS first: one atomic on the list's count per workgroup
+  if (tid == 0) L.nlist = 0;
+  __syncthreads();
+  each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t i) {
+    append(L.list, &L.nlist, ok && row_bin(a, bv, v) == bin, composite(v, i));
+  });
+  __syncthreads();
+  const uint32_t n = L.nlist;
+  if (tid == 0) L.at = n ? atomicAdd(&h.nlist[next], n) : 0;
+  __syncthreads();
+  const uint32_t to_at = L.at;
+  if (n > RS_CAP || to_at + n > RS_CAP) {  // the list is full, whichever workgroup sees it
+    if (tid == 0) h.slow[next] = 1;
+    return;
+  }
+  for (uint32_t j = tid; j < n; j += RS_T) h.list[next][to_at + j] = L.list[j];
+}
+
+// The token: the best where nothing is drawn, else from the draw's list.
+__global__ __launch_bounds__(RS_T) void k_rows_last(RowsK a, uint32_t drawn) {
+  extern __shared__ uint64_t pick_lds[];
+  PickLds &L = *(PickLds *)pick_lds;
+  RowHist &h = a.hist[blockIdx.x];
   uint64_t best;
   uint32_t finite;
   row_best(a, h, &best, &finite);
   const double u = a.uniforms[blockIdx.x];
-  if (!finite || a.temperature == 0.0 || a.top_k == 1 || !(u > 0.0 && u < 1.0)) {
-    if (threadIdx.x == 0) a.tokens[blockIdx.x] = finite ? (int32_t)comp_index(best) : -1;
-    return;
-  }
-  const float bv = comp_value(best);
-  const uint32_t K = a.top_k && a.top_k < finite ? a.top_k : finite;
-  auto at_least = [](double x, uint64_t most) { return min(max((uint64_t)ceil(x), (uint64_t)1), most); };
-  load_hist(L, h);
-  uint64_t S = 0;  // the weight of the first K
-  bool listed = false;
-  if (K < finite) {
-    find_cross(L, false, 0, 0, K, ALL);
-    const uint32_t bin = L.x_bin;
-    if (L.x_count + L.count[bin] <= RS_CAP) {
-      gather(a, L, row, bv, [&](float v, uint32_t) { return row_bin(a, bv, v) <= bin; });
-      listed = true;
-      S = L.cum[K - 1];
+  int32_t token = finite ? (int32_t)comp_index(best) : -1;
+  if (finite && drawn && u > 0.0 && u < 1.0) {
+    const float bv = comp_value(best);
+    if (h.slow[0] || h.slow[1] || h.slow[2]) {
+      row_hist(a, L, h, a.logits + blockIdx.x * a.stride, bv);
+      token = pick_row(a, L, h, a.logits + blockIdx.x * a.stride, bv, finite, u);
     } else {
-      first_token(a, L, h, row, bv, K, ALL, &S);
-    }
-  } else {
-    uint64_t m = 0;
-    for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) m += L.mass[b];
-    m = wave_sum_u64(m);
-    if ((threadIdx.x & 63) == 0) L.wmass[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (uint32_t w = 0; w < RS_T / 64; w++) S += L.wmass[w];
-    __syncthreads();
-  }
-  const uint64_t X = a.top_p < 1.0 ? at_least(a.top_p * (double)S, S) : S;
-  if (!listed && a.top_p < 1.0) {
-    load_hist(L, h);
-    find_cross(L, false, 0, 0, ALL, X);
-    const uint32_t bin = L.x_bin;
-    if (bin < RS_BINS && L.x_count + L.count[bin] <= RS_CAP) {
-      gather(a, L, row, bv, [&](float v, uint32_t) { return row_bin(a, bv, v) <= bin; });
-      listed = true;
+      uint64_t unused;
+      load_hist(L, h);
+      find_cross(L, false, 0, 0, ~0ull, h.target);
+      const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[CUT_DRAW], RS_CAP);
+      const uint64_t mbefore = L.x_mass;
+      for (uint32_t j = threadIdx.x; j < n; j += RS_T) L.part[j] = h.list[CUT_DRAW][j];
+      token = (int32_t)comp_index(cut_list(a, L, bv, bin, n, before, mbefore, ~0ull, h.target, &unused));
     }
   }
-  uint64_t R = S, token;
-  if (listed) {
-    if (a.top_p < 1.0) R = L.cum[find_place(L, 0, ALL, X)];
-    R = min(R, h.minp);
-    token = L.list[find_place(L, 0, ALL, at_least(u * (double)R, R))];
-  } else {
-    if (a.top_p < 1.0) first_token(a, L, h, row, bv, ALL, X, &R);
-    R = min(R, h.minp);
-    uint64_t unused;
-    token = first_token(a, L, h, row, bv, ALL, at_least(u * (double)R, R), &unused);
-  }
-  if (threadIdx.x == 0) a.tokens[blockIdx.x] = (int32_t)comp_index(token);
+  if (threadIdx.x == 0) a.tokens[blockIdx.x] = token;
 }
 
-uint64_t sample_rows_scratch_bytes(const SampleRowsArgs &a) { return (uint64_t)std::min(a.rows, RS_ROWS) * sizeof(RowHist); }
+// ------------------------------------------------------------------ rows: few
+
+// Group j of 4 lanes of a wavefront's part of the row (a.steps steps of 256 logits): its largest key, 0 without a
+// finite logit. Lane l of step s reads logits 256 s + 4 l .. + 4 of the part.
+__global__ __launch_bounds__(RG_T) void k_rows_groups(RowsK a) {
+  const uint32_t lane = threadIdx.x & 63, part = blockIdx.x * (RG_T / 64) + (threadIdx.x >> 6);
+  const uint32_t lo = part * a.steps * RG_STEP;
+  if (lo >= a.n) return;
+  const float *row = a.logits + blockIdx.y * a.stride;
+  uint32_t key = 0;
+  auto take = [&](float v) { key = max(key, finite_f(v) ? order_key(v) : 0u); };
+  for (uint32_t s0 = 0; s0 < a.steps; s0 += 8) {
+    float4 v[8];
+#pragma unroll
+    for (uint32_t e = 0; e < 8; e++) v[e] = s0 + e < a.steps ? row_load4(a, row, lo + (s0 + e) * RG_STEP + 4 * lane) : make_float4(NAN, NAN, NAN, NAN);
+#pragma unroll
+    for (uint32_t e = 0; e < 8; e++) { take(v[e].x); take(v[e].y); take(v[e].z); take(v[e].w); }
+  }
+  key = max(key, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)key, 0xB1, 0xf, 0xf, false));  // quad_perm [1,0,3,2]
+  key = max(key, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)key, 0x4E, 0xf, 0xf, false));  // quad_perm [2,3,0,1]
+  if ((lane & 3) == 0) a.groups[blockIdx.y].key[16 * part + lane / 4] = key;
+}
+
+__global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
+  extern __shared__ uint64_t pick_lds[];
+  PickLds &L = *(PickLds *)pick_lds;
+  const uint32_t tid = threadIdx.x, lane = tid & 63;
+  const float *row = a.logits + blockIdx.x * a.stride;
+  float bv = 0.f;
+  if (a.n <= RS_CAP) {
+    if (tid == 0) L.nlist = 0;
+    __syncthreads();
+    float top = -INFINITY;
+    for (uint32_t i0 = 0; i0 < a.n; i0 += RS_T) {
+      const float v = i0 + tid < a.n ? row[i0 + tid] : NAN;
+      append(L.list, &L.nlist, finite_f(v), composite(v, i0 + tid));
+      top = finite_f(v) ? fmaxf(top, v) : top;
+    }
+    top = wave_max_f(top);
+    if (lane == 0) L.wcount[tid >> 6] = __float_as_uint(top);
+    __syncthreads();
+    for (uint32_t w = 0; w < RS_T / 64; w++) top = fmaxf(top, __uint_as_float(L.wcount[w]));
+    if (L.nlist == 0) {
+      if (tid == 0) a.tokens[blockIdx.x] = -1;
+      return;
+    }
+    bv = top;
+    __syncthreads();
+  } else {
+    uint32_t *chosen = (uint32_t *)L.cum;  // groups that reach the bound
+    const uint32_t *keys = a.groups[blockIdx.x].key;
+    constexpr uint32_t PER = RS_GROUPS / RS_T;
+    uint32_t key[PER], top_key = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < PER; e++) {
+      key[e] = e * RS_T + tid < a.ngroups ? keys[e * RS_T + tid] : 0;
+      top_key = max(top_key, key[e]);
+    }
+    for (int o = 32; o > 0; o >>= 1) top_key = max(top_key, (uint32_t)__shfl_xor((int)top_key, o));
+    if (lane == 0) L.wcount[tid >> 6] = top_key;
+    for (uint32_t b = tid; b < RS_BINS; b += RS_T) { L.count[b] = 0; L.mass[b] = 0; }
+    if (tid == 0) { L.nlist = 0; L.at = 0; }
+    __syncthreads();
+    for (uint32_t w = 0; w < RS_T / 64; w++) top_key = max(top_key, L.wcount[w]);
+    if (!top_key) {  // nothing finite
+      if (tid == 0) a.tokens[blockIdx.x] = -1;
+      return;
+    }
+    bv = comp_value((uint64_t)top_key << 32);
+#pragma unroll
+    for (uint32_t e = 0; e < PER; e++)
+      if (key[e]) atomicAdd(&L.count[row_bin(a, bv, comp_value((uint64_t)key[e] << 32))], 1u);
+    __syncthreads();
+    find_cross(L, false, 0, 0, a.top_k, ~0ull);
+    // what lies in the last bin has no weight: without top_k groups before it, the tokens before it are all that count
+    const uint32_t bound = min(L.x_bin, RS_BINS - 2);
+#pragma unroll
+    for (uint32_t e = 0; e < PER; e++)
+      if (key[e] && row_bin(a, bv, comp_value((uint64_t)key[e] << 32)) <= bound) chosen[atomicAdd(&L.at, 1u)] = e * RS_T + tid;
+    __syncthreads();
+    const uint32_t pieces = L.at * 4 * a.steps;  // of four logits
+    for (uint32_t i0 = 0; i0 < pieces; i0 += RS_T) {
+      const uint32_t i = i0 + tid, j = i < pieces ? chosen[i / (4 * a.steps)] : 0, in = i % (4 * a.steps);
+      const uint32_t at = (j / 16) * a.steps * RG_STEP + (in / 4) * RG_STEP + (j % 16) * 16 + (in % 4) * 4;
+      const float4 v = i < pieces ? row_load4(a, row, at) : make_float4(NAN, NAN, NAN, NAN);
+      auto put = [&](float x, uint32_t e) { append(L.list, &L.nlist, finite_f(x) && row_bin(a, bv, x) <= bound, composite(x, at + e)); };
+      put(v.x, 0); put(v.y, 1); put(v.z, 2); put(v.w, 3);
+    }
+    __syncthreads();
+  }
+  const uint32_t nl = L.nlist;
+  if (nl > RS_CAP) {  // ties: the row goes through its histogram, formed here
+    RowHist &h = a.hist[blockIdx.x];
+    uint32_t cnt = 0;
+    uint64_t best = 0;
+    each_logit<RS_T>(a, row, 0, a.n, [&](bool ok, float v, uint32_t i) {
+      cnt += ok;
+      if (ok) best = max(best, composite(v, i));
+    });
+    best = wave_max_u64(best);
+    cnt = wave_sum_u32(cnt);
+    __syncthreads();
+    if (lane == 0) { L.wmass[tid >> 6] = best; L.wcount[tid >> 6] = cnt; }
+    __syncthreads();
+    uint32_t finite = 0;
+    for (uint32_t w = 0; w < RS_T / 64; w++) { best = max(best, L.wmass[w]); finite += L.wcount[w]; }
+    row_hist(a, L, h, row, bv);
+    const double u = a.uniforms[blockIdx.x];
+    const int32_t token = u > 0.0 && u < 1.0 ? pick_row(a, L, h, row, bv, finite, u) : (int32_t)comp_index(best);
+    if (tid == 0) a.tokens[blockIdx.x] = token;
+    return;
+  }
+  const double u = a.uniforms[blockIdx.x];
+  sort_list(a, L, bv);
+  int32_t token = (int32_t)comp_index(L.list[0]);
+  if (u > 0.0 && u < 1.0) {
+    const uint32_t K = a.top_k ? min(a.top_k, nl) : nl;
+    const uint64_t S = L.cum[K - 1];
+    uint32_t last = K - 1;
+    if (a.top_p < 1.0) last = min(last, find_place(L, 0, ~0ull, at_least(a.top_p * (double)S, S)));
+    if (a.min_p > 0.0) {  // weights fall along the list
+      __syncthreads();
+      if (tid == 0) L.at = 0;
+      __syncthreads();
+      uint32_t kept = 0;
+      for (uint32_t j = tid; j <= last; j += RS_T) kept += row_weight(a, bv, comp_value(L.list[j])) >= a.min_p;
+      kept = wave_sum_u32(kept);
+      if (lane == 0 && kept) atomicAdd(&L.at, kept);
+      __syncthreads();
+      last = min(last, max(L.at, 1u) - 1);
+    }
+    const uint64_t R = L.cum[last];
+    token = (int32_t)comp_index(L.list[find_place(L, 0, ~0ull, at_least(u * (double)R, R))]);
+  }
+  if (tid == 0) a.tokens[blockIdx.x] = token;
+}
+
+// Steps of a wavefront's part so that a row has at most RS_GROUPS groups: of 16 logits up to 32768, 64 at 128256.
+static uint32_t group_steps(uint32_t n) {
+  constexpr uint64_t most = RS_GROUPS / 16 * RG_STEP;
+  return (uint32_t)((n + most - 1) / most);
+}
+static uint32_t group_count(uint32_t n) {
+  const uint64_t part = (uint64_t)group_steps(n) * RG_STEP;
+  return (uint32_t)((n + part - 1) / part) * 16;
+}
+
+uint64_t sample_rows_scratch_bytes(const SampleRowsArgs &a) {
+  return (uint64_t)std::min(a.rows, RS_ROWS) * (sizeof(RowHist) + sizeof(RowGroups));
+}
 
 hipError_t sample_rows(hipStream_t s, const SampleRowsArgs &in) {
   if (!in.rows) return hipSuccess;
   if (!in.n || !in.scratch || in.stride < in.n) return hipErrorInvalidValue;
   RowsK a{};
   a.n = in.n; a.stride = in.stride;
-  a.slice = std::max(RS_MIN, (in.n + RS_SLICES - 1) / RS_SLICES);
+  a.slice = (std::max(RS_SLICE, (in.n + RS_SLICES - 1) / RS_SLICES) + 3) & ~3u;
   a.nslices = (in.n + a.slice - 1) / a.slice;
+  a.steps = group_steps(in.n); a.ngroups = group_count(in.n);
+  a.aligned = (uintptr_t)in.logits % 16 == 0 && in.stride % 4 == 0;
   a.hist = (RowHist *)in.scratch;
-  a.temperature = in.temperature; a.top_p = in.top_p; a.min_p = in.min_p; a.top_k = in.top_k;
+  a.groups = (RowGroups *)(a.hist + std::min(in.rows, RS_ROWS));
+  a.inv_t = in.temperature > 0.0 ? std::min(1e300, 1.0 / in.temperature) : 0.0;
+  a.top_p = in.top_p; a.min_p = in.min_p; a.top_k = in.top_k;
   int log2n = 0;
   while (log2n < 32 && (1ull << log2n) < in.n) log2n++;
   a.unit = std::ldexp(1.0, 62 - log2n);
   // a temperature near 0 has no finite scale: any large one keeps the bins monotonic
   a.bins = in.temperature > 0.0 ? (float)std::min(1e30, RS_BINS / (RS_SPAN * in.temperature)) : 0.f;
-  lds_opt_in((const void *)k_rows_pick);
+  lds_opt_in((const void *)k_rows_stage);
+  lds_opt_in((const void *)k_rows_last);
+  lds_opt_in((const void *)k_rows_few);
+  const bool drawn = in.temperature != 0.0 && in.top_k != 1;
+  const bool whole = in.n <= RS_CAP, few = drawn && (whole || (in.top_k >= 2 && in.top_k <= RS_FEW && 2 * in.top_k <= a.ngroups));
   for (uint32_t r0 = 0; r0 < in.rows; r0 += RS_ROWS) {
     const uint32_t nr = std::min(RS_ROWS, in.rows - r0);
     a.logits = in.logits + (uint64_t)r0 * in.stride; a.uniforms = in.uniforms + r0; a.tokens = in.tokens + r0;
-    hipLaunchKernelGGL(k_rows_best, dim3(a.nslices, nr), dim3(RS_HT), 0, s, a);
-    WGD_HIP(hipGetLastError());
-    if (in.temperature != 0.0 && in.top_k != 1) {
-      hipLaunchKernelGGL(k_rows_hist, dim3(a.nslices, nr), dim3(RS_HT), 0, s, a);
+    if (few) {
+      if (!whole) hipLaunchKernelGGL(k_rows_groups, dim3((a.ngroups / 16 + RG_T / 64 - 1) / (RG_T / 64), nr), dim3(RG_T), 0, s, a);
       WGD_HIP(hipGetLastError());
+      hipLaunchKernelGGL(k_rows_few, dim3(nr), dim3(RS_T), sizeof(PickLds), s, a);
+      WGD_HIP(hipGetLastError());
+      continue;
     }
-    hipLaunchKernelGGL(k_rows_pick, dim3(nr), dim3(RS_T), sizeof(PickLds), s, a);
+    const dim3 grid(a.nslices, nr);
+    hipLaunchKernelGGL(k_rows_best, grid, dim3(256), 0, s, a);
+    WGD_HIP(hipGetLastError());
+    if (drawn) {
+      if (in.top_k && in.top_k < in.n) hipLaunchKernelGGL(k_rows_hist<true>, grid, dim3(RS_T), 0, s, a);
+      else hipLaunchKernelGGL(k_rows_hist<false>, grid, dim3(RS_T), 0, s, a);
+      WGD_HIP(hipGetLastError());
+      uint32_t done = CUT_NONE;
+      for (uint32_t next = CUT_K; next <= CUT_DRAW; next++) {
+        if ((next == CUT_K && (!in.top_k || in.top_k >= in.n)) || (next == CUT_P && in.top_p >= 1.0)) continue;
+        hipLaunchKernelGGL(k_rows_stage, grid, dim3(RS_T), sizeof(PickLds), s, a, done, next);
+        WGD_HIP(hipGetLastError());
+        done = next;
+      }
+    }
+    hipLaunchKernelGGL(k_rows_last, dim3(nr), dim3(RS_T), sizeof(PickLds), s, a, drawn ? 1u : 0u);
     WGD_HIP(hipGetLastError());
   }
   return hipSuccess;
