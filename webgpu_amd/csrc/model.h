@@ -2,6 +2,7 @@
 #pragma once
 #include <map>
 #include <set>
+#include <unordered_set>
 #include <string>
 #include <vector>
 
@@ -15,7 +16,7 @@ struct wgd_context {
   hipStream_t stream = nullptr;
   uint64_t limit = 0, allocated = 0, peak = 0;
   std::string error, adapter;
-  std::set<wgd_buffer *> buffers;
+  std::unordered_set<wgd_buffer *> buffers;
   std::set<wgd_model *> models;
   std::map<void *, uint64_t> sizes;   // every device allocation of the context
   int32_t *argmax_scratch = nullptr;  // int32 result + 256 partial keys

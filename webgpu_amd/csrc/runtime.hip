@@ -815,13 +815,16 @@ int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, co
   if (!count) return WGD_OK;
   if (!rings) return fail(ctx, WGD_E_INVALID, "kv_commit: NULL rings");
   std::vector<void *> at(count);
-  std::set<const wgd_buffer *> seen;
   for (uint32_t i = 0; i < count; i++) {
     NEED_BUF(ctx, rings[i], "kv_commit");
     NEED_FIT(ctx, rings[i], (uint64_t)capacity * row_bytes, "kv_commit ring");
-    if (rings[i] == path || !seen.insert(rings[i]).second) return fail(ctx, WGD_E_INVALID, "kv_commit: ring %u (%s) is given twice or is the path", i, rings[i]->label.c_str());
     at[i] = rings[i]->ptr;
   }
+  std::vector<void *> sorted = at;
+  sorted.push_back(path->ptr);
+  std::sort(sorted.begin(), sorted.end());
+  if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+    return fail(ctx, WGD_E_INVALID, "kv_commit: a ring is given twice, or is the path");
   return ctx_check(ctx, kv_commit(ctx->stream, at.data(), count, (const int32_t *)path->ptr, row_bytes, start, capacity, nodes), "kv_commit");
 }
 

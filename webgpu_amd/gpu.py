@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 from typing import Optional
 
 import numpy as np
@@ -59,7 +60,7 @@ SIGNATURES = {
     "wgd_attention_tree_f16kv": (C.c_int, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _F, _U32, _U32, _U32]),
     "wgd_sample_rows": (C.c_int, [_P, _P, _U32, _U32, _U32, _P, _P, _D, _U32, _D, _D]),
     "wgd_tree_accept": (C.c_int, [_P, _P, _P, _P, _P, _U32]),
-    "wgd_kv_commit": (C.c_int, [_P, C.POINTER(_P), _U32, _P, _U64, _U32, _U32, _U32]),
+    "wgd_kv_commit": (C.c_int, [_P, _P, _U32, _P, _U64, _U32, _U32, _U32]),
     "wgd_probe_read": (C.c_int, [_P, _P, _U64, _U32, _U32, _U32, _U32, _U32, _P, _U32]),
     "wgd_add": (C.c_int, [_P, _P, _P, _U32]),
     "wgd_silu": (C.c_int, [_P, _P, _P, _P, _U32]),
@@ -356,8 +357,8 @@ class Compute:
 
     def kv_commit(self, rings, path: Buffer, row_bytes: int, start: int, capacity: int, nodes: int) -> None:
         """Moves the path's rows of every ring (K and V of any layers) to the slots they keep."""
-        ptrs = (C.c_void_p * max(1, len(rings)))(*[r.ptr for r in rings])
-        self.check(lib().wgd_kv_commit(self.ctx, ptrs, len(rings), path.ptr, row_bytes, start, capacity, nodes))
+        ptrs = array("Q", [r.ptr for r in rings])
+        self.check(lib().wgd_kv_commit(self.ctx, ptrs.buffer_info()[0], len(ptrs), path.ptr, row_bytes, start, capacity, nodes))
 
     def embed(self, type_: int, table: Buffer, ids: Buffer, out: Buffer, hidden: int, n: int, scale: float = 1.0) -> None:
         self.check(lib().wgd_embed(self.ctx, type_, table.ptr, ids.ptr, out.ptr, hidden, n, scale))
