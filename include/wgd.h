@@ -264,7 +264,7 @@ int wgd_attention_tree_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_bu
  * shortest prefix whose share of their weight reaches top_p, and of these the ones with a weight
  * of min_p or more; the token is the first whose running sum reaches uniform * (the kept
  * weight). With min_p 0 that is wgd_sample's rule. Weights and sums are integers of
- * 2^-(62 - ceil(log2 n)) of the largest weight, so a draw does not depend on the order of the sums.
+ * 2^-(62 - ceil(log2 n)), at most 2^-51, of the largest weight, so a draw does not depend on the order of the sums.
  * Temperature 0 takes the best; so does a uniform outside [0, 1). A row without a finite logit
  * gets -1. temperature <= 2, 0 < top_p <= 1, 0 <= min_p <= 1 (WGD_E_INVALID otherwise). */
 int wgd_sample_rows(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, uint32_t rows, uint32_t stride,

@@ -458,7 +458,7 @@ hipError_t sample(hipStream_t s, const float *logits, uint32_t n, const SamplePa
 // ------------------------------------------------------------------ rows with given uniforms
 //
 // wgd_sample_rows: for every row the finite logits in descending order (composites, as above) have the
-// weights w = exp((l - best) / T) in f64, rounded to integers of 2^-shift with shift = 62 - ceil(log2 n): their sums fit
+// weights w = exp((l - best) / T) in f64, rounded to integers of 2^-shift with shift = 62 - ceil(log2 n), at most 51: their sums fit
 // 64 bits, are exact, and do not depend on the order of the adds, so atomics give the same token every time.
 // A top-k, top-p or min-p cut and the draw itself are all "the first token whose running count reaches A or whose
 // running weight reaches X". Two ways, by top_k alone:
@@ -468,31 +468,32 @@ hipError_t sample(hipStream_t s, const float *logits, uint32_t n, const SamplePa
 //   * k_rows_few, a workgroup a row: the bin (below) that holds the top_k-th largest of those keys bounds the bin of the
 //     top_k-th largest logit (top_k logits reach it). Only groups that reach it are read again; of their
 //     logits little more than top_k do, which are sorted and summed in LDS. A row of at most RS_CAP logits is one list.
-// Many (top_k 0 or above), four to six launches, each a pass over the rows by all CUs:
+// Many (top_k 0 or above), four or five launches, each a pass over the rows by all CUs:
 //   * k_rows_best: the best composite and the count of finite logits, by slices;
-//   * k_rows_hist: counts and weights over RS_BINS bins of (best - l) / T, which is monotonic in l;
-//   * k_rows_stage for each of the cuts that there are (top-k, top-p) and the draw: the bin that holds the cut's token,
-//     from the running histogram, and that bin's tokens into a list; the cut before it, from its list;
-//   * k_rows_last: the token from the draw's list.
+//   * k_rows_hist: counts (for a top-k cut) and weights over RS_BINS bins of (best - l) / T, which is monotonic in l;
+//   * k_rows_topk where top_k cuts: the bin of its token, from the running histogram, and that bin's tokens into a list;
+//   * k_rows_cuts: the same for top-p, and for the draw: what top-p keeps is known to within its bin, so the bins
+//     that the draw can fall into are known too, one or two;
+//   * k_rows_last: what top-p keeps and the token, from their lists.
 // A cut's token is found in its list by a histogram of RS_SUB parts of the bin and a sort of the one part
 // that holds it (a sort of the whole list took four times as long).
 // A bin or bound with more tokens than a list holds (ties, logits close together for the temperature) goes through
 // pick_row, which refines by 12 bits of the composite at a time, in one workgroup.
-constexpr uint32_t RS_T = 512, RS_BINS = 2048, RS_CAP = 2048, RS_SUB = 1024;
+constexpr uint32_t RS_T = 512, RS_BINS = 2048, RS_CAP = 2048, RS_DRAW = 8192, RS_SUB = 1024;
 constexpr uint32_t RS_ROWS = 256;  // rows per launch: the histograms of more would only fill memory
 constexpr float RS_SPAN = 48.f;    // bins cover exp(0) to exp(-48) < 2^-62; the last one all below
 constexpr uint32_t RS_SLICES = 64, RS_SLICE = 16384;  // most slices of a row, least logits of one
 constexpr uint32_t RS_FEW = 512, RS_GROUPS = 2048;   // top_k by groups; most groups of a row
 constexpr uint32_t RG_T = 256, RG_STEP = 256;        // k_rows_groups: threads; logits of a wavefront's step
-enum RowCut : uint32_t { CUT_K = 0, CUT_P = 1, CUT_DRAW = 2, CUT_NONE = 3 };
+enum RowCut : uint32_t { CUT_K = 0, CUT_P = 1, CUT_DRAW = 2 };
 
 struct RowSlice { uint64_t best; uint32_t finite, pad; };
 struct RowHist {
   uint64_t mass[RS_BINS];
   uint32_t count[RS_BINS];
-  uint64_t list[3][RS_CAP];
-  uint32_t nlist[3], slow[3];  // slow: a cut's bin holds more than its list
-  uint64_t minp, s, target;
+  uint64_t list[2][RS_CAP], draw[RS_DRAW];  // of top-k, top-p and the draw
+  uint32_t nlist[3], slow[2];                // slow: k_rows_topk or k_rows_cuts has a list that is full
+  uint64_t minp, s;                          // the weights that min-p and top-k keep
   RowSlice slice[RS_SLICES];
 };
 struct RowGroups { uint32_t key[RS_GROUPS]; };
@@ -502,14 +503,36 @@ struct RowsK {
   const double *uniforms; int32_t *tokens; RowHist *hist; RowGroups *groups;
   double inv_t, top_p, min_p, unit;  // 1 / temperature; unit: 2^shift
   float bins;                        // bins per unit of logit
-  uint32_t top_k, steps, ngroups, aligned;
+  uint32_t top_k, steps, ngroups, aligned, bslice, bslices;  // b..: slices of k_rows_best
 };
 
 __device__ __forceinline__ uint32_t row_bin(const RowsK &a, float best, float l) {
   return (uint32_t)fminf((best - l) * a.bins, (float)(RS_BINS - 1));
 }
-__device__ __forceinline__ double row_weight(const RowsK &a, float best, float l) { return exp(((double)l - (double)best) * a.inv_t); }
-__device__ __forceinline__ uint64_t row_mass(const RowsK &a, double w) { return (uint64_t)(w * a.unit + 0.5); }
+// exp((l - best) / T) to 2^-48 of it: 2^k times the Taylor sum of the rest r, |r| <= ln 2 / 2, whose next term is below 7e-15.
+// Below 2^-70 it is 0: less than half of the least integer below, whatever n.
+__device__ __forceinline__ double row_weight(const RowsK &a, float best, float l) {
+  const double x = fmax(((double)l - (double)best) * a.inv_t, -64.0);
+  const double k = rint(x * 1.44269504088896340736);
+  const double r = fma(-k, 0.69314718055994530942, x);
+  double p = 1.0 / 39916800;
+  p = fma(p, r, 1.0 / 3628800);
+  p = fma(p, r, 1.0 / 362880);
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return x <= -48.6 ? 0.0 : ldexp(p, (int)k);
+}
+// w times 2^shift (at most 2^51) as an integer: the low bits of its sum with 2^52, which rounds it.
+__device__ __forceinline__ uint64_t row_mass(const RowsK &a, double w) {
+  return (uint64_t)__double_as_longlong(w * a.unit + 0x1p52) & ((1ull << 52) - 1);
+}
 __device__ __forceinline__ uint64_t composite(float l, uint32_t i) { return ((uint64_t)order_key(l) << 32) | (0xFFFFFFFFu - i); }
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -554,7 +577,7 @@ __device__ __forceinline__ void each_logit(const RowsK &a, const float *row, uin
 __global__ __launch_bounds__(256) void k_rows_best(RowsK a) {
   __shared__ uint64_t wmax[4];
   __shared__ uint32_t wsum[4];
-  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.bslice, hi = min(lo + a.bslice, a.n);
   RowHist &h = a.hist[blockIdx.y];
   float top = -INFINITY;
   uint32_t at = 0, cnt = 0;
@@ -567,10 +590,10 @@ __global__ __launch_bounds__(256) void k_rows_best(RowsK a) {
   cnt = wave_sum_u32(cnt);
   if ((tid & 63) == 0) { wmax[tid >> 6] = best; wsum[tid >> 6] = cnt; }
   // this slice's share of what the launches behind it add to
-  for (uint32_t b = blockIdx.x * 256 + tid; b < RS_BINS; b += a.nslices * 256) { h.mass[b] = 0; h.count[b] = 0; }
+  for (uint32_t b = blockIdx.x * 256 + tid; b < RS_BINS; b += a.bslices * 256) { h.mass[b] = 0; h.count[b] = 0; }
   if (blockIdx.x == 0 && tid == 0) {
     h.minp = 0;
-    for (int e = 0; e < 3; e++) h.nlist[e] = h.slow[e] = 0;
+    h.nlist[0] = h.nlist[1] = h.nlist[2] = h.slow[0] = h.slow[1] = 0;
   }
   __syncthreads();
   if (tid != 0) return;
@@ -581,29 +604,17 @@ __global__ __launch_bounds__(256) void k_rows_best(RowsK a) {
 // The row's best composite and finite count, in every thread of a wavefront.
 __device__ __forceinline__ void row_best(const RowsK &a, const RowHist &h, uint64_t *best, uint32_t *finite) {
   const uint32_t lane = threadIdx.x & 63;
-  const RowSlice s = lane < a.nslices ? h.slice[lane] : RowSlice{0, 0, 0};
+  const RowSlice s = lane < a.bslices ? h.slice[lane] : RowSlice{0, 0, 0};
   *best = wave_max_u64(s.best);
   *finite = wave_sum_u32(s.finite);
 }
 
-// One token's weight into a histogram in LDS: a wavefront whose tokens all share a key adds once.
-// COUNT: counts too.
+// One token's weight, and with COUNT the token, into a histogram in LDS.
 template <bool COUNT>
-__device__ __forceinline__ void hist_add(uint64_t *mass, uint32_t *count, bool ok, uint32_t bin, uint32_t key, uint64_t m) {
-  const uint64_t on = __ballot(ok);
-  if (!on) return;
-  const int first = (int)__ffsll((unsigned long long)on) - 1;
-  const uint32_t bin0 = __shfl(bin, first), key0 = __shfl(key, first);
-  if (__ballot(ok && (bin != bin0 || key != key0)) == 0) {
-    const uint32_t c = (uint32_t)__popcll(on);
-    if ((int)(threadIdx.x & 63) == first) {
-      if (COUNT) atomicAdd(&count[bin], c);
-      atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)(m * c));
-    }
-  } else if (ok) {
-    if (COUNT) atomicAdd(&count[bin], 1u);
-    if (m) atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)m);
-  }
+__device__ __forceinline__ void hist_add(uint64_t *mass, uint32_t *count, bool ok, uint32_t bin, uint64_t m) {
+  if (!ok) return;
+  if (COUNT) atomicAdd(&count[bin], 1u);
+  if (m) atomicAdd((unsigned long long *)&mass[bin], (unsigned long long)m);
 }
 
 template <bool COUNT>
@@ -627,7 +638,7 @@ __global__ __launch_bounds__(RS_T) void k_rows_hist(RowsK a) {
     const double w = ok ? row_weight(a, bv, v) : 0.0;
     const uint64_t m = row_mass(a, w);
     if (ok && w >= a.min_p) minp += m;
-    hist_add<COUNT>(mass, count, ok, ok ? row_bin(a, bv, v) : 0, ok ? order_key(v) : 0, m);
+    hist_add<COUNT>(mass, count, ok, ok ? row_bin(a, bv, v) : 0, m);
   });
   __syncthreads();
   for (uint32_t b = tid; b < RS_BINS; b += RS_T) {
@@ -640,46 +651,77 @@ __global__ __launch_bounds__(RS_T) void k_rows_hist(RowsK a) {
 
 struct PickLds {
   uint64_t mass[RS_BINS];
-  uint32_t count[RS_BINS];
+  uint32_t count[RS_BINS];         // both with what lies in the bins before, once scanned
+  uint64_t smass[RS_SUB];
+  uint32_t scount[RS_SUB];         // the same of the parts of one bin
   uint64_t list[RS_CAP], cum[RS_CAP];
-  uint64_t part[RS_CAP];           // one part of a bin's tokens; tokens on their way to a list
+  uint64_t part[RS_CAP];           // one bin's tokens; tokens on their way to a list
   uint64_t wmass[RS_T / 64];
   uint32_t wcount[RS_T / 64];
   uint64_t x_mass;                 // of find_cross: the weight and count before the bin
-  uint32_t x_bin, x_count, nlist, at;
+  uint32_t x_bin, x_count, nlist, npart, at;
 };
 
-// The first bin at which the running count reaches A or the running weight X, added to count0 and
-// mass0, and both before that bin; bins run from 0, or with `down` from the last. Callers ask only for
-// what the bins hold; without such a bin x_bin stays RS_BINS.
-template <uint32_t BINS = RS_BINS>
-__device__ __forceinline__ void find_cross(PickLds &L, bool down, uint32_t count0, uint64_t mass0, uint64_t A, uint64_t X) {
+// The sum of v over this lane and the ones below it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  v += dpp_u64<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_u64<0x112, 0xf>(v);
+  v += dpp_u64<0x114, 0xf>(v);
+  v += dpp_u64<0x118, 0xf>(v);
+  v += dpp_u64<0x142, 0xa>(v);  // row_bcast15 into rows 1 and 3
+  v += dpp_u64<0x143, 0xc>(v);  // row_bcast31 into rows 2 and 3
+  return v;
+}
+
+// Running sums of the bins, in place.
+template <uint32_t BINS>
+__device__ __forceinline__ void scan_bins(PickLds &L, uint64_t *mass, uint32_t *count) {
   constexpr uint32_t PER = BINS / RS_T;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  uint32_t c = 0;
-  uint64_t m = 0;
-  auto at = [&](uint32_t e) { return down ? BINS - 1 - (PER * tid + e) : PER * tid + e; };
-  for (uint32_t e = 0; e < PER; e++) { c += L.count[at(e)]; m += L.mass[at(e)]; }
-  uint32_t ci = c;
-  uint64_t mi = m;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t cw = __shfl_up(ci, o);
-    const uint64_t mw = __shfl_up(mi, o);
-    if ((int)lane >= o) { ci += cw; mi += mw; }
-  }
+  uint64_t m[PER], ms = 0;
+  uint32_t c[PER], cs = 0;
   __syncthreads();
-  if (lane == 63) { L.wcount[wv] = ci; L.wmass[wv] = mi; }
-  if (tid == 0) L.x_bin = RS_BINS;
-  __syncthreads();
-  uint64_t cb = (uint64_t)count0 + ci - c, mb = mass0 + mi - m;
-  for (uint32_t w = 0; w < wv; w++) { cb += L.wcount[w]; mb += L.wmass[w]; }
+#pragma unroll
   for (uint32_t e = 0; e < PER; e++) {
-    const uint64_t c1 = cb + L.count[at(e)], m1 = mb + L.mass[at(e)];
-    if (cb < A && mb < X && (c1 >= A || m1 >= X)) { L.x_bin = at(e); L.x_count = (uint32_t)cb; L.x_mass = mb; }
-    cb = c1; mb = m1;
+    m[e] = ms += mass[PER * tid + e];
+    c[e] = cs += count[PER * tid + e];
+  }
+  const uint64_t mi = wave_scan_u64(ms), ci = wave_scan_u64(cs);
+  if (lane == 63) { L.wmass[wv] = mi; L.wcount[wv] = (uint32_t)ci; }
+  __syncthreads();
+  uint64_t mb = mi - ms, cb = ci - cs;
+  for (uint32_t w = 0; w < wv; w++) { mb += L.wmass[w]; cb += L.wcount[w]; }
+#pragma unroll
+  for (uint32_t e = 0; e < PER; e++) {
+    mass[PER * tid + e] = mb + m[e];
+    count[PER * tid + e] = (uint32_t)cb + c[e];
   }
   __syncthreads();
 }
+
+// The first bin of scanned ones at which the running count reaches A or the running weight X, from count0 and mass0
+// on, and both before that bin. Callers ask only for what the bins hold; without such a bin x_bin is BINS.
+template <uint32_t BINS>
+__device__ __forceinline__ void find_cross(PickLds &L, const uint64_t *mass, const uint32_t *count, uint32_t count0, uint64_t mass0, uint64_t A,
+                                           uint64_t X) {
+  __syncthreads();
+  if (threadIdx.x == 0) L.x_bin = BINS;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t b = threadIdx.x; b < BINS; b += RS_T) {
+    const uint64_t c1 = (uint64_t)count0 + count[b], m1 = mass0 + mass[b];
+    const uint64_t cb = b ? (uint64_t)count0 + count[b - 1] : count0, mb = b ? mass0 + mass[b - 1] : mass0;
+    if (cb < A && mb < X && (c1 >= A || m1 >= X)) { L.x_bin = b; L.x_count = (uint32_t)cb; L.x_mass = mb; }
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void find_cross(PickLds &L, uint64_t A, uint64_t X) { find_cross<RS_BINS>(L, L.mass, L.count, 0, 0, A, X); }
 
 // L.list[0 .. L.nlist) (at most RS_CAP) in descending order, and its running weights in L.cum. Up to RS_RANK tokens are
 // placed by the count of larger ones, without a barrier per step.
@@ -719,10 +761,7 @@ __device__ __forceinline__ void sort_list(const RowsK &a, PickLds &L, float bv) 
     m[e] = j < nl ? row_mass(a, row_weight(a, bv, comp_value(L.list[j]))) : 0;
     incl += m[e];
   }
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t w = __shfl_up(incl, o);
-    if ((int)lane >= o) incl += w;
-  }
+  incl = wave_scan_u64(incl);
   if (lane == 63) L.wmass[wv] = incl;
   __syncthreads();
   for (uint32_t w = 0; w < wv; w++) incl += L.wmass[w];
@@ -747,22 +786,11 @@ __device__ __forceinline__ uint32_t find_place(PickLds &L, uint64_t mass0, uint6
   return L.at;
 }
 
+// The row's histogram, scanned: the last bin has the sum of all weights.
 __device__ __forceinline__ void load_hist(PickLds &L, const RowHist &h) {
   __syncthreads();
   for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) { L.mass[b] = h.mass[b]; L.count[b] = h.count[b]; }
-  __syncthreads();
-}
-// The sum of the histogram's weights.
-__device__ __forceinline__ uint64_t hist_mass(PickLds &L) {
-  uint64_t m = 0, s = 0;
-  for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) m += L.mass[b];
-  m = wave_sum_u64(m);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) L.wmass[threadIdx.x >> 6] = m;
-  __syncthreads();
-  for (uint32_t w = 0; w < RS_T / 64; w++) s += L.wmass[w];
-  __syncthreads();
-  return s;
+  scan_bins<RS_BINS>(L, L.mass, L.count);
 }
 
 // Appends the wavefront's tokens for which `take` holds to a list with room for RS_CAP; the count goes on past it.
@@ -785,16 +813,15 @@ __device__ __forceinline__ uint64_t cut_list(const RowsK &a, PickLds &L, float b
     return (uint32_t)fminf(fmaxf(x, 0.f) * (float)RS_SUB, (float)(RS_SUB - 1));
   };
   __syncthreads();
-  for (uint32_t b = threadIdx.x; b < RS_SUB; b += RS_T) { L.mass[b] = 0; L.count[b] = 0; }
+  for (uint32_t b = threadIdx.x; b < RS_SUB; b += RS_T) { L.smass[b] = 0; L.scount[b] = 0; }
   if (threadIdx.x == 0) L.nlist = 0;
   __syncthreads();
-  for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {
-    const uint32_t j = j0 + threadIdx.x;
-    const uint64_t c = j < n ? L.part[j] : 0;
-    hist_add<true>(L.mass, L.count, j < n, j < n ? part(c) : 0, (uint32_t)(c >> 32), j < n ? row_mass(a, row_weight(a, bv, comp_value(c))) : 0);
+  for (uint32_t j = threadIdx.x; j < n; j += RS_T) {
+    const uint64_t c = L.part[j];
+    hist_add<true>(L.smass, L.scount, true, part(c), row_mass(a, row_weight(a, bv, comp_value(c))));
   }
-  __syncthreads();
-  find_cross<RS_SUB>(L, false, before, mbefore, A, X);
+  scan_bins<RS_SUB>(L, L.smass, L.scount);
+  find_cross<RS_SUB>(L, L.smass, L.scount, before, mbefore, A, X);
   const uint32_t sub = L.x_bin < RS_SUB ? L.x_bin : RS_SUB - 1;
   const bool found = L.x_bin < RS_SUB;
   for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {
@@ -818,9 +845,10 @@ __device__ __forceinline__ uint64_t cut_list(const RowsK &a, PickLds &L, float b
 __device__ __forceinline__ uint64_t first_token(const RowsK &a, PickLds &L, const RowHist &h, const float *row, float bv,
                                                 uint64_t A, uint64_t X, uint64_t *mass) {
   load_hist(L, h);
-  find_cross(L, false, 0, 0, A, X);
+  find_cross(L, A, X);
+  auto in_bin = [&](uint32_t b) { return b < RS_BINS ? L.count[b] - (b ? L.count[b - 1] : 0) : 0; };
   const uint32_t bin = L.x_bin;
-  uint32_t before = L.x_count, inside = L.count[bin < RS_BINS ? bin : 0];
+  uint32_t before = L.x_count, inside = in_bin(bin);
   uint64_t mbefore = L.x_mass, prefix = 0, hi_mask = 0;
   uint32_t shift = 64;
   while (inside > RS_CAP && shift > 0) {
@@ -831,14 +859,15 @@ __device__ __forceinline__ uint64_t first_token(const RowsK &a, PickLds &L, cons
     each_logit<RS_T>(a, row, 0, a.n, [&](bool ok, float v, uint32_t i) {
       const uint64_t c = composite(v, i);
       ok = ok && row_bin(a, bv, v) == bin && (c & hi_mask) == prefix;
-      hist_add<true>(L.mass, L.count, ok, (uint32_t)(c >> next) & fmask, order_key(v), ok ? row_mass(a, row_weight(a, bv, v)) : 0);
+      // larger composites first
+      hist_add<true>(L.mass, L.count, ok, RS_BINS - 1 - ((uint32_t)(c >> next) & fmask), ok ? row_mass(a, row_weight(a, bv, v)) : 0);
     });
-    __syncthreads();
-    find_cross(L, true, before, mbefore, A, X);
+    scan_bins<RS_BINS>(L, L.mass, L.count);
+    find_cross<RS_BINS>(L, L.mass, L.count, before, mbefore, A, X);
     before = L.x_count;
     mbefore = L.x_mass;
-    inside = L.count[L.x_bin < RS_BINS ? L.x_bin : 0];
-    prefix |= (uint64_t)L.x_bin << next;
+    inside = in_bin(L.x_bin);
+    prefix |= (uint64_t)(RS_BINS - 1 - L.x_bin) << next;
     hi_mask = ~((1ull << next) - 1);
     shift = next;
     __syncthreads();
@@ -866,7 +895,7 @@ __device__ __forceinline__ void row_hist(const RowsK &a, PickLds &L, RowHist &h,
   each_logit<RS_T>(a, row, 0, a.n, [&](bool ok, float v, uint32_t) {
     const double w = ok ? row_weight(a, bv, v) : 0.0;
     if (ok && w >= a.min_p) minp += row_mass(a, w);
-    hist_add<true>(L.mass, L.count, ok, ok ? row_bin(a, bv, v) : 0, ok ? order_key(v) : 0, row_mass(a, w));
+    hist_add<true>(L.mass, L.count, ok, ok ? row_bin(a, bv, v) : 0, row_mass(a, w));
   });
   minp = wave_sum_u64(minp);
   if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long *)&L.x_mass, (unsigned long long)minp);
@@ -885,7 +914,7 @@ __device__ __forceinline__ int32_t pick_row(const RowsK &a, PickLds &L, const Ro
     first_token(a, L, h, row, bv, a.top_k, ALL, &S);
   } else {
     load_hist(L, h);
-    S = hist_mass(L);
+    S = L.mass[RS_BINS - 1];
   }
   R = S;
   if (a.top_p < 1.0) first_token(a, L, h, row, bv, ALL, at_least(a.top_p * (double)S, S), &R);
@@ -895,77 +924,98 @@ __device__ __forceinline__ int32_t pick_row(const RowsK &a, PickLds &L, const Ro
 
 // ------------------------------------------------------------------ rows: many
 
-// Resolves the cut `done` from its list (CUT_NONE: there is none yet) and gathers the list of `next` over this
-// workgroup's slice.
-__global__ __launch_bounds__(RS_T) void k_rows_stage(RowsK a, uint32_t done, uint32_t next) {
+// This workgroup's n tokens from LDS into a list of the row, with one atomic on the list's count. Whichever workgroup
+// finds the list full says so.
+__device__ __forceinline__ void put_list(PickLds &L, const uint64_t *from, uint32_t n, uint64_t *list, uint32_t cap, uint32_t *nlist,
+                                         uint32_t *slow) {
+  if (threadIdx.x == 0) L.at = n ? atomicAdd(nlist, n) : 0;
+  __syncthreads();
+  const uint32_t at = L.at;
+  __syncthreads();
+  if (n > RS_CAP || at + n > cap) {
+    if (threadIdx.x == 0) *slow = 1;
+    return;
+  }
+  for (uint32_t j = threadIdx.x; j < n; j += RS_T) list[at + j] = from[j];
+}
+
+__global__ __launch_bounds__(RS_T) void k_rows_topk(RowsK a) {
   extern __shared__ uint64_t pick_lds[];
   PickLds &L = *(PickLds *)pick_lds;
-  constexpr uint64_t ALL = ~0ull;
-  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
   RowHist &h = a.hist[blockIdx.y];
   uint64_t best;
   uint32_t finite;
   row_best(a, h, &best, &finite);
-  if (!finite) return;
-  for (uint32_t e = 0; e < next; e++)  // launches before this one
-    if (h.slow[e]) return;
-  const float bv = comp_value(best);
-  const bool cut_k = a.top_k && a.top_k < finite;
+  if (a.top_k >= finite) return;
   load_hist(L, h);
-  const uint64_t total = hist_mass(L);
-  // the weight that the cut `done` leaves: up to and with its token
-  auto resolve = [&](uint32_t cut, uint64_t A, uint64_t X) -> uint64_t {
-    uint64_t m;
-    find_cross(L, false, 0, 0, A, X);
-    const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[cut], RS_CAP);
-    const uint64_t mbefore = L.x_mass;
-    for (uint32_t j = tid; j < n; j += RS_T) L.part[j] = h.list[cut][j];
-    cut_list(a, L, bv, bin, n, before, mbefore, A, X, &m);
-    load_hist(L, h);  // cut_list used its place
-    return m;
-  };
-  uint64_t S = done == CUT_P ? h.s : total, R = 0;
-  if (done == CUT_K && cut_k) S = resolve(CUT_K, a.top_k, ALL);
-  const uint64_t X = at_least(a.top_p * (double)S, S);
-  if (done == CUT_P) R = resolve(CUT_P, ALL, X);
-  else R = S;
-  uint64_t A = ALL, to = ALL;
-  if (next == CUT_K) {
-    if (!cut_k) return;
-    A = a.top_k;
-  } else if (next == CUT_P) {
-    to = X;
-    if (blockIdx.x == 0 && tid == 0) h.s = S;
-  } else {
-    R = min(R, h.minp);
-    to = at_least(a.uniforms[blockIdx.y] * (double)R, R);
-    if (blockIdx.x == 0 && tid == 0) h.target = to;
-  }
-  find_cross(L, false, 0, 0, A, to);
-  const uint32_t bin = L.x_bin;
-  // this slice's tokens of the bin, in LDS first: one atomic on the list's count per workgroup
-  if (tid == 0) L.nlist = 0;
+  find_cross(L, a.top_k, ~0ull);
+  const uint32_t bin = L.x_bin, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const float bv = comp_value(best);
+  if (threadIdx.x == 0) L.nlist = 0;
   __syncthreads();
   each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t i) {
     append(L.list, &L.nlist, ok && row_bin(a, bv, v) == bin, composite(v, i));
   });
   __syncthreads();
-  const uint32_t n = L.nlist;
-  if (tid == 0) L.at = n ? atomicAdd(&h.nlist[next], n) : 0;
-  __syncthreads();
-  const uint32_t to_at = L.at;
-  if (n > RS_CAP || to_at + n > RS_CAP) {  // the list is full, whichever workgroup sees it
-    if (tid == 0) h.slow[next] = 1;
-    return;
-  }
-  for (uint32_t j = tid; j < n; j += RS_T) h.list[next][to_at + j] = L.list[j];
+  put_list(L, L.list, L.nlist, h.list[CUT_K], RS_CAP, &h.nlist[CUT_K], &h.slow[0]);
 }
 
-// The token: the best where nothing is drawn, else from the draw's list.
+// The weight that the top-k cut leaves, from its list.
+__device__ __forceinline__ uint64_t topk_mass(const RowsK &a, PickLds &L, const RowHist &h, float bv) {
+  uint64_t m;
+  find_cross(L, a.top_k, ~0ull);
+  const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[CUT_K], RS_CAP);
+  const uint64_t mbefore = L.x_mass;
+  for (uint32_t j = threadIdx.x; j < n; j += RS_T) L.part[j] = h.list[CUT_K][j];
+  cut_list(a, L, bv, bin, n, before, mbefore, a.top_k, ~0ull, &m);
+  return m;
+}
+
+__global__ __launch_bounds__(RS_T) void k_rows_cuts(RowsK a) {
+  extern __shared__ uint64_t pick_lds[];
+  PickLds &L = *(PickLds *)pick_lds;
+  RowHist &h = a.hist[blockIdx.y];
+  uint64_t best;
+  uint32_t finite;
+  row_best(a, h, &best, &finite);
+  const double u = a.uniforms[blockIdx.y];
+  if (!finite || h.slow[0] || !(u > 0.0 && u < 1.0)) return;  // slow[0]: of the launch before
+  const float bv = comp_value(best);
+  load_hist(L, h);
+  const uint64_t S = a.top_k && a.top_k < finite ? topk_mass(a, L, h, bv) : L.mass[RS_BINS - 1];
+  if (blockIdx.x == 0 && threadIdx.x == 0) h.s = S;
+  uint64_t least = S, most = S;  // of the weight that top-p keeps
+  uint32_t pbin = RS_BINS;       // none
+  if (a.top_p < 1.0) {
+    least = at_least(a.top_p * (double)S, S);
+    find_cross(L, ~0ull, least);
+    pbin = min(L.x_bin, RS_BINS - 1);
+    most = min(L.mass[pbin], S);
+  }
+  least = min(least, h.minp);
+  most = min(most, h.minp);
+  find_cross(L, ~0ull, at_least(u * (double)least, least));
+  const uint32_t b0 = L.x_bin;
+  find_cross(L, ~0ull, at_least(u * (double)most, most));
+  const uint32_t b1 = L.x_bin, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  if (threadIdx.x == 0) L.nlist = L.npart = 0;
+  __syncthreads();
+  each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t i) {
+    const uint32_t b = ok ? row_bin(a, bv, v) : RS_BINS + 1;
+    append(L.list, &L.nlist, b == pbin, composite(v, i));
+    append(L.part, &L.npart, b >= b0 && b <= b1, composite(v, i));
+  });
+  __syncthreads();
+  put_list(L, L.list, L.nlist, h.list[CUT_P], RS_CAP, &h.nlist[CUT_P], &h.slow[1]);
+  put_list(L, L.part, L.npart, h.draw, RS_DRAW, &h.nlist[CUT_DRAW], &h.slow[1]);
+}
+
+// The token: the best where nothing is drawn, else from the lists.
 __global__ __launch_bounds__(RS_T) void k_rows_last(RowsK a, uint32_t drawn) {
   extern __shared__ uint64_t pick_lds[];
   PickLds &L = *(PickLds *)pick_lds;
   RowHist &h = a.hist[blockIdx.x];
+  const uint32_t tid = threadIdx.x;
   uint64_t best;
   uint32_t finite;
   row_best(a, h, &best, &finite);
@@ -973,20 +1023,42 @@ __global__ __launch_bounds__(RS_T) void k_rows_last(RowsK a, uint32_t drawn) {
   int32_t token = finite ? (int32_t)comp_index(best) : -1;
   if (finite && drawn && u > 0.0 && u < 1.0) {
     const float bv = comp_value(best);
-    if (h.slow[0] || h.slow[1] || h.slow[2]) {
+    if (h.slow[0] || h.slow[1]) {
       row_hist(a, L, h, a.logits + blockIdx.x * a.stride, bv);
       token = pick_row(a, L, h, a.logits + blockIdx.x * a.stride, bv, finite, u);
     } else {
-      uint64_t unused;
+      uint64_t R = h.s, unused;
       load_hist(L, h);
-      find_cross(L, false, 0, 0, ~0ull, h.target);
-      const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[CUT_DRAW], RS_CAP);
+      if (a.top_p < 1.0) {
+        const uint64_t X = at_least(a.top_p * (double)R, R);
+        find_cross(L, ~0ull, X);
+        const uint32_t bin = min(L.x_bin, RS_BINS - 1), n = min(h.nlist[CUT_P], RS_CAP);
+        const uint64_t mbefore = L.x_mass;
+        for (uint32_t j = tid; j < n; j += RS_T) L.part[j] = h.list[CUT_P][j];
+        cut_list(a, L, bv, bin, n, 0, mbefore, ~0ull, X, &R);
+      }
+      R = min(R, h.minp);
+      const uint64_t target = at_least(u * (double)R, R);
+      find_cross(L, ~0ull, target);
+      const uint32_t bin = L.x_bin, n = min(h.nlist[CUT_DRAW], RS_DRAW);
       const uint64_t mbefore = L.x_mass;
-      for (uint32_t j = threadIdx.x; j < n; j += RS_T) L.part[j] = h.list[CUT_DRAW][j];
-      token = (int32_t)comp_index(cut_list(a, L, bv, bin, n, before, mbefore, ~0ull, h.target, &unused));
+      if (tid == 0) L.nlist = 0;
+      __syncthreads();
+      for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {  // the one bin of those in the list
+        const uint64_t c = j0 + tid < n ? h.draw[j0 + tid] : 0;
+        append(L.part, &L.nlist, j0 + tid < n && row_bin(a, bv, comp_value(c)) == bin, c);
+      }
+      __syncthreads();
+      const uint32_t np = min(L.nlist, RS_CAP);
+      if (L.nlist > RS_CAP) {  // a bin with more tokens than cut_list takes
+        row_hist(a, L, h, a.logits + blockIdx.x * a.stride, bv);
+        token = pick_row(a, L, h, a.logits + blockIdx.x * a.stride, bv, finite, u);
+      } else {
+        token = (int32_t)comp_index(cut_list(a, L, bv, bin, np, 0, mbefore, ~0ull, target, &unused));
+      }
     }
   }
-  if (threadIdx.x == 0) a.tokens[blockIdx.x] = token;
+  if (tid == 0) a.tokens[blockIdx.x] = token;
 }
 
 // ------------------------------------------------------------------ rows: few
@@ -1061,8 +1133,8 @@ __global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
 #pragma unroll
     for (uint32_t e = 0; e < PER; e++)
       if (key[e]) atomicAdd(&L.count[row_bin(a, bv, comp_value((uint64_t)key[e] << 32))], 1u);
-    __syncthreads();
-    find_cross(L, false, 0, 0, a.top_k, ~0ull);
+    scan_bins<RS_BINS>(L, L.mass, L.count);
+    find_cross(L, a.top_k, ~0ull);
     // what lies in the last bin has no weight: without top_k groups before it, the tokens before it are all that count
     const uint32_t bound = min(L.x_bin, RS_BINS - 2);
 #pragma unroll
@@ -1147,6 +1219,8 @@ hipError_t sample_rows(hipStream_t s, const SampleRowsArgs &in) {
   a.n = in.n; a.stride = in.stride;
   a.slice = (std::max(RS_SLICE, (in.n + RS_SLICES - 1) / RS_SLICES) + 3) & ~3u;
   a.nslices = (in.n + a.slice - 1) / a.slice;
+  a.bslice = (std::max(4096u, (in.n + RS_SLICES - 1) / RS_SLICES) + 3) & ~3u;
+  a.bslices = (in.n + a.bslice - 1) / a.bslice;
   a.steps = group_steps(in.n); a.ngroups = group_count(in.n);
   a.aligned = (uintptr_t)in.logits % 16 == 0 && in.stride % 4 == 0;
   a.hist = (RowHist *)in.scratch;
@@ -1155,10 +1229,11 @@ hipError_t sample_rows(hipStream_t s, const SampleRowsArgs &in) {
   a.top_p = in.top_p; a.min_p = in.min_p; a.top_k = in.top_k;
   int log2n = 0;
   while (log2n < 32 && (1ull << log2n) < in.n) log2n++;
-  a.unit = std::ldexp(1.0, 62 - log2n);
+  a.unit = std::ldexp(1.0, std::min(51, 62 - log2n));
   // a temperature near 0 has no finite scale: any large one keeps the bins monotonic
   a.bins = in.temperature > 0.0 ? (float)std::min(1e30, RS_BINS / (RS_SPAN * in.temperature)) : 0.f;
-  lds_opt_in((const void *)k_rows_stage);
+  lds_opt_in((const void *)k_rows_topk);
+  lds_opt_in((const void *)k_rows_cuts);
   lds_opt_in((const void *)k_rows_last);
   lds_opt_in((const void *)k_rows_few);
   const bool drawn = in.temperature != 0.0 && in.top_k != 1;
@@ -1174,19 +1249,18 @@ hipError_t sample_rows(hipStream_t s, const SampleRowsArgs &in) {
       continue;
     }
     const dim3 grid(a.nslices, nr);
-    hipLaunchKernelGGL(k_rows_best, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL(k_rows_best, dim3(a.bslices, nr), dim3(256), 0, s, a);
     WGD_HIP(hipGetLastError());
     if (drawn) {
       if (in.top_k && in.top_k < in.n) hipLaunchKernelGGL(k_rows_hist<true>, grid, dim3(RS_T), 0, s, a);
       else hipLaunchKernelGGL(k_rows_hist<false>, grid, dim3(RS_T), 0, s, a);
       WGD_HIP(hipGetLastError());
-      uint32_t done = CUT_NONE;
-      for (uint32_t next = CUT_K; next <= CUT_DRAW; next++) {
-        if ((next == CUT_K && (!in.top_k || in.top_k >= in.n)) || (next == CUT_P && in.top_p >= 1.0)) continue;
-        hipLaunchKernelGGL(k_rows_stage, grid, dim3(RS_T), sizeof(PickLds), s, a, done, next);
+      if (in.top_k && in.top_k < in.n) {
+        hipLaunchKernelGGL(k_rows_topk, grid, dim3(RS_T), sizeof(PickLds), s, a);
         WGD_HIP(hipGetLastError());
-        done = next;
       }
+      hipLaunchKernelGGL(k_rows_cuts, grid, dim3(RS_T), sizeof(PickLds), s, a);
+      WGD_HIP(hipGetLastError());
     }
     hipLaunchKernelGGL(k_rows_last, dim3(nr), dim3(RS_T), sizeof(PickLds), s, a, drawn ? 1u : 0u);
     WGD_HIP(hipGetLastError());
