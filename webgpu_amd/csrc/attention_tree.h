@@ -956,22 +956,29 @@ static TreePlan tree_plan(const TreeAttnArgs &in) {
     p.RT = p.staged && p.HD <= 128 ? 2 : 1;
     p.waves = p.staged || p.HD <= 128 ? 8 : 4;
     const uint32_t groups = (tiles + p.RT - 1) / p.RT;
-    // row groups of a staged workgroup: four read the keys half as often, but two leave fewer wavefronts without rows
-    // and more slices; hd 128, 16 tiles: 31000 keys 80 us with four, 85 with two; 4000 keys 26.2 and 24.6
-    p.rw = !p.staged ? 1 : keys >= 8000 && (groups >= 8 || (p.HD == 256 && groups >= 4)) ? 4 : 2;
-    const uint32_t slices = p.waves / p.rw, kb = (keys + unit - 1) / unit;
-    p.blocks = (groups + p.rw - 1) / p.rw;
-    // Splits by estimated time (us): a CU has one workgroup at a time; it starts and ends in 4.5 and works 2.1
-    // (f16) or 3.1 (f32) for a block of each slice; the join adds 3.3. hd 128, 8 kv heads, one node: f16 300 keys 8.9 in one
-    // split, 11.3 in two; 1000 keys 14.9 and 13.7, 11.9 in four; f32 300 keys 13.2 in one, 12.3 in three.
-    const uint32_t wgs = in.kv_heads * p.blocks, rounds = (kb + slices - 1) / slices;
+    // Splits, and the row groups of a workgroup, by estimated time (us): a CU has one workgroup at a time; it starts and
+    // ends in 4.5 and works 2.1 (f16) or 3.1 (f32) for a block of each slice; the join adds 3.3. hd 128, 8 kv heads, one
+    // node: f16 300 keys 8.9 in one split, 11.3 in two; 1000 keys 14.9 and 13.7, 11.9 in four; f32 300 keys 13.2
+    // in one, 12.3 in three; f32 1071 keys of 16 kv heads, 6 tiles: 24.4 us with one row group in two splits, 22.7 with two
+    // in five.
+    const uint32_t kb = (keys + unit - 1) / unit;
     const double block = in.kv16 ? 2.1 : 3.1;
     uint32_t want = 1;
     double best = 1e30;
-    for (uint32_t n = 1; n <= std::min(rounds, TREE_SPLITS); n++) {
-      const uint32_t per = (kb + n - 1) / n, deep = (per + slices - 1) / slices;
-      const double t = (double)(((uint64_t)wgs * n + cus - 1) / cus) * (4.5 + block * deep) + (n > 1 ? 3.3 : 0);
-      if (t < best) { best = t; want = n; }
+    auto splits = [&](uint32_t rw) {
+      const uint32_t blocks = (groups + rw - 1) / rw, wgs = in.kv_heads * blocks, slices = p.waves / rw;
+      for (uint32_t n = 1; n <= std::min((kb + slices - 1) / slices, TREE_SPLITS); n++) {
+        const uint32_t per = (kb + n - 1) / n, deep = (per + slices - 1) / slices;
+        const double t = (double)(((uint64_t)wgs * n + cus - 1) / cus) * (4.5 + block * deep) + (n > 1 ? 3.3 : 0);
+        if (t < best) { best = t; want = n; p.rw = rw; p.blocks = blocks; }
+      }
+    };
+    if (p.staged) {
+      // four row groups read the keys half as often, but two leave fewer wavefronts without rows and more slices; hd
+      // 128, 16 tiles: 31000 keys 80 us with four, 85 with two; 4000 keys 26.2 and 24.6
+      splits(keys >= 8000 && (groups >= 8 || (p.HD == 256 && groups >= 4)) ? 4 : 2);
+    } else {
+      for (uint32_t rw = 1; rw <= 4 && rw <= groups; rw *= 2) splits(rw);
     }
     p.per = (kb + want - 1) / want;
     p.nsplit = (kb + p.per - 1) / p.per;
