@@ -478,7 +478,7 @@ hipError_t sample(hipStream_t s, const float *logits, uint32_t n, const SamplePa
 // A cut's token is found in its list by a histogram of RS_SUB parts of the bin and a sort of the one part
 // that holds it (a sort of the whole list took four times as long).
 // A bin or bound with more tokens than a list holds (ties, logits close together for the temperature) goes through
-// pick_row, which refines by 12 bits of the composite at a time, in one workgroup.
+// pick_row, which refines by 11 bits of the composite at a time, in one workgroup.
 constexpr uint32_t RS_T = 512, RS_BINS = 2048, RS_CAP = 2048, RS_DRAW = 8192, RS_SUB = 1024;
 constexpr uint32_t RS_ROWS = 256;  // rows per launch: the histograms of more would only fill memory
 constexpr float RS_SPAN = 48.f;    // bins cover exp(0) to exp(-48) < 2^-62; the last one all below
@@ -541,6 +541,45 @@ __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
 __device__ __forceinline__ float wave_max_f(float v) {
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   return v;
+}
+// The values of the lanes up to and with this one, combined: row_shr 1, 2, 4, 8, then row_bcast15 into rows 1 and 3 and
+// row_bcast31 into rows 2 and 3. Lanes without a source take 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+  return (uint64_t)dpp_u32<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp_u32<CTRL, ROWS>((uint32_t)v);
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  v += dpp_u64<0x111, 0xf>(v);
+  v += dpp_u64<0x112, 0xf>(v);
+  v += dpp_u64<0x114, 0xf>(v);
+  v += dpp_u64<0x118, 0xf>(v);
+  v += dpp_u64<0x142, 0xa>(v);
+  v += dpp_u64<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+  v += dpp_u32<0x111, 0xf>(v);
+  v += dpp_u32<0x112, 0xf>(v);
+  v += dpp_u32<0x114, 0xf>(v);
+  v += dpp_u32<0x118, 0xf>(v);
+  v += dpp_u32<0x142, 0xa>(v);
+  v += dpp_u32<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_top_u32(uint32_t v) {  // the largest, in every lane
+  v = max(v, dpp_u32<0x111, 0xf>(v));
+  v = max(v, dpp_u32<0x112, 0xf>(v));
+  v = max(v, dpp_u32<0x114, 0xf>(v));
+  v = max(v, dpp_u32<0x118, 0xf>(v));
+  v = max(v, dpp_u32<0x142, 0xa>(v));
+  v = max(v, dpp_u32<0x143, 0xc>(v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, uint32_t lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), (int)lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, (int)lane);
 }
 // At least x and 1, at most `most`.
 __device__ __forceinline__ uint64_t at_least(double x, uint64_t most) { return min(max((uint64_t)ceil(x), (uint64_t)1), most); }
@@ -662,23 +701,6 @@ struct PickLds {
   uint32_t x_bin, x_count, nlist, npart, at;
 };
 
-// The sum of v over this lane and the ones below it.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
-  return (uint64_t)hi << 32 | lo;
-}
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
-  v += dpp_u64<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
-  v += dpp_u64<0x112, 0xf>(v);
-  v += dpp_u64<0x114, 0xf>(v);
-  v += dpp_u64<0x118, 0xf>(v);
-  v += dpp_u64<0x142, 0xa>(v);  // row_bcast15 into rows 1 and 3
-  v += dpp_u64<0x143, 0xc>(v);  // row_bcast31 into rows 2 and 3
-  return v;
-}
-
 // Running sums of the bins, in place.
 template <uint32_t BINS>
 __device__ __forceinline__ void scan_bins(PickLds &L, uint64_t *mass, uint32_t *count) {
@@ -692,15 +714,17 @@ __device__ __forceinline__ void scan_bins(PickLds &L, uint64_t *mass, uint32_t *
     m[e] = ms += mass[PER * tid + e];
     c[e] = cs += count[PER * tid + e];
   }
-  const uint64_t mi = wave_scan_u64(ms), ci = wave_scan_u64(cs);
-  if (lane == 63) { L.wmass[wv] = mi; L.wcount[wv] = (uint32_t)ci; }
+  const uint64_t mi = wave_scan_u64(ms);
+  const uint32_t ci = wave_scan_u32(cs);
+  if (lane == 63) { L.wmass[wv] = mi; L.wcount[wv] = ci; }
   __syncthreads();
-  uint64_t mb = mi - ms, cb = ci - cs;
+  uint64_t mb = mi - ms;
+  uint32_t cb = ci - cs;
   for (uint32_t w = 0; w < wv; w++) { mb += L.wmass[w]; cb += L.wcount[w]; }
 #pragma unroll
   for (uint32_t e = 0; e < PER; e++) {
     mass[PER * tid + e] = mb + m[e];
-    count[PER * tid + e] = (uint32_t)cb + c[e];
+    count[PER * tid + e] = cb + c[e];
   }
   __syncthreads();
 }
@@ -778,7 +802,7 @@ __device__ __forceinline__ void sort_list(const RowsK &a, PickLds &L, float bv) 
 __device__ __forceinline__ uint32_t find_place(PickLds &L, uint64_t mass0, uint64_t A, uint64_t X) {
   const uint32_t nl = min(L.nlist, RS_CAP);
   __syncthreads();
-  if (threadIdx.x == 0) L.at = nl - 1;
+  if (threadIdx.x == 0) L.at = max(nl, 1u) - 1;
   __syncthreads();
   for (uint32_t j = threadIdx.x; j < nl; j += RS_T)
     if (j + 1 >= A || mass0 + L.cum[j] >= X) { atomicMin(&L.at, j); break; }
@@ -800,7 +824,7 @@ __device__ __forceinline__ void append(uint64_t *list, uint32_t *nlist, bool tak
   const uint32_t lane = threadIdx.x & 63;
   uint32_t base = 0;
   if (lane == 0) base = atomicAdd(nlist, (uint32_t)__popcll(m));
-  base = __shfl(base, 0) + (uint32_t)__popcll(m & ((1ull << lane) - 1));
+  base = (uint32_t)__builtin_amdgcn_readfirstlane((int)base) + (uint32_t)__popcll(m & ((1ull << lane) - 1));
   if (take && base < RS_CAP) list[base] = c;
 }
 
@@ -1084,11 +1108,44 @@ __global__ __launch_bounds__(RG_T) void k_rows_groups(RowsK a) {
   if ((lane & 3) == 0) a.groups[blockIdx.y].key[16 * part + lane / 4] = key;
 }
 
+// The token of a row whose candidates, L.list[0 .. nl) with 0 < nl <= 64, fit a wavefront: all cuts, in this one.
+__device__ __forceinline__ int32_t pick_wave(const RowsK &a, const PickLds &L, float bv, double u, uint32_t nl) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint64_t c = lane < nl ? L.list[lane] : 0;
+  uint32_t rank = 0;
+#pragma unroll 8
+  for (uint32_t j = 0; j < nl; j++) rank += L.list[j] > c ? 1u : 0u;
+  if (lane >= nl) rank = lane;
+  c = (uint64_t)(uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)(uint32_t)(c >> 32)) << 32 |
+      (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)(uint32_t)c);
+  uint32_t at = 0;
+  if (u > 0.0 && u < 1.0) {
+    const double w = lane < nl ? row_weight(a, bv, comp_value(c)) : 0.0;
+    const uint64_t cum = wave_scan_u64(row_mass(a, w));
+    // the first lane at which the running weight reaches x, the last candidate if none does
+    auto place = [&](uint64_t x) {
+      const uint64_t m = __ballot(lane < nl && cum >= x);
+      return m ? (uint32_t)__builtin_ctzll(m) : nl - 1;
+    };
+    uint32_t last = (a.top_k ? min(a.top_k, nl) : nl) - 1;
+    const uint64_t S = lane_u64(cum, last);
+    if (a.top_p < 1.0) last = min(last, place(at_least(a.top_p * (double)S, S)));
+    if (a.min_p > 0.0) {  // weights fall along the lanes
+      const uint32_t kept = (uint32_t)__popcll(__ballot(lane <= last && w >= a.min_p));
+      last = min(last, max(kept, 1u) - 1);
+    }
+    const uint64_t R = lane_u64(cum, last);
+    at = place(at_least(u * (double)R, R));
+  }
+  return (int32_t)comp_index(lane_u64(c, at));
+}
+
 __global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
   extern __shared__ uint64_t pick_lds[];
   PickLds &L = *(PickLds *)pick_lds;
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const float *row = a.logits + blockIdx.x * a.stride;
+  const double u = a.uniforms[blockIdx.x];
   float bv = 0.f;
   if (a.n <= RS_CAP) {
     if (tid == 0) L.nlist = 0;
@@ -1114,15 +1171,15 @@ __global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
     const uint32_t *keys = a.groups[blockIdx.x].key;
     constexpr uint32_t PER = RS_GROUPS / RS_T;
     uint32_t key[PER], top_key = 0;
+    for (uint32_t b = tid; b < RS_BINS; b += RS_T) L.count[b] = 0;
+    if (tid == 0) { L.nlist = 0; L.at = 0; L.x_bin = RS_BINS; }
 #pragma unroll
     for (uint32_t e = 0; e < PER; e++) {
       key[e] = e * RS_T + tid < a.ngroups ? keys[e * RS_T + tid] : 0;
       top_key = max(top_key, key[e]);
     }
-    for (int o = 32; o > 0; o >>= 1) top_key = max(top_key, (uint32_t)__shfl_xor((int)top_key, o));
+    top_key = wave_top_u32(top_key);
     if (lane == 0) L.wcount[tid >> 6] = top_key;
-    for (uint32_t b = tid; b < RS_BINS; b += RS_T) { L.count[b] = 0; L.mass[b] = 0; }
-    if (tid == 0) { L.nlist = 0; L.at = 0; }
     __syncthreads();
     for (uint32_t w = 0; w < RS_T / 64; w++) top_key = max(top_key, L.wcount[w]);
     if (!top_key) {  // nothing finite
@@ -1133,8 +1190,21 @@ __global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
 #pragma unroll
     for (uint32_t e = 0; e < PER; e++)
       if (key[e]) atomicAdd(&L.count[row_bin(a, bv, comp_value((uint64_t)key[e] << 32))], 1u);
-    scan_bins<RS_BINS>(L, L.mass, L.count);
-    find_cross(L, a.top_k, ~0ull);
+    __syncthreads();
+    // the bin at which their running count reaches top_k
+    constexpr uint32_t B = RS_BINS / RS_T;
+    uint32_t c[B], upto = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < B; e++) c[e] = upto += L.count[B * tid + e];
+    const uint32_t incl = wave_scan_u32(upto);
+    if (lane == 63) L.scount[tid >> 6] = incl;
+    __syncthreads();
+    uint32_t before = incl - upto;
+    for (uint32_t w = 0; w < tid >> 6; w++) before += L.scount[w];
+#pragma unroll
+    for (uint32_t e = 0; e < B; e++)
+      if (before + c[e] >= a.top_k && before + (e ? c[e - 1] : 0) < a.top_k) L.x_bin = B * tid + e;
+    __syncthreads();
     // what lies in the last bin has no weight: without top_k groups before it, the tokens before it are all that count
     const uint32_t bound = min(L.x_bin, RS_BINS - 2);
 #pragma unroll
@@ -1146,8 +1216,24 @@ __global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
       const uint32_t i = i0 + tid, j = i < pieces ? chosen[i / (4 * a.steps)] : 0, in = i % (4 * a.steps);
       const uint32_t at = (j / 16) * a.steps * RG_STEP + (in / 4) * RG_STEP + (j % 16) * 16 + (in % 4) * 4;
       const float4 v = i < pieces ? row_load4(a, row, at) : make_float4(NAN, NAN, NAN, NAN);
-      auto put = [&](float x, uint32_t e) { append(L.list, &L.nlist, finite_f(x) && row_bin(a, bv, x) <= bound, composite(x, at + e)); };
-      put(v.x, 0); put(v.y, 1); put(v.z, 2); put(v.w, 3);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      uint64_t take[4];
+      uint32_t n = 0;
+#pragma unroll
+      for (uint32_t e = 0; e < 4; e++) {
+        take[e] = __ballot(finite_f(x[e]) && row_bin(a, bv, x[e]) <= bound);
+        n += (uint32_t)__popcll(take[e]);
+      }
+      if (!n) continue;
+      uint32_t to = 0;
+      if (lane == 0) to = atomicAdd(&L.nlist, n);
+      to = (uint32_t)__builtin_amdgcn_readfirstlane((int)to);
+#pragma unroll
+      for (uint32_t e = 0; e < 4; e++) {
+        const uint32_t place = to + (uint32_t)__popcll(take[e] & ((1ull << lane) - 1));
+        if ((take[e] >> lane & 1) && place < RS_CAP) L.list[place] = composite(x[e], at + e);
+        to += (uint32_t)__popcll(take[e]);
+      }
     }
     __syncthreads();
   }
@@ -1168,12 +1254,16 @@ __global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
     uint32_t finite = 0;
     for (uint32_t w = 0; w < RS_T / 64; w++) { best = max(best, L.wmass[w]); finite += L.wcount[w]; }
     row_hist(a, L, h, row, bv);
-    const double u = a.uniforms[blockIdx.x];
     const int32_t token = u > 0.0 && u < 1.0 ? pick_row(a, L, h, row, bv, finite, u) : (int32_t)comp_index(best);
     if (tid == 0) a.tokens[blockIdx.x] = token;
     return;
   }
-  const double u = a.uniforms[blockIdx.x];
+  if (nl <= 64) {
+    if (tid >= 64) return;
+    const int32_t token = pick_wave(a, L, bv, u, nl);
+    if (tid == 0) a.tokens[blockIdx.x] = token;
+    return;
+  }
   sort_list(a, L, bv);
   int32_t token = (int32_t)comp_index(L.list[0]);
   if (u > 0.0 && u < 1.0) {
