@@ -494,6 +494,8 @@ struct RowHist {
   uint64_t list[2][RS_CAP], draw[RS_DRAW];  // of top-k, top-p and the draw
   uint32_t nlist[3], slow[2];                // slow: k_rows_topk or k_rows_cuts has a list that is full
   uint64_t minp, s;                          // the weights that min-p and top-k keep
+  uint64_t pmass, dmass;                     // the weights before top-p's bin and before the draw's bins b0 .. b1
+  uint32_t pbin, b0, b1;
   RowSlice slice[RS_SLICES];
 };
 struct RowGroups { uint32_t key[RS_GROUPS]; };
@@ -797,6 +799,24 @@ __device__ __forceinline__ void sort_list(const RowsK &a, PickLds &L, float bv) 
   __syncthreads();
 }
 
+// L.list[0 .. nl) with nl <= 64 in descending order, one token a lane of this wavefront, each with its weight and the
+// running weights.
+struct WaveList { uint64_t c, cum; double w; };
+__device__ __forceinline__ WaveList wave_list(const RowsK &a, const PickLds &L, float bv, uint32_t nl) {
+  const uint32_t lane = threadIdx.x & 63;
+  WaveList t;
+  t.c = lane < nl ? L.list[lane] : 0;
+  uint32_t rank = 0;
+#pragma unroll 8
+  for (uint32_t j = 0; j < nl; j++) rank += L.list[j] > t.c ? 1u : 0u;
+  if (lane >= nl) rank = lane;
+  t.c = (uint64_t)(uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)(uint32_t)(t.c >> 32)) << 32 |
+        (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)(uint32_t)t.c);
+  t.w = lane < nl ? row_weight(a, bv, comp_value(t.c)) : 0.0;
+  t.cum = wave_scan_u64(row_mass(a, t.w));
+  return t;
+}
+
 // The place in L.list at which the running count (1 for the first) reaches A or mass0 and the running
 // weight reach X; the last place if none does.
 __device__ __forceinline__ uint32_t find_place(PickLds &L, uint64_t mass0, uint64_t A, uint64_t X) {
@@ -828,38 +848,58 @@ __device__ __forceinline__ void append(uint64_t *list, uint32_t *nlist, bool tak
   if (take && base < RS_CAP) list[base] = c;
 }
 
-// The first of the n tokens in L.part (one bin's, in any order) whose running count, from `before` on, reaches A or whose
-// running weight, from mbefore on, reaches X (the last if none does): its composite, and the weight up to and with it.
-__device__ __forceinline__ uint64_t cut_list(const RowsK &a, PickLds &L, float bv, uint32_t bin, uint32_t n, uint32_t before, uint64_t mbefore,
-                                             uint64_t A, uint64_t X, uint64_t *mass) {
-  auto part = [&](uint64_t c) {  // monotonic within the bin, as row_bin is
-    const float x = (bv - comp_value(c)) * a.bins - (float)bin;
-    return (uint32_t)fminf(fmaxf(x, 0.f) * (float)RS_SUB, (float)(RS_SUB - 1));
+// The first token of L.list whose running count (1 for the first) reaches A or mass0 and the running weight reach X (the
+// last if none does): its composite, and the weight up to and with it.
+__device__ __forceinline__ uint64_t cut_sorted(const RowsK &a, PickLds &L, float bv, uint64_t mass0, uint64_t A, uint64_t X, uint64_t *mass) {
+  const uint32_t nl = min(L.nlist, RS_CAP), lane = threadIdx.x & 63;
+  if (nl > 64) {
+    sort_list(a, L, bv);
+    const uint32_t at = find_place(L, mass0, A, X);
+    *mass = mass0 + L.cum[at];
+    return L.list[at];
+  }
+  if (threadIdx.x < 64) {
+    const WaveList t = wave_list(a, L, bv, nl);
+    const uint64_t m = __ballot(lane < nl && (lane + 1 >= A || mass0 + t.cum >= X));
+    if (lane == (m ? (uint32_t)__builtin_ctzll(m) : max(nl, 1u) - 1)) { L.cum[0] = t.cum; L.part[0] = t.c; }
+  }
+  __syncthreads();
+  *mass = mass0 + L.cum[0];
+  return L.part[0];
+}
+
+// The same of n tokens in memory, in any order and with the bins b0 .. b1, before which lie the count `before` and the
+// weight mbefore. *ok is off if too many tokens lie in one part of the bins.
+__device__ __forceinline__ uint64_t cut_list(const RowsK &a, PickLds &L, float bv, const uint64_t *from, uint32_t n, uint32_t b0, uint32_t b1,
+                                             uint32_t before, uint64_t mbefore, uint64_t A, uint64_t X, uint64_t *mass, bool *ok) {
+  const float parts = (float)RS_SUB / (float)(b1 - b0 + 1);
+  auto part = [&](uint64_t c) {  // monotonic, as row_bin is
+    const float x = (bv - comp_value(c)) * a.bins - (float)b0;
+    return (uint32_t)fminf(fmaxf(x, 0.f) * parts, (float)(RS_SUB - 1));
   };
   __syncthreads();
-  for (uint32_t b = threadIdx.x; b < RS_SUB; b += RS_T) { L.smass[b] = 0; L.scount[b] = 0; }
   if (threadIdx.x == 0) L.nlist = 0;
-  __syncthreads();
-  for (uint32_t j = threadIdx.x; j < n; j += RS_T) {
-    const uint64_t c = L.part[j];
-    hist_add<true>(L.smass, L.scount, true, part(c), row_mass(a, row_weight(a, bv, comp_value(c))));
+  if (n <= 64) {
+    if (threadIdx.x < n) L.list[threadIdx.x] = from[threadIdx.x];
+    if (threadIdx.x == 0) L.nlist = n;
+  } else {
+    for (uint32_t b = threadIdx.x; b < RS_SUB; b += RS_T) { L.smass[b] = 0; L.scount[b] = 0; }
+    __syncthreads();
+    for (uint32_t j = threadIdx.x; j < n; j += RS_T)
+      hist_add<true>(L.smass, L.scount, true, part(from[j]), row_mass(a, row_weight(a, bv, comp_value(from[j]))));
+    scan_bins<RS_SUB>(L, L.smass, L.scount);
+    find_cross<RS_SUB>(L, L.smass, L.scount, before, mbefore, A, X);
+    const uint32_t sub = L.x_bin;
+    for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {
+      const uint32_t j = j0 + threadIdx.x;
+      const uint64_t c = j < n ? from[j] : 0;
+      append(L.list, &L.nlist, j < n && (sub >= RS_SUB || part(c) == sub), c);
+    }
+    if (sub < RS_SUB) { before = L.x_count; mbefore = L.x_mass; }
   }
-  scan_bins<RS_SUB>(L, L.smass, L.scount);
-  find_cross<RS_SUB>(L, L.smass, L.scount, before, mbefore, A, X);
-  const uint32_t sub = L.x_bin < RS_SUB ? L.x_bin : RS_SUB - 1;
-  const bool found = L.x_bin < RS_SUB;
-  for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {
-    const uint32_t j = j0 + threadIdx.x;
-    const uint64_t c = j < n ? L.part[j] : 0;
-    append(L.list, &L.nlist, j < n && (!found || part(c) == sub), c);
-  }
   __syncthreads();
-  sort_list(a, L, bv);
-  const uint32_t b0 = found ? L.x_count : before;
-  const uint64_t m0 = found ? L.x_mass : mbefore;
-  const uint32_t at = find_place(L, m0, A > b0 ? A - b0 : 1, X);
-  *mass = m0 + L.cum[at];
-  return L.list[at];
+  *ok = L.nlist <= RS_CAP;
+  return cut_sorted(a, L, bv, mbefore, A > before ? A - before : 1, X, mass);
 }
 
 // ------------------------------------------------------------------ rows: one workgroup, any bins
@@ -903,10 +943,7 @@ __device__ __forceinline__ uint64_t first_token(const RowsK &a, PickLds &L, cons
     append(L.list, &L.nlist, ok && row_bin(a, bv, v) == bin && (c & hi_mask) == prefix, c);
   });
   __syncthreads();
-  sort_list(a, L, bv);
-  const uint32_t at = find_place(L, mbefore, A > before ? A - before : 1, X);
-  *mass = mbefore + L.cum[at];
-  return L.list[at];
+  return cut_sorted(a, L, bv, mbefore, A > before ? A - before : 1, X, mass);
 }
 
 // The row's histogram, and the weight that min-p keeps, by this workgroup alone, into h.
@@ -990,8 +1027,8 @@ __device__ __forceinline__ uint64_t topk_mass(const RowsK &a, PickLds &L, const 
   find_cross(L, a.top_k, ~0ull);
   const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[CUT_K], RS_CAP);
   const uint64_t mbefore = L.x_mass;
-  for (uint32_t j = threadIdx.x; j < n; j += RS_T) L.part[j] = h.list[CUT_K][j];
-  cut_list(a, L, bv, bin, n, before, mbefore, a.top_k, ~0ull, &m);
+  bool ok;  // the list is no longer than cut_list takes
+  cut_list(a, L, bv, h.list[CUT_K], n, bin, bin, before, mbefore, a.top_k, ~0ull, &m, &ok);
   return m;
 }
 
@@ -1007,21 +1044,29 @@ __global__ __launch_bounds__(RS_T) void k_rows_cuts(RowsK a) {
   const float bv = comp_value(best);
   load_hist(L, h);
   const uint64_t S = a.top_k && a.top_k < finite ? topk_mass(a, L, h, bv) : L.mass[RS_BINS - 1];
-  if (blockIdx.x == 0 && threadIdx.x == 0) h.s = S;
-  uint64_t least = S, most = S;  // of the weight that top-p keeps
-  uint32_t pbin = RS_BINS;       // none
+  uint64_t least = S, most = S, pmass = 0;  // of the weight that top-p keeps; before its bin
+  uint32_t pbin = RS_BINS;                  // none
   if (a.top_p < 1.0) {
     least = at_least(a.top_p * (double)S, S);
     find_cross(L, ~0ull, least);
     pbin = min(L.x_bin, RS_BINS - 1);
+    pmass = L.x_mass;
     most = min(L.mass[pbin], S);
   }
   least = min(least, h.minp);
   most = min(most, h.minp);
-  find_cross(L, ~0ull, at_least(u * (double)least, least));
-  const uint32_t b0 = L.x_bin;
-  find_cross(L, ~0ull, at_least(u * (double)most, most));
-  const uint32_t b1 = L.x_bin, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  least = at_least(u * (double)least, least);
+  most = at_least(u * (double)most, most);
+  __syncthreads();
+#pragma unroll
+  for (uint32_t b = threadIdx.x; b < RS_BINS; b += RS_T) {
+    const uint64_t m1 = L.mass[b], mb = b ? L.mass[b - 1] : 0;
+    if (mb < least && m1 >= least) { L.x_bin = b; L.x_mass = mb; }
+    if (mb < most && m1 >= most) L.at = b;
+  }
+  __syncthreads();
+  const uint32_t b0 = L.x_bin, b1 = L.at, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  if (blockIdx.x == 0 && threadIdx.x == 0) { h.s = S; h.pbin = pbin; h.pmass = pmass; h.b0 = b0; h.b1 = b1; h.dmass = L.x_mass; }
   if (threadIdx.x == 0) L.nlist = L.npart = 0;
   __syncthreads();
   each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t i) {
@@ -1047,39 +1092,21 @@ __global__ __launch_bounds__(RS_T) void k_rows_last(RowsK a, uint32_t drawn) {
   int32_t token = finite ? (int32_t)comp_index(best) : -1;
   if (finite && drawn && u > 0.0 && u < 1.0) {
     const float bv = comp_value(best);
-    if (h.slow[0] || h.slow[1]) {
+    bool slow = h.slow[0] || h.slow[1];
+    if (!slow) {
+      uint64_t R = h.s, unused;
+      bool ok;
+      if (a.top_p < 1.0)  // (its list is no longer than cut_list takes)
+        cut_list(a, L, bv, h.list[CUT_P], min(h.nlist[CUT_P], RS_CAP), h.pbin, h.pbin, 0, h.pmass, ~0ull, at_least(a.top_p * (double)R, R), &R, &ok);
+      R = min(R, h.minp);
+      const uint64_t c = cut_list(a, L, bv, h.draw, min(h.nlist[CUT_DRAW], RS_DRAW), h.b0, h.b1, 0, h.dmass, ~0ull, at_least(u * (double)R, R),
+                                  &unused, &ok);
+      slow = !ok;
+      token = (int32_t)comp_index(c);
+    }
+    if (slow) {
       row_hist(a, L, h, a.logits + blockIdx.x * a.stride, bv);
       token = pick_row(a, L, h, a.logits + blockIdx.x * a.stride, bv, finite, u);
-    } else {
-      uint64_t R = h.s, unused;
-      load_hist(L, h);
-      if (a.top_p < 1.0) {
-        const uint64_t X = at_least(a.top_p * (double)R, R);
-        find_cross(L, ~0ull, X);
-        const uint32_t bin = min(L.x_bin, RS_BINS - 1), n = min(h.nlist[CUT_P], RS_CAP);
-        const uint64_t mbefore = L.x_mass;
-        for (uint32_t j = tid; j < n; j += RS_T) L.part[j] = h.list[CUT_P][j];
-        cut_list(a, L, bv, bin, n, 0, mbefore, ~0ull, X, &R);
-      }
-      R = min(R, h.minp);
-      const uint64_t target = at_least(u * (double)R, R);
-      find_cross(L, ~0ull, target);
-      const uint32_t bin = L.x_bin, n = min(h.nlist[CUT_DRAW], RS_DRAW);
-      const uint64_t mbefore = L.x_mass;
-      if (tid == 0) L.nlist = 0;
-      __syncthreads();
-      for (uint32_t j0 = 0; j0 < n; j0 += RS_T) {  // the one bin of those in the list
-        const uint64_t c = j0 + tid < n ? h.draw[j0 + tid] : 0;
-        append(L.part, &L.nlist, j0 + tid < n && row_bin(a, bv, comp_value(c)) == bin, c);
-      }
-      __syncthreads();
-      const uint32_t np = min(L.nlist, RS_CAP);
-      if (L.nlist > RS_CAP) {  // a bin with more tokens than cut_list takes
-        row_hist(a, L, h, a.logits + blockIdx.x * a.stride, bv);
-        token = pick_row(a, L, h, a.logits + blockIdx.x * a.stride, bv, finite, u);
-      } else {
-        token = (int32_t)comp_index(cut_list(a, L, bv, bin, np, 0, mbefore, ~0ull, target, &unused));
-      }
     }
   }
   if (tid == 0) a.tokens[blockIdx.x] = token;
@@ -1111,33 +1138,25 @@ __global__ __launch_bounds__(RG_T) void k_rows_groups(RowsK a) {
 // The token of a row whose candidates, L.list[0 .. nl) with 0 < nl <= 64, fit a wavefront: all cuts, in this one.
 __device__ __forceinline__ int32_t pick_wave(const RowsK &a, const PickLds &L, float bv, double u, uint32_t nl) {
   const uint32_t lane = threadIdx.x & 63;
-  uint64_t c = lane < nl ? L.list[lane] : 0;
-  uint32_t rank = 0;
-#pragma unroll 8
-  for (uint32_t j = 0; j < nl; j++) rank += L.list[j] > c ? 1u : 0u;
-  if (lane >= nl) rank = lane;
-  c = (uint64_t)(uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)(uint32_t)(c >> 32)) << 32 |
-      (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)(uint32_t)c);
+  const WaveList t = wave_list(a, L, bv, nl);
   uint32_t at = 0;
   if (u > 0.0 && u < 1.0) {
-    const double w = lane < nl ? row_weight(a, bv, comp_value(c)) : 0.0;
-    const uint64_t cum = wave_scan_u64(row_mass(a, w));
     // the first lane at which the running weight reaches x, the last candidate if none does
     auto place = [&](uint64_t x) {
-      const uint64_t m = __ballot(lane < nl && cum >= x);
+      const uint64_t m = __ballot(lane < nl && t.cum >= x);
       return m ? (uint32_t)__builtin_ctzll(m) : nl - 1;
     };
     uint32_t last = (a.top_k ? min(a.top_k, nl) : nl) - 1;
-    const uint64_t S = lane_u64(cum, last);
+    const uint64_t S = lane_u64(t.cum, last);
     if (a.top_p < 1.0) last = min(last, place(at_least(a.top_p * (double)S, S)));
     if (a.min_p > 0.0) {  // weights fall along the lanes
-      const uint32_t kept = (uint32_t)__popcll(__ballot(lane <= last && w >= a.min_p));
+      const uint32_t kept = (uint32_t)__popcll(__ballot(lane <= last && t.w >= a.min_p));
       last = min(last, max(kept, 1u) - 1);
     }
-    const uint64_t R = lane_u64(cum, last);
+    const uint64_t R = lane_u64(t.cum, last);
     at = place(at_least(u * (double)R, R));
   }
-  return (int32_t)comp_index(lane_u64(c, at));
+  return (int32_t)comp_index(lane_u64(t.c, at));
 }
 
 __global__ __launch_bounds__(RS_T) void k_rows_few(RowsK a) {
