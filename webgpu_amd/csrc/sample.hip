@@ -593,26 +593,41 @@ __device__ __forceinline__ float4 row_load4(const RowsK &a, const float *row, ui
   return make_float4(i < a.n ? row[i] : none, i + 1 < a.n ? row[i + 1] : none, i + 2 < a.n ? row[i + 2] : none,
                      i + 3 < a.n ? row[i + 3] : none);
 }
-// f(finite, logit, index) over the logits [lo, hi) (lo a multiple of 4), for every thread of T alike.
+// Logits of T threads on their way: 16 a thread, four in a row.
+struct RowQuads { float4 v[4]; };
+template <uint32_t T>
+__device__ __forceinline__ RowQuads load_quads(const RowsK &a, const float *row, uint32_t i0, uint32_t hi) {
+  const float none = __uint_as_float(0x7FC00000u);
+  RowQuads q;
+#pragma unroll
+  for (uint32_t e = 0; e < 4; e++) {
+    const uint32_t i = i0 + 4 * (e * T + threadIdx.x);
+    q.v[e] = i < hi ? row_load4(a, row, i) : make_float4(none, none, none, none);
+  }
+  return q;
+}
+// f(finite, logit, index) over the logits [lo, hi) (lo a multiple of 4), for every thread of T alike. `now` are the first
+// of them, which a caller loads ahead of what it waits for.
+template <uint32_t T, class F>
+__device__ __forceinline__ void each_logit(const RowsK &a, const float *row, uint32_t lo, uint32_t hi, RowQuads now, F f) {
+  for (uint32_t i0 = lo; i0 < hi; i0 += 16 * T) {
+    RowQuads next = {};
+    if (i0 + 16 * T < hi) next = load_quads<T>(a, row, i0 + 16 * T, hi);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e++) {
+      const uint32_t i = i0 + 4 * (e * T + threadIdx.x);
+      const float4 v = now.v[e];
+      f(finite_f(v.x) && i < hi, v.x, i);
+      f(finite_f(v.y) && i + 1 < hi, v.y, i + 1);
+      f(finite_f(v.z) && i + 2 < hi, v.z, i + 2);
+      f(finite_f(v.w) && i + 3 < hi, v.w, i + 3);
+    }
+    now = next;
+  }
+}
 template <uint32_t T, class F>
 __device__ __forceinline__ void each_logit(const RowsK &a, const float *row, uint32_t lo, uint32_t hi, F f) {
-  constexpr uint32_t E = 4;
-  for (uint32_t i0 = lo; i0 < hi; i0 += 4 * T * E) {
-    float4 v[E];
-#pragma unroll
-    for (uint32_t e = 0; e < E; e++) {
-      const uint32_t i = i0 + 4 * (e * T + threadIdx.x);
-      v[e] = i < hi ? row_load4(a, row, i) : make_float4(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
-    }
-#pragma unroll
-    for (uint32_t e = 0; e < E; e++) {
-      const uint32_t i = i0 + 4 * (e * T + threadIdx.x);
-      f(finite_f(v[e].x) && i < hi, v[e].x, i);
-      f(finite_f(v[e].y) && i + 1 < hi, v[e].y, i + 1);
-      f(finite_f(v[e].z) && i + 2 < hi, v[e].z, i + 2);
-      f(finite_f(v[e].w) && i + 3 < hi, v[e].w, i + 3);
-    }
-  }
+  each_logit<T>(a, row, lo, hi, load_quads<T>(a, row, lo, hi), f);
 }
 
 __global__ __launch_bounds__(256) void k_rows_best(RowsK a) {
@@ -646,8 +661,9 @@ __global__ __launch_bounds__(256) void k_rows_best(RowsK a) {
 __device__ __forceinline__ void row_best(const RowsK &a, const RowHist &h, uint64_t *best, uint32_t *finite) {
   const uint32_t lane = threadIdx.x & 63;
   const RowSlice s = lane < a.bslices ? h.slice[lane] : RowSlice{0, 0, 0};
-  *best = wave_max_u64(s.best);
-  *finite = wave_sum_u32(s.finite);
+  const uint32_t key = wave_top_u32((uint32_t)(s.best >> 32));
+  *best = (uint64_t)key << 32 | wave_top_u32((uint32_t)(s.best >> 32) == key ? (uint32_t)s.best : 0);
+  *finite = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(s.finite), 63);
 }
 
 // One token's weight, and with COUNT the token, into a histogram in LDS.
@@ -662,8 +678,11 @@ template <bool COUNT>
 __global__ __launch_bounds__(RS_T) void k_rows_hist(RowsK a) {
   __shared__ uint64_t mass[RS_BINS];
   __shared__ uint32_t count[COUNT ? RS_BINS : 1];
-  const uint32_t tid = threadIdx.x, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const uint32_t tid = threadIdx.x;
   RowHist &h = a.hist[blockIdx.y];
+  const uint32_t lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const float *row = a.logits + blockIdx.y * a.stride;
+  const RowQuads first = load_quads<RS_T>(a, row, lo, hi);
   uint64_t best;
   uint32_t finite;
   row_best(a, h, &best, &finite);
@@ -675,7 +694,7 @@ __global__ __launch_bounds__(RS_T) void k_rows_hist(RowsK a) {
   }
   __syncthreads();
   uint64_t minp = 0;
-  each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t) {
+  each_logit<RS_T>(a, row, lo, hi, first, [&](bool ok, float v, uint32_t) {
     const double w = ok ? row_weight(a, bv, v) : 0.0;
     const uint64_t m = row_mass(a, w);
     if (ok && w >= a.min_p) minp += m;
@@ -1004,17 +1023,20 @@ __global__ __launch_bounds__(RS_T) void k_rows_topk(RowsK a) {
   extern __shared__ uint64_t pick_lds[];
   PickLds &L = *(PickLds *)pick_lds;
   RowHist &h = a.hist[blockIdx.y];
+  const uint32_t lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const float *row = a.logits + blockIdx.y * a.stride;
+  const RowQuads first = load_quads<RS_T>(a, row, lo, hi);
   uint64_t best;
   uint32_t finite;
   row_best(a, h, &best, &finite);
   if (a.top_k >= finite) return;
   load_hist(L, h);
   find_cross(L, a.top_k, ~0ull);
-  const uint32_t bin = L.x_bin, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const uint32_t bin = L.x_bin;
   const float bv = comp_value(best);
   if (threadIdx.x == 0) L.nlist = 0;
   __syncthreads();
-  each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t i) {
+  each_logit<RS_T>(a, row, lo, hi, first, [&](bool ok, float v, uint32_t i) {
     append(L.list, &L.nlist, ok && row_bin(a, bv, v) == bin, composite(v, i));
   });
   __syncthreads();
@@ -1036,6 +1058,9 @@ __global__ __launch_bounds__(RS_T) void k_rows_cuts(RowsK a) {
   extern __shared__ uint64_t pick_lds[];
   PickLds &L = *(PickLds *)pick_lds;
   RowHist &h = a.hist[blockIdx.y];
+  const uint32_t lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const float *row = a.logits + blockIdx.y * a.stride;
+  const RowQuads first = load_quads<RS_T>(a, row, lo, hi);
   uint64_t best;
   uint32_t finite;
   row_best(a, h, &best, &finite);
@@ -1065,11 +1090,11 @@ __global__ __launch_bounds__(RS_T) void k_rows_cuts(RowsK a) {
     if (mb < most && m1 >= most) L.at = b;
   }
   __syncthreads();
-  const uint32_t b0 = L.x_bin, b1 = L.at, lo = blockIdx.x * a.slice, hi = min(lo + a.slice, a.n);
+  const uint32_t b0 = L.x_bin, b1 = L.at;
   if (blockIdx.x == 0 && threadIdx.x == 0) { h.s = S; h.pbin = pbin; h.pmass = pmass; h.b0 = b0; h.b1 = b1; h.dmass = L.x_mass; }
   if (threadIdx.x == 0) L.nlist = L.npart = 0;
   __syncthreads();
-  each_logit<RS_T>(a, a.logits + blockIdx.y * a.stride, lo, hi, [&](bool ok, float v, uint32_t i) {
+  each_logit<RS_T>(a, row, lo, hi, first, [&](bool ok, float v, uint32_t i) {
     const uint32_t b = ok ? row_bin(a, bv, v) : RS_BINS + 1;
     append(L.list, &L.nlist, b == pbin, composite(v, i));
     append(L.part, &L.npart, b >= b0 && b <= b1, composite(v, i));
