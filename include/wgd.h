@@ -264,7 +264,8 @@ int wgd_attention_tree_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_bu
  * shortest prefix whose share of their weight reaches top_p, and of these the ones with a weight
  * of min_p or more; the token is the first whose running sum reaches uniform * (the kept
  * weight). With min_p 0 that is wgd_sample's rule. Weights and sums are integers of
- * 2^-(62 - ceil(log2 n)), at most 2^-51, of the largest weight, so a draw does not depend on the order of the sums.
+ * 2^-min(51, 62 - ceil(log2 n)) of the largest weight, so a draw does not depend on the order of
+ * the sums.
  * Temperature 0 takes the best; so does a uniform outside [0, 1). A row without a finite logit
  * gets -1. temperature <= 2, 0 < top_p <= 1, 0 <= min_p <= 1 (WGD_E_INVALID otherwise). */
 int wgd_sample_rows(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, uint32_t rows, uint32_t stride,
@@ -279,8 +280,8 @@ int wgd_tree_accept(wgd_context *ctx, const wgd_buffer *parents, const wgd_buffe
                     wgd_buffer *path, uint32_t nodes);
 /* Moves the K/V rows of an accepted path (as wgd_tree_accept writes it) to the slots that its
  * tokens keep: row (start + path[2 + j]) % capacity of every ring to row (start + j) % capacity,
- * for j < path[0]; the other rows stay. `rings` is a host array of `count` distinct buffers of
- * [capacity][row_bytes] (K and V of any number of layers; row_bytes = kv_heads * head_dim * 4, or
+ * for j < path[0]; the other rows stay. `rings` is a host array of `count` distinct buffers (at most
+ * 65536) of [capacity][row_bytes] (K and V of any number of layers; row_bytes = kv_heads * head_dim * 4, or
  * * 2 for f16 rings, a multiple of 2); nodes <= capacity. Entries of the path that do not lie
  * beyond their own place and below `nodes` move nothing. */
 int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, const wgd_buffer *path,

@@ -706,3 +706,63 @@ def test_refusals(gpu, up):
         assert gpu.address(f) and gpu.address(f) != gpu.address(y)
     finally:
         other.dispose()
+
+
+# ------------------------------------------------------------------------------- paths of the launchers
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
+@pytest.mark.parametrize("case", [
+    # several row groups in a workgroup, the last ones without rows; several splits
+    (32, 16, 128, 45, 1071, 1024, 0), (8, 2, 256, 35, 700, NO_WINDOW, 3), (4, 4, 64, 250, 900, NO_WINDOW, 0), (5, 1, 128, 61, 2500, NO_WINDOW, 0),
+    (6, 3, 72, 50, 1500, 800, 1),
+], ids=lambda c: "-".join("w" if v == NO_WINDOW else str(v) for v in c))
+def test_attention_tree_row_groups(gpu, up, case, kv):
+    test_attention_tree(gpu, up, case, kv)
+
+
+@pytest.mark.parametrize("hd,heads,nodes,start", [(128, 7, 64, 3000), (64, 16, 70, 2000), (256, 8, 33, 2500)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_attention_tree_of_many_rows_keeps_masked_places_out(gpu, up, hd, heads, nodes, start, bad):
+    rng = np.random.default_rng(hd + nodes)
+    q, k, v, cap = tree_case(rng, heads, 1, hd, nodes, start, NO_WINDOW, 4, "f16")
+    parents = random_tree(rng, nodes)
+    hit = nodes // 2
+    free = [i for i, p in enumerate(tree_ref.paths(parents)) if hit not in p]
+    assert 0 < len(free) < nodes
+    slot = (start + hit) % cap
+    k[slot], v[slot] = 0, 0
+    want = tree_ref.attention(q, k, v, parents, start, 1 / math.sqrt(hd), NO_WINDOW)
+    k[slot], v[slot] = bad, bad
+    unused = [(start + nodes + e) % cap for e in range(4)]
+    k[unused], v[unused] = bad, bad
+    got = run_tree(gpu, up, q, k, v, parents, start, 1 / math.sqrt(hd), NO_WINDOW)
+    # |score| <= S: its error is (hd + 4) eps S on either side, a sum of n weights adds (n + 8) eps
+    S = float(np.abs(q).max() * np.abs(k[np.isfinite(k)]).max()) * math.sqrt(hd)
+    bound = (2 * (hd + 4) * EPS * S + 2 * (start + nodes + 8) * EPS) * float(np.abs(v[np.isfinite(v)]).astype(np.float64).max())
+    assert np.isfinite(got[free]).all() and np.abs(got[free] - want[free]).max() <= bound
+    assert not np.isfinite(got[hit]).any()
+
+
+@pytest.mark.parametrize("rows,n,stride", [(300, 5003, 5011), (3, 70001, 70004), (1, 140000, 140000), (40, 33000, 33000)])
+@pytest.mark.parametrize("settings", [(0.9, 0, 0.9, 0.01), (1.3, 600, 0.95, 0.0), (0.7, 40, 0.9, 0.0), (1.0, 300, 1.0, 0.0)])
+def test_sample_rows_of_different_rows(gpu, up, rows, n, stride, settings):
+    rng = np.random.default_rng(rows + n)
+    logits = (rng.standard_normal((rows, stride)) * rng.uniform(0.1, 5, (rows, 1))).astype(np.float32)
+    logits[:, n:] = 1e9  # beyond the row
+    logits[rng.integers(0, rows, 50), rng.integers(0, n, 50)] = np.nan
+    logits[rng.integers(0, rows, 50), rng.integers(0, n, 50)] = -np.inf
+    if rows > 2:
+        logits[1, :n] = -np.inf
+        logits[2, :n] = np.round(logits[2, :n])
+    us = rng.random(rows)
+    got = draw_rows(gpu, up, logits, us, *settings, stride=(n,))
+    for i in range(rows):
+        assert got[i] in tree_ref.draw(logits[i, :n], us[i], *settings), i
+    assert got == draw_rows(gpu, up, logits, us, *settings, stride=(n,))
+
+
+def test_kv_commit_refuses_more_rings_than_a_call_takes(gpu, up):
+    ring, path = up(np.zeros(512, np.uint8)), up(np.zeros(64, np.uint8))
+    with pytest.raises(WgdError) as e:
+        gpu.kv_commit([ring] * 65537, path, 32, 3, 16, 4)
+    assert e.value.status == WGD_E_INVALID

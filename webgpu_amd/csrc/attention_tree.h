@@ -283,8 +283,8 @@ template <class E> constexpr uint32_t tree_nb() { return sizeof(E) == 2 ? 2 : 1;
 template <uint32_t HD, class E> constexpr uint32_t tree_ve() { return sizeof(E) == 2 && HD >= 128 ? 8 : 4; }
 
 // Threads of a workgroup: as many as their registers allow.
-template <uint32_t HD, uint32_t RT>
-constexpr uint32_t tree_threads() { return RT <= 2 && HD <= 128 ? 512 : 256; }
+template <uint32_t HD>
+constexpr uint32_t tree_threads() { return HD <= 128 ? 512 : 256; }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -422,18 +422,18 @@ __device__ __forceinline__ float tree_query(const float *q, uint32_t hd, float f
 }
 
 // FULL: the head dim is HD itself.
-template <uint32_t HD, class E, uint32_t RT, bool FULL>
-struct TreeWave : TreeRows<HD, RT, tree_nb<E>(), tree_ve<HD, E>()> {
+template <uint32_t HD, class E, bool FULL>
+struct TreeWave : TreeRows<HD, 1, tree_nb<E>(), tree_ve<HD, E>()> {
   static constexpr bool HALF = sizeof(E) == 2;
   static constexpr uint32_t NB = tree_nb<E>();
-  typedef TreeRows<HD, RT, NB, tree_ve<HD, E>()> Rows;
+  typedef TreeRows<HD, 1, NB, tree_ve<HD, E>()> Rows;
   using Rows::KEYS, Rows::VE, Rows::NX, Rows::o;
   static constexpr uint32_t KT = HALF ? HD / 32 : HD / 16;  // 16-byte pieces of a key per lane
   static constexpr uint32_t VK = 4 * NB;                    // keys per lane of a block of V
   typedef uint32_t vpiece __attribute__((ext_vector_type(VE * sizeof(E) / 4)));
 
-  u32x4 qh[RT][KT], ql[HALF ? RT : 1][KT];  // f16 hi and lo; f32: qh alone
-  float qs[RT];                              // the power of two taken out of the row's query
+  u32x4 qh[KT], ql[KT];  // f16 hi and lo; f32: qh alone
+  float qs;              // the power of two taken out of the row's query
   // the ring: this kv head's K and V, bytes between rows, slots; the end of the keys and the slot of the block's first
   const uint8_t *k, *v;
   uint64_t rowb;
@@ -490,23 +490,23 @@ struct TreeWave : TreeRows<HD, RT, tree_nb<E>(), tree_ve<HD, E>()> {
   }
 
   // The row's query times scale log2 e as operand.
-  __device__ __forceinline__ void load_q(const TreeK &a, uint32_t rt, const float *q, bool ok) {
+  __device__ __forceinline__ void load_q(const TreeK &a, const float *q, bool ok) {
     const float f = a.scale * TREE_LOG2E;
     if constexpr (!HALF) {
       const uint32_t g = (threadIdx.x & 63) >> 4;
 #pragma unroll
       for (uint32_t t = 0; t < KT; t++) {
         const f32x4 x = ok && (FULL || 16 * t + 4 * g < a.hd) ? *(const f32x4 *)(q + 16 * t + 4 * g) : f32x4{0, 0, 0, 0};
-        qh[rt][t] = __builtin_bit_cast(u32x4, f32x4{x.x * f, x.y * f, x.z * f, x.w * f});
+        qh[t] = __builtin_bit_cast(u32x4, f32x4{x.x * f, x.y * f, x.z * f, x.w * f});
       }
-      qs[rt] = 1.f;
+      qs = 1.f;
     } else {
-      qs[rt] = tree_query<KT>(q, FULL ? HD : a.hd, f, ok, qh[rt], ql[rt]);
+      qs = tree_query<KT>(q, FULL ? HD : a.hd, f, ok, qh, ql);
     }
   }
 
   // Keys [t0, ..) in steps of `step` up to hi.
-  __device__ __forceinline__ void walk(const TreeK &a, const TreeLds &L, const TreeSeen *seen, uint32_t t0, uint32_t step,
+  __device__ __forceinline__ void walk(const TreeK &a, const TreeLds &L, const TreeSeen &seen, uint32_t t0, uint32_t step,
                                        uint32_t masked_below) {
     const uint32_t g = (threadIdx.x & 63) >> 4;
     this->clear();
@@ -528,39 +528,34 @@ struct TreeWave : TreeRows<HD, RT, tree_nb<E>(), tree_ve<HD, E>()> {
         }
       }
       // ---- scores
-      f32x4 s[RT][NB];
+      f32x4 s[NB];
 #pragma unroll
-      for (uint32_t rt = 0; rt < RT; rt++)
+      for (uint32_t b = 0; b < NB; b++) {
+        f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t b = 0; b < NB; b++) {
-          f32x4 acc = {0, 0, 0, 0};
+        for (uint32_t t = 0; t < KT; t++) {
+          if constexpr (HALF) {
+            const f16x8 kf = __builtin_bit_cast(f16x8, kr[b][t]);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, qh[t]), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, ql[t]), acc, 0, 0, 0);
+          } else {
+            const f32x4 kf = __builtin_bit_cast(f32x4, kr[b][t]), qf = __builtin_bit_cast(f32x4, qh[t]);
 #pragma unroll
-          for (uint32_t t = 0; t < KT; t++) {
-            if constexpr (HALF) {
-              const f16x8 kf = __builtin_bit_cast(f16x8, kr[b][t]);
-              acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, qh[rt][t]), acc, 0, 0, 0);
-              acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, ql[rt][t]), acc, 0, 0, 0);
-            } else {
-              const f32x4 kf = __builtin_bit_cast(f32x4, kr[b][t]), qf = __builtin_bit_cast(f32x4, qh[rt][t]);
-#pragma unroll
-              for (int u = 0; u < 4; u++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[u], qf[u], acc, 0, 0, 0);
-            }
+            for (int u = 0; u < 4; u++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[u], qf[u], acc, 0, 0, 0);
           }
-          s[rt][b] = acc;
         }
+        s[b] = acc;
+      }
       base += step;
       if (base >= cap) base %= cap;
       if (t0 + step < hi) load_k(t0 + step);
       // ---- weights, in place of the scores
       const bool masked = t0 + KEYS > min(hi, a.start) || t0 < masked_below;
-#pragma unroll
-      for (uint32_t rt = 0; rt < RT; rt++)
-        this->weigh(rt, s[rt], qs[rt], masked, masked ? tree_sees(a, L, seen[rt], t0, hi) : 0);
+      this->weigh(0, s, qs, masked, masked ? tree_sees(a, L, seen, t0, hi) : 0);
       // ---- values
       if constexpr (HALF) {
-        f16x8 ph[RT], pl[RT];
-#pragma unroll
-        for (uint32_t rt = 0; rt < RT; rt++) tree_split(s[rt], ph[rt], pl[rt]);
+        f16x8 ph, pl;
+        tree_split(s, ph, pl);
 #pragma unroll
         for (uint32_t x = 0; x < NX; x++)
 #pragma unroll
@@ -570,11 +565,8 @@ struct TreeWave : TreeRows<HD, RT, tree_nb<E>(), tree_ve<HD, E>()> {
             for (uint32_t i = 0; i < 4; i++)
               f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][x][e / 2], vr[2 * i][x][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
             const f16x8 vf = __builtin_bit_cast(f16x8, f);
-#pragma unroll
-            for (uint32_t rt = 0; rt < RT; rt++) {
-              o[rt][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[rt], o[rt][x][e], 0, 0, 0);
-              o[rt][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[rt], o[rt][x][e], 0, 0, 0);
-            }
+            o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[0][x][e], 0, 0, 0);
+            o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[0][x][e], 0, 0, 0);
           }
       } else {
 #pragma unroll
@@ -583,9 +575,7 @@ struct TreeWave : TreeRows<HD, RT, tree_nb<E>(), tree_ve<HD, E>()> {
           for (uint32_t x = 0; x < NX; x++)
 #pragma unroll
             for (uint32_t e = 0; e < VE; e++)
-#pragma unroll
-              for (uint32_t rt = 0; rt < RT; rt++)
-                o[rt][x][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i][x][e]), s[rt][0][i], o[rt][x][e], 0, 0, 0);
+              o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i][x][e]), s[0][i], o[0][x][e], 0, 0, 0);
       }
     }
   }
@@ -709,23 +699,21 @@ __device__ __forceinline__ void tree_end(const TreeK &a, const TreeGrid &gr, Tre
   }
 }
 
-template <uint32_t HD, class E, uint32_t RT, bool FULL>
-__global__ __launch_bounds__((tree_threads<HD, RT>())) void k_attn_tree(TreeK a, TreeGrid gr) {
-  typedef TreeWave<HD, E, RT, FULL> Wave;
+template <uint32_t HD, class E, bool FULL>
+__global__ __launch_bounds__((tree_threads<HD>())) void k_attn_tree(TreeK a, TreeGrid gr) {
+  typedef TreeWave<HD, E, FULL> Wave;
   extern __shared__ float lds[];
   __shared__ TreeLds L;
-  const TreePart p = tree_part(a, gr, RT, Wave::KEYS);
+  const TreePart p = tree_part(a, gr, 1, Wave::KEYS);
   const uint32_t from = p.lo + p.slice * Wave::KEYS;
   Wave s;
   s.begin(a, p.kv, from, p.wrow < p.nrows ? p.hi : 0);
-  uint32_t row[RT];
-  TreeSeen seen[RT];
-  tree_rows<RT>(a, L, p, row, seen);
-#pragma unroll
-  for (uint32_t rt = 0; rt < RT; rt++)
-    s.load_q(a, rt, a.q + tree_row(a, p.kv, row[rt]) * a.hd, p.wrow + 16 * rt + (threadIdx.x & 15) < p.nrows);
-  s.walk(a, L, seen, from, p.slices * Wave::KEYS, p.masked_below);
-  tree_end<HD, E, RT, tree_threads<HD, RT>()>(a, gr, L, lds, p, s, seen);
+  uint32_t row[1];
+  TreeSeen seen[1];
+  tree_rows<1>(a, L, p, row, seen);
+  s.load_q(a, a.q + tree_row(a, p.kv, row[0]) * a.hd, p.wrow + (threadIdx.x & 15) < p.nrows);
+  s.walk(a, L, seen[0], from, p.slices * Wave::KEYS, p.masked_below);
+  tree_end<HD, E, 1, tree_threads<HD>()>(a, gr, L, lds, p, s, seen);
 }
 
 // ------------------------------------------------------------------ many rows: keys staged in LDS
@@ -999,13 +987,13 @@ uint64_t attention_tree_scratch_floats(const TreeAttnArgs &in) {
   return n > 1 ? (uint64_t)n * in.nodes * in.heads * (in.hd + 2) : 0;
 }
 
-template <uint32_t HD, class E, uint32_t RT, bool FULL>
+template <uint32_t HD, class E, bool FULL>
 static void launch_tree(hipStream_t s, const TreeK &a, const TreePlan &p) {
-  constexpr uint32_t waves = tree_threads<HD, RT>() / 64;
-  constexpr size_t lds = std::max(tree_wave_lds<HD, RT>() * waves, tree_any_lds(HD, tree_any_tile(HD)));
+  constexpr uint32_t waves = tree_threads<HD>() / 64;
+  constexpr size_t lds = std::max(tree_wave_lds<HD, 1>() * waves, tree_any_lds(HD, tree_any_tile(HD)));
   static_assert(lds + sizeof(TreeLds) + 1024 <= LDS_MAX, "the wavefronts' outputs fit LDS");
-  lds_opt_in_bytes((const void *)k_attn_tree<HD, E, RT, FULL>, (uint32_t)lds);
-  hipLaunchKernelGGL((k_attn_tree<HD, E, RT, FULL>), dim3(a.kvh, p.blocks, p.nsplit), dim3(64 * waves), lds, s, a, TreeGrid{p.rw, p.per});
+  lds_opt_in_bytes((const void *)k_attn_tree<HD, E, FULL>, (uint32_t)lds);
+  hipLaunchKernelGGL((k_attn_tree<HD, E, FULL>), dim3(a.kvh, p.blocks, p.nsplit), dim3(64 * waves), lds, s, a, TreeGrid{p.rw, p.per});
 }
 template <uint32_t HD>
 static void launch_tree_staged(hipStream_t s, const TreeK &a, const TreePlan &p) {
@@ -1017,10 +1005,10 @@ static void launch_tree_staged(hipStream_t s, const TreeK &a, const TreePlan &p)
 }
 template <uint32_t HD, class E>
 static void launch_tree_hd(hipStream_t s, const TreeK &a, const TreePlan &p) {
-  if (a.hd < HD) return launch_tree<HD, E, 1, false>(s, a, p);
+  if (a.hd < HD) return launch_tree<HD, E, false>(s, a, p);
   if constexpr (sizeof(E) == 2)
     if (p.staged) return launch_tree_staged<HD>(s, a, p);
-  launch_tree<HD, E, 1, true>(s, a, p);
+  launch_tree<HD, E, true>(s, a, p);
 }
 
 hipError_t attention_tree(hipStream_t s, const TreeAttnArgs &in) {

@@ -813,7 +813,7 @@ int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, co
     return fail(ctx, WGD_E_INVALID, "kv_commit: %u nodes at %u in a ring of %u rows of %llu bytes", nodes, start, capacity, (unsigned long long)row_bytes);
   NEED_FIT(ctx, path, (uint64_t)(nodes + 2) * 4, "accepted path");
   if (!count) return WGD_OK;
-  if (!rings) return fail(ctx, WGD_E_INVALID, "kv_commit: NULL rings");
+  if (!rings || count > 65536) return fail(ctx, WGD_E_INVALID, rings ? "kv_commit: %u rings, at most 65536 in one call" : "kv_commit: NULL rings", count);
   std::vector<void *> at(count);
   for (uint32_t i = 0; i < count; i++) {
     NEED_BUF(ctx, rings[i], "kv_commit");
