@@ -475,6 +475,10 @@ hipError_t sample(hipStream_t s, const float *logits, uint32_t n, const SamplePa
 //   * k_rows_cuts: the same for top-p, and for the draw: what top-p keeps is known to within its bin, so the bins
 //     that the draw can fall into are known too, one or two;
 //   * k_rows_last: what top-p keeps and the token, from their lists.
+// Few is bound by the row's one read where there are many rows and by latency else: 64 rows of 128256, top-k 40: groups 7.0 us
+// (4.7 TB/s), few 6.0; one row of 151936: 3.2 and 5.6. Up to 64 candidates are cut in one wavefront, without barriers (all
+// 512 threads: 11.5). Many is bound by latency and by atomics: 16 rows of 262144, top-p 0.95: best 4.0, hist 12.1, cuts 11.7,
+// last 7.6.
 // A cut's token is found in its list by a histogram of RS_SUB parts of the bin and a sort of the one part
 // that holds it (a sort of the whole list took four times as long).
 // A bin or bound with more tokens than a list holds (ties, logits close together for the temperature) goes through
