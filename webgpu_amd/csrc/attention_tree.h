@@ -822,19 +822,36 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_attn_tree_staged(TreeK a, Tr
   uint8_t *stages = (uint8_t *)lds;
   const uint64_t rowb = (uint64_t)a.kvh * ROW, head = (uint64_t)p.kv * ROW;
   const uint8_t *k = (const uint8_t *)a.k + head, *v = (const uint8_t *)a.v + head;
-  // keys t0 .. + SK into stage s, 64 chunks per wavefront and step; keys past the end read the last one
+  // Keys t0 .. + SK (t0 in slot base) into stage s, 64 chunks per wavefront and step; keys past the end read the last one.
+  // A step of all wavefronts is STEP keys on, a multiple of the swizzles' period: lane offsets are the same for all.
+  constexpr uint32_t STEP = TREE_STAGED_NT / CH;
+  static_assert(STEP % 16 == 0, "the swizzles repeat after 16 keys");
+  const uint32_t key0 = tid / CH, k_place = (tid % CH ^ Wave::k_swizzle(key0)) * 16, v_place = (tid % CH ^ Wave::v_swizzle(key0)) * 16;
+  const uint32_t off = key0 * (uint32_t)rowb, k_off = off + k_place, v_off = off + v_place;  // below 2^32 (tree_plan)
+  uint32_t base = p.lo % cap;
   auto load = [&](uint32_t t0, uint32_t s) {
-    uint8_t *K = stages + s * 2 * SK * ROW, *V = K + SK * ROW;
-    const uint32_t base = t0 % cap;
-    for (uint32_t q = w; q < SK * CH / 64; q += TREE_STAGED_NT / 64) {
-      const uint32_t i = 64 * q + lane, key = i / CH, place = i % CH;
-      const uint32_t at = base + min(key, p.hi - 1 - t0);
-      const uint64_t row = (uint64_t)min(at, at - cap) * rowb;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(k + row + (place ^ Wave::k_swizzle(key)) * 16),
-                                       (__attribute__((address_space(3))) void *)(K + 1024 * q), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(v + row + (place ^ Wave::v_swizzle(key)) * 16),
-                                       (__attribute__((address_space(3))) void *)(V + 1024 * q), 16, 0, 0);
+    uint8_t *K = stages + s * 2 * SK * ROW + 1024 * w, *V = K + SK * ROW;
+    auto put = [](const uint8_t *from, uint8_t *to) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+    };
+    if (base + SK <= cap && t0 + SK <= p.hi) {
+#pragma unroll
+      for (uint32_t n = 0; n < SK / STEP; n++) {
+        const uint64_t first = (uint64_t)(base + n * STEP) * rowb;
+        put(k + first + k_off, K + n * STEP * ROW);
+        put(v + first + v_off, V + n * STEP * ROW);
+      }
+    } else {
+#pragma unroll 1
+      for (uint32_t n = 0; n < SK / STEP; n++) {
+        const uint32_t at = base + min(key0 + n * STEP, p.hi - 1 - t0);
+        const uint64_t row = (uint64_t)min(at, at - cap) * rowb;
+        put(k + row + k_place, K + n * STEP * ROW);
+        put(v + row + v_place, V + n * STEP * ROW);
+      }
     }
+    base += SK;
+    if (base >= cap) base %= cap;
   };
   if (p.lo < p.hi) load(p.lo, 0);
   uint32_t row[RT];
