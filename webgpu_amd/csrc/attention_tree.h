@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256) void k_attn_tree_any(TreeK a) {
 // finite would turn it into NaN, and a split key or query could turn an infinity into NaN: a workgroup
 // that ends with anything not finite forms its rows again with tree_any.
 // Latency bounds it: a wavefront is 40% of its time at waits for loads and 40% at waits to issue, two to a SIMD. 48
-// nodes, 32 heads on 16 of 128, 1071 f32 keys: 18.6 us and 3.3 to join (the products alone 4.9), 64 nodes over 15000 f32 keys
+// nodes, 32 heads on 16 of 128, 1071 f32 keys: 18.7 us and 4 to join (the products alone 4.9), 64 nodes over 15000 f32 keys
 // of 8 heads 178 us, 88 TFLOP/s of the 153 that f32 matrix products reach. With two tiles a wavefront, which spill, the latter
 // takes 163 but shorter rings more.
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -727,9 +727,9 @@ __global__ __launch_bounds__((tree_threads<HD>())) void k_attn_tree(TreeK a, Tre
 // stage of SK keys into LDS once, straight from memory (no registers), while they work on the one before; a
 // wavefront's blocks of 32 keys are its slice's. K rows and V rows lie in 16-byte chunks; chunk i of key k
 // at place i ^ swizzle(k), so that the 16 keys of a K operand, and the 16-bit transposing reads that make V
-// operands (4 keys of one dim per lane), meet all banks evenly. 64 nodes, 32 heads on 8 of 128, 31000 keys: 78 us (direct
-// 112), 417 TFLOP/s counted once, twice that with the split operands: matrix products take 40% of the cycles and vector
-// instructions (weights, their split) 53%, and the two do not overlap.
+// operands (4 keys of one dim per lane), meet all banks evenly. 64 nodes, 32 heads on 8 of 128, 31000 keys: 75 us (direct
+// 112), 433 TFLOP/s counted once, twice that with the split operands. Matrix products take 36% of the cycles and the issue of
+// vector instructions 39%; a wavefront is at waits for LDS, loads and the others of its stage 37% of its life, two to a SIMD.
 // Two V operands at LDS addresses `at`: dims in transposing reads of keys 0 .. 4 and, OFF bytes on, 16 .. 20 of each lane
 // group. The builtin of this read waits for every load from memory into LDS that is under way, the next
 // stage's too, so it is written here with its own wait.
