@@ -228,6 +228,8 @@ static bool owned(wgd_context *ctx, const wgd_buffer *b) { return b && ctx->buff
 #define NEED_CTX(ctx) do { if (!(ctx)) return fail(nullptr, WGD_E_INVALID, "NULL context"); hipSetDevice((ctx)->device); } while (0)
 #define NEED_BUF(ctx, b, what) do { if (!owned(ctx, b)) return fail(ctx, WGD_E_INVALID, "%s: missing or foreign buffer", what); } while (0)
 #define NEED_FIT(ctx, b, bytes, what) do { if ((uint64_t)(bytes) > (b)->size) return fail(ctx, WGD_E_INVALID, "%s: buffer %s holds %llu bytes, the launch reads or writes %llu", what, (b)->label.c_str(), (unsigned long long)(b)->size, (unsigned long long)(bytes)); } while (0)
+// The same in floats from `at` (within b) on, for counts whose bytes do not fit 64 bits.
+#define NEED_FLOATS(ctx, b, at, floats, what) do { if ((uint64_t)(floats) > (b)->size / 4 - (at)) return fail(ctx, WGD_E_INVALID, "%s: buffer %s holds %llu bytes, the launch reads or writes %llu floats from float %llu on", what, (b)->label.c_str(), (unsigned long long)(b)->size, (unsigned long long)(floats), (unsigned long long)(at)); } while (0)
 
 int wgd_write(wgd_context *ctx, wgd_buffer *b, uint64_t offset, const void *data, uint64_t bytes) {
   NEED_CTX(ctx); NEED_BUF(ctx, b, "wgd_write");
@@ -716,7 +718,7 @@ int wgd_rope_at(wgd_context *ctx, wgd_buffer *x, const wgd_buffer *positions, co
   a.heads = heads; a.hd = hd; a.rot = rot ? rot : hd; a.stride = stride ? stride : (uint32_t)row; a.batch = batch;
   a.theta = theta; a.scale = scale; a.magnitude = magnitude; a.adjacent = adjacent != 0;
   if (offset > x->size / 4) return fail(ctx, WGD_E_INVALID, "rope_at: offset %llu outside buffer %s", (unsigned long long)offset, x->label.c_str());
-  NEED_FIT(ctx, x, (offset + (uint64_t)(batch - 1) * a.stride + row) * 4, "rope_at input");
+  NEED_FLOATS(ctx, x, offset, (uint64_t)(batch - 1) * a.stride + row, "rope_at input");
   NEED_FIT(ctx, positions, (uint64_t)batch * 4, "rope_at positions");
   if (factors) { NEED_BUF(ctx, factors, "rope_at"); NEED_FIT(ctx, factors, (uint64_t)a.rot / 2 * 4, "rope_at factors"); }
   if (x == positions || x == factors) return fail(ctx, WGD_E_INVALID, "rope_at: positions and factors need buffers of their own");
