@@ -33,3 +33,9 @@ def test_rope_at_refuses_rows_whose_bytes_pass_64_bits(gpu, up):
     for offset in (0, 64):
         refused(lambda: gpu.rope_at(x, positions, 1, 2, 1e4, 1.0, 2, 2 ** 31 + 1, stride=2 ** 31, offset=offset), "rope_at input")
     refused(lambda: gpu.rope_at(x, positions, 1, 2, 1e4, 1.0, 2, 2 ** 32 - 1, stride=2 ** 32 - 1), "rope_at input")
+
+
+def test_sample_rows_refuses_rows_whose_bytes_pass_64_bits(gpu, up):
+    logits, uniforms, tokens = up(np.zeros(64, np.float32)), up(np.zeros(8, np.float64)), up(np.zeros(8, np.int32))
+    refused(lambda: gpu.sample_rows(logits, 16, 2 ** 31 + 1, uniforms, tokens, 0.5, stride=2 ** 31), "sample_rows logits")
+    refused(lambda: gpu.sample_rows(logits, 16, 2 ** 32 - 1, uniforms, tokens, 0.5, stride=2 ** 32 - 1), "sample_rows logits")

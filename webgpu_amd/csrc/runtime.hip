@@ -783,7 +783,7 @@ int wgd_sample_rows(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, uint
   if (!rows) return WGD_OK;
   SampleRowsArgs a{};
   a.n = n; a.rows = rows; a.stride = stride ? stride : n;
-  NEED_FIT(ctx, logits, ((uint64_t)(rows - 1) * a.stride + n) * 4, "sample_rows logits");
+  NEED_FLOATS(ctx, logits, 0, (uint64_t)(rows - 1) * a.stride + n, "sample_rows logits");
   NEED_FIT(ctx, uniforms, (uint64_t)rows * 8, "sample_rows uniforms");
   NEED_FIT(ctx, tokens, (uint64_t)rows * 4, "sample_rows tokens");
   a.logits = (const float *)logits->ptr; a.uniforms = (const double *)uniforms->ptr; a.tokens = (int32_t *)tokens->ptr;
