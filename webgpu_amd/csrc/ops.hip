@@ -586,10 +586,22 @@ hipError_t rope_at(hipStream_t s, const RopeAtArgs &a) {
   const uint32_t n4 = a.rot / 8;
   const bool vec = (uintptr_t)a.x % 16 == 0 && a.stride % 4 == 0 && a.hd % 4 == 0 && a.rot % 8 == 0 && a.rot <= 512;
   const uint32_t per = std::min(a.heads, vec ? 256 / n4 : 16u);
-  const dim3 grid(a.batch, (a.heads + per - 1) / per);
-  if (vec) hipLaunchKernelGGL(k_rope_at<true>, grid, dim3(256), 0, s, a, f, per);
-  else hipLaunchKernelGGL(k_rope_at<false>, grid, dim3(256), 0, s, a, f, per);
-  return hipGetLastError();
+  // A launch has fewer than 2^32 threads along x and at most 65535 workgroups along y: more tokens or heads are more launches.
+  constexpr uint32_t TOKENS = 1u << 23;
+  const uint64_t heads = 65535ull * per;
+  for (uint64_t t = 0; t < a.batch; t += TOKENS)
+    for (uint64_t h = 0; h < a.heads; h += heads) {
+      RopeAtArgs b = a;
+      b.x += t * a.stride + h * a.hd;
+      b.positions += t;
+      b.batch = (uint32_t)std::min<uint64_t>(TOKENS, a.batch - t);
+      b.heads = (uint32_t)std::min<uint64_t>(heads, a.heads - h);
+      const dim3 grid(b.batch, (b.heads + per - 1) / per);
+      if (vec) hipLaunchKernelGGL(k_rope_at<true>, grid, dim3(256), 0, s, b, f, per);
+      else hipLaunchKernelGGL(k_rope_at<false>, grid, dim3(256), 0, s, b, f, per);
+      WGD_HIP(hipGetLastError());
+    }
+  return hipSuccess;
 }
 
 // ------------------------------------------------------------------ drafted trees: the accepted path
