@@ -247,8 +247,9 @@ int wgd_rope_at(wgd_context *ctx, wgd_buffer *x, const wgd_buffer *positions, co
  * (position_i - window, start), at ring slot t % capacity as in wgd_attention, and over i itself
  * and its ancestors within the window; y[i][h] = softmax(scale * q.k) V, zeros for padding. A
  * node outside i's ancestors never reaches y[i], whatever its K/V hold. Needs nodes <=
- * WGD_TREE_MAX, head_dim <= 512, start < 2^31 and a ring that holds every key that some node sees,
- * min(start, window - 1) + nodes <= capacity. */
+ * WGD_TREE_MAX, head_dim <= 512, start < 2^31, heads <= 2^20, nodes * heads < 2^26, nodes * heads /
+ * kv_heads <= 1048560 and a ring that holds every key that some node sees, min(start, window - 1) + nodes
+ * <= capacity. */
 int wgd_attention_tree(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *y,
                        const wgd_buffer *parents, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t start,
                        float scale, uint32_t window, uint32_t capacity, uint32_t nodes);

@@ -91,3 +91,25 @@ def test_rope_at_of_more_heads_than_a_launch_takes(gpu, up):
     got = np.frombuffer(gpu.read(xb, x.nbytes), np.float32).reshape(x.shape)
     size = np.abs(x.astype(np.float64)).sum(-1, keepdims=True)
     assert np.all(np.abs(got - tree_ref.rope(x, pos, 1e4, 1.0, 2, False)) <= ROPE_E * size)
+
+
+@pytest.mark.parametrize("nodes,heads,kv_heads", [(256, 4096, 1), (256, 2 ** 18, 2 ** 18), (1, 2 ** 21, 2 ** 21)])
+def test_attention_tree_refuses_more_rows_than_a_launch_takes(gpu, nodes, heads, kv_heads):
+    """65536 workgroups along y; 2^26 rows to join; more heads than the operator takes. Buffers of the whole size."""
+    sizes = [4 * nodes * heads, 4 * nodes * kv_heads, 4 * nodes * kv_heads, 4 * nodes * heads, 4 * nodes]
+    held = [gpu.buffer(n) for n in sizes]
+    try:
+        for op in (gpu.attention_tree, gpu.attention_tree_f16kv):
+            refused(lambda: op(*held, heads, kv_heads, 1, 0, 1.0, 1 << 30, nodes, nodes), "more than a launch takes")
+    finally:
+        for b in held:
+            gpu.destroy(b)
+
+
+def test_attention_tree_of_the_most_rows_of_a_kv_head(gpu, up):
+    """65535 workgroups along y, for one node: zero queries weigh its one key alone."""
+    heads, hd = 65535 * 16, 1
+    q, k, v, y = up(np.zeros(heads, np.float32)), up(np.zeros(1, np.float32)), up(np.full(1, 2.5, np.float32)), up(np.zeros(heads, np.float32))
+    refused(lambda: gpu.attention_tree(q, k, v, y, up(np.array([-1], np.int32)), 2 ** 20 + 1, 1, hd, 0, 1.0, 9, 1, 1), "more than a launch takes")
+    gpu.attention_tree(q, k, v, y, up(np.array([-1], np.int32)), heads, 1, hd, 0, 1.0, 9, 1, 1)
+    assert np.all(np.frombuffer(gpu.read(y, 4 * heads), np.float32) == 2.5)

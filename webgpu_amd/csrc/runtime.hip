@@ -738,7 +738,10 @@ static int attention_tree_common(wgd_context *ctx, const char *what, const wgd_b
     return fail(ctx, WGD_E_INVALID, "%s: invalid heads %u/%u, head_dim %u, capacity %u or window %u", what, heads, kv_heads, hd, capacity, window);
   if (nodes > WGD_TREE_MAX) return fail(ctx, WGD_E_INVALID, "%s: %u nodes, a tree has at most %u", what, nodes, WGD_TREE_MAX);
   if (start > 0x7FFFFFFFu) return fail(ctx, WGD_E_INVALID, "%s: start %u is beyond 2^31 - 1", what, start);
-  if (heads > (1u << 20)) return fail(ctx, WGD_E_INVALID, "%s: %u heads", what, heads);
+  // a launch has at most 65535 workgroups of 16 rows along y, and fewer than 2^32 threads along x, 64 a row in the join
+  const uint64_t rows = (uint64_t)nodes * heads;
+  if (heads > (1u << 20) || rows >= (1u << 26) || rows / kv_heads > 65535 * 16)
+    return fail(ctx, WGD_E_INVALID, "%s: %u heads on %u for each of %u nodes are more than a launch takes", what, heads, kv_heads, nodes);
   if ((uint64_t)std::min(start, window - 1) + nodes > capacity)
     return fail(ctx, WGD_E_INVALID, "%s: %u cached keys and %u nodes do not fit a ring of %u slots", what, std::min(start, window - 1), nodes, capacity);
   if (y == q || y == k || y == v || y == parents) return fail(ctx, WGD_E_INVALID, "%s: the output needs a buffer of its own", what);
