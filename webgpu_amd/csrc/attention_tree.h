@@ -27,6 +27,12 @@ __device__ __forceinline__ uint64_t tree_row(const TreeK &a, uint32_t kv, uint32
   return (uint64_t)(r / a.group) * a.heads + kv * a.group + r % a.group;
 }
 
+// The partial outputs of several splits are [split][row][hd], and from an even float on, 8-byte aligned whatever the
+// head dim, (max, sum) pairs [split][row].
+__host__ __device__ __forceinline__ uint64_t tree_pairs(uint32_t nsplit, uint64_t rows, uint32_t hd) {
+  return (nsplit * rows * hd + 1) / 2 * 2;
+}
+
 // What the nodes see of each other: bits[i] is i's path to the root (within the window), len[i] its length and
 // up[i] -1, or -2 for padding. Formed by doubling the steps of all nodes at once.
 struct TreeLds { uint32_t bits[WGD_TREE_MAX][TREE_WORDS]; int32_t up[WGD_TREE_MAX]; uint32_t len[WGD_TREE_MAX]; };
@@ -239,7 +245,7 @@ __device__ __forceinline__ void tree_any(const TreeK &a, const TreeLds &L, float
       a.y[row * hd + d] = pad ? 0.f : O[i] / lrow[r];
     } else {
       a.part[at * hd + d] = O[i];
-      if (d == 0) *(float2 *)(a.part + a.nsplit * all * hd + 2 * at) = make_float2(mrow[r], pad ? -1.f : lrow[r]);
+      if (d == 0) *(float2 *)(a.part + tree_pairs(a.nsplit, all, hd) + 2 * at) = make_float2(mrow[r], pad ? -1.f : lrow[r]);
     }
   }
 }
@@ -692,7 +698,7 @@ __device__ __forceinline__ void tree_end(const TreeK &a, const TreeGrid &gr, Tre
     float inv = 1.f;
     if (a.nsplit > 1) {
       to = a.part + ((uint64_t)p.z * rows + row) * a.hd + d;
-      if (d == 0) *(float2 *)(a.part + (uint64_t)a.nsplit * rows * a.hd + 2 * ((uint64_t)p.z * rows + row)) = make_float2(M - TREE_BIAS, pad ? -1.f : l);
+      if (d == 0) *(float2 *)(a.part + tree_pairs(a.nsplit, rows, a.hd) + 2 * ((uint64_t)p.z * rows + row)) = make_float2(M - TREE_BIAS, pad ? -1.f : l);
     } else {
       inv = 1.f / l;
     }
@@ -876,11 +882,10 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_attn_tree_staged(TreeK a, Tr
   tree_end<HD, _Float16, RT, TREE_STAGED_NT>(a, gr, L, lds, p, s, seen);
 }
 
-// The splits of a row in order, of partial outputs [split][row][hd] and behind them (max, sum) pairs
-// [split][row], maxima in powers of two. A sum of zero is a split without keys that the row sees (or
-// without a finite score, which adds nothing either); the last split knows padding, by a negative sum. A row
-// always sees itself, so sums that are all zero mean scores that were all -inf: 0 / 0, as the
-// formula has it.
+// The splits of a row in order, of partial outputs and (max, sum) pairs (tree_pairs), maxima in powers of
+// two. A sum of zero is a split without keys that the row sees (or without a finite score, which adds
+// nothing either); the last split knows padding, by a negative sum. A row always sees itself, so sums
+// that are all zero mean scores that were all -inf: 0 / 0, as the formula has it.
 // A wavefront per row: the splits' weights go over its lanes and LDS, then (VEC: hd a power of two of 4 to 256) lane groups
 // of hd / 4 (at most 64) lanes take every (64 / group)-th split, 16 bytes a lane and eight loads ahead.
 constexpr uint32_t TREE_SPLITS = 256;
@@ -889,7 +894,7 @@ __global__ __launch_bounds__(256) void k_attn_tree_join(const float *part, float
   __shared__ float wz[4][TREE_SPLITS];
   const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const uint64_t row = min(blockIdx.x * 4 + wv, rows - 1);
-  const float2 *ml = (const float2 *)(part + (uint64_t)nsplit * rows * hd) + row;
+  const float2 *ml = (const float2 *)(part + tree_pairs(nsplit, rows, hd)) + row;
   float2 s[TREE_SPLITS / 64];
   float M = -INFINITY;
 #pragma unroll
@@ -1007,7 +1012,8 @@ static TreePlan tree_plan(const TreeAttnArgs &in) {
 uint64_t attention_tree_scratch_floats(const TreeAttnArgs &in) {
   if (!in.nodes) return 0;
   const uint32_t n = tree_plan(in).nsplit;
-  return n > 1 ? (uint64_t)n * in.nodes * in.heads * (in.hd + 2) : 0;
+  const uint64_t rows = (uint64_t)in.nodes * in.heads;
+  return n > 1 ? tree_pairs(n, rows, in.hd) + 2 * n * rows : 0;
 }
 
 template <uint32_t HD, class E, bool FULL>
