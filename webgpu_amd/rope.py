@@ -15,7 +15,7 @@ import numpy as np
 
 def _wavelengths(rotary_dim: int, theta: float) -> np.ndarray:
     """Positions per turn of each pair."""
-    if rotary_dim < 2 or rotary_dim % 2 or not theta > 0:
+    if rotary_dim < 2 or rotary_dim % 2 or not 0 < theta < math.inf:
         raise ValueError(f"Rotary dims {rotary_dim} / theta {theta} are invalid.")
     return 2 * math.pi * float(theta) ** (np.arange(0, rotary_dim, 2, dtype=np.float64) / rotary_dim)
 
@@ -35,8 +35,8 @@ def yarn_factors(rotary_dim: int, theta: float, factor: float, original: int, fa
     """YaRN (Peng et al., 2023): a ramp over the pair index from the pair that turns ``fast`` times
     within the ``original`` context (kept) to the one that turns ``slow`` times (slowed by ``factor``).
     Returns the factors and the magnitude 0.1 ln(factor) + 1."""
-    if not (factor >= 1 and fast > slow > 0 and original > 0):
-        raise ValueError("YaRN scaling needs factor >= 1, fast > slow > 0 and an original context.")
+    if not (factor >= 1 and fast > slow > 0 and original > 0 and theta > 1):
+        raise ValueError("YaRN scaling needs factor >= 1, fast > slow > 0, an original context and theta > 1.")
     _wavelengths(rotary_dim, theta)
     pair = lambda turns: rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
     first, last = max(0, math.floor(pair(fast))), min(rotary_dim - 1, math.ceil(pair(slow)))
