@@ -186,6 +186,19 @@ _INPUTS = {"rope": _rope_inputs, "attention": _attention_inputs, "sample": _samp
 _compute = None
 
 
+def _connect():
+    """The framework's context. Its stream becomes torch's current one, so that what torch does with the buffers, before
+    the operators run or with what they wrote, keeps its place among their launches; a caller who makes another
+    stream the current one orders it after this one."""
+    global _compute
+    if _compute is None:
+        from webgpu_amd.gpu import Compute
+        _compute = Compute().init()
+    if torch.cuda.current_stream().cuda_stream != _compute.stream:
+        torch.cuda.synchronize()
+        torch.cuda.set_stream(torch.cuda.ExternalStream(_compute.stream))
+
+
 class _View:
     """The CUDA array interface of a framework buffer that lives as long as the tensors over it."""
 
@@ -203,10 +216,6 @@ class _Buffers:
     """The inputs of a case in buffers of the framework, and torch tensors over the same memory."""
 
     def __init__(self, inputs):
-        global _compute
-        if _compute is None:
-            from webgpu_amd.gpu import Compute
-            _compute = Compute().init()
         self.at, self.tensor = {}, {}
         for name, t in inputs.items():
             if name in ("sees", "depth") or t is None:
@@ -337,6 +346,8 @@ def _full(case):
 
 
 def prepare(case, seed):
+    if own:
+        _connect()
     inputs = _INPUTS[case["kind"]](case, seed)
     return _full(case), _Buffers(inputs) if own else inputs
 
