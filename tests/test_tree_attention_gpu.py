@@ -1,10 +1,15 @@
-"""Tree attention where its launches differ: what lies behind the partial outputs of splits."""
+"""Tree attention where its launches differ: what lies behind the partial outputs of splits, and the kernel that
+stages keys in LDS (k_attn_tree_staged) with two and four row groups in a workgroup, windows that hide cached
+keys, and rings that wrap. Bounds are those of tests/tree_dense.py.
+"""
 import math
 
 import numpy as np
 import pytest
 
-from tests.test_tree_gpu import NO_WINDOW, Held, assert_near, random_tree, run_tree, tree_case
+from tests import tree_dense
+from tests.test_tree_gpu import Held, assert_near, random_tree, run_tree, tree_case, up  # noqa: F401
+from tests.tree_dense import NO_WINDOW, STAGED
 from webgpu_amd.gpu import Compute
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +35,14 @@ def test_pairs_behind_an_odd_count_of_partial_outputs(heads, hd, nodes, start, s
     finally:
         up.free()
         gpu.dispose()
+
+
+@pytest.mark.parametrize("case", STAGED, ids=lambda c: "-".join("w" if v == NO_WINDOW else str(v) for v in c))
+def test_staged_keys(gpu, up, case):  # noqa: F811
+    start, window = case[4:6]
+    q, k, v, parents, sees, first, scale = tree_dense.inputs(case, case[3] // 8)
+    want, S = tree_dense.attention(q, k, v, sees, first, scale)
+    got = run_tree(gpu, up, q, k, v, parents, start, scale, window, tail=5)
+    keys, most = sees.shape[1], float(np.abs(v).max())
+    assert tree_dense.within(got, want, S, keys, most), (np.abs(got - want).max(), np.linalg.norm(got - want), tree_dense.bounds(want, S, keys, most))
+    assert np.all(got[~sees.any(1)] == 0)
