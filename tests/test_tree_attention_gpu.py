@@ -46,3 +46,32 @@ def test_staged_keys(gpu, up, case):  # noqa: F811
     keys, most = sees.shape[1], float(np.abs(v).max())
     assert tree_dense.within(got, want, S, keys, most), (np.abs(got - want).max(), np.linalg.norm(got - want), tree_dense.bounds(want, S, keys, most))
     assert np.all(got[~sees.any(1)] == 0)
+
+
+# heads, kv_heads, head_dim, nodes, start, window, slots to spare: staged with two row groups, with four, in a window
+REDONE = [(7, 1, 128, 64, 3000, NO_WINDOW, 4), (16, 1, 64, 70, 2000, NO_WINDOW, 4), (8, 1, 256, 33, 2500, NO_WINDOW, 4),
+          (8, 1, 128, 64, 9001, 2500, 27), (4, 1, 128, 64, 20011, 8200, 3), (4, 1, 256, 32, 6000, 2100, 27)]
+
+
+@pytest.mark.parametrize("case", REDONE, ids=lambda c: "-".join("w" if v == NO_WINDOW else str(v) for v in c))
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_rows_formed_again_hold_the_formula(gpu, up, case, bad):  # noqa: F811
+    """A node's K and V that are not finite: the nodes that do not see it keep the values that the formula gives
+    (tests/test_tree_dense.py shows what the bounds tell apart)."""
+    start, window, nodes = case[4], case[5], case[3]
+    q, k, v, parents, sees, first, scale = tree_dense.inputs(case, 0)
+    want, S = tree_dense.attention(q, k, v, sees, first, scale)
+    most, keys, hit = float(np.abs(v).max()), sees.shape[1], nodes // 2
+    hits = [(start + hit, sees[:, hit - nodes])]
+    if window != NO_WINDOW:
+        hits.append((first, sees[:, 0]))  # the cached key that only nodes of depth 0 see
+    for t, seen in hits:
+        free = np.flatnonzero(~seen)
+        assert 0 < len(free) < nodes
+        k1, v1 = k.copy(), v.copy()
+        k1[t % len(k)], v1[t % len(k)] = bad, bad
+        unused = [(start + nodes + e) % len(k) for e in range(case[6])]
+        k1[unused], v1[unused] = bad, bad
+        got = run_tree(gpu, up, q, k1, v1, parents, start, scale, window)
+        assert tree_dense.within(got[free], want[free], S, keys, most), (np.abs(got - want)[free].max(), tree_dense.bounds(want[free], S, keys, most))
+        assert not np.isfinite(got[seen]).any()

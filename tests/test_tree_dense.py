@@ -31,7 +31,7 @@ def mistakes(sees, nodes, window):
     yield "a block of keys lost", wrong
 
 
-@pytest.mark.parametrize("case", [c for c in STAGED if c[1] == 1], ids=lambda c: "-".join("w" if v == NO_WINDOW else str(v) for v in c))
+@pytest.mark.parametrize("case", [c for c in STAGED if c[1] == 1] + [(7, 1, 128, 64, 3000, NO_WINDOW, 4), (8, 1, 256, 33, 2500, NO_WINDOW, 4)], ids=lambda c: "-".join("w" if v == NO_WINDOW else str(v) for v in c))
 def test_the_bounds_tell_wrong_masks_apart(case):
     q, k, v, parents, sees, first, scale = tree_dense.inputs(case, case[3] // 8)
     want, S = tree_dense.attention(q, k, v, sees, first, scale)
