@@ -481,9 +481,12 @@ hipError_t sample(hipStream_t s, const float *logits, uint32_t n, const SamplePa
 // last 7.6.
 // A cut's token is found in its list by a histogram of RS_SUB parts of the bin and a sort of the one part
 // that holds it (a sort of the whole list took four times as long).
-// A bin or bound with more tokens than a list holds (ties, logits close together for the temperature) goes through
-// pick_row, which refines by 11 bits of the composite at a time, in one workgroup.
-constexpr uint32_t RS_T = 512, RS_BINS = 2048, RS_CAP = 2048, RS_DRAW = 8192, RS_SUB = 1024;
+// A bin with more tokens than its list holds (RS_LIST in all, RS_CAP from one workgroup and in one part of the bin: ties, or
+// logits that lie within a few tens of bins, so less than the temperature apart), or more than RS_CAP candidates of a
+// small top-k, send a row through pick_row, which refines by 11 bits of the composite at a time, in one workgroup. 16 rows
+// of 262144, top-p: 40 us where that bin holds 700 tokens, 49 where it holds 2300 (650 by pick_row, with lists of
+// RS_CAP), 5.0 ms where all are equal; top-k 40 of equal logits 7.4 ms.
+constexpr uint32_t RS_T = 512, RS_BINS = 2048, RS_CAP = 2048, RS_LIST = 8192, RS_SUB = 1024;
 constexpr uint32_t RS_ROWS = 256;  // rows per launch: the histograms of more would only fill memory
 constexpr float RS_SPAN = 48.f;    // bins cover exp(0) to exp(-48) < 2^-62; the last one all below
 constexpr uint32_t RS_SLICES = 64, RS_SLICE = 4096;  // most slices of a row, least logits of one
@@ -495,7 +498,7 @@ struct RowSlice { uint64_t best; uint32_t finite, pad; };
 struct RowHist {
   uint64_t mass[RS_BINS];
   uint32_t count[RS_BINS];
-  uint64_t list[2][RS_CAP], draw[RS_DRAW];  // of top-k, top-p and the draw
+  uint64_t list[3][RS_LIST];                 // of top-k, top-p and the draw
   uint32_t nlist[3], slow[2];                // slow: k_rows_topk or k_rows_cuts has a list that is full
   uint64_t minp, s;                          // the weights that min-p and top-k keep
   uint64_t pmass, dmass;                     // the weights before top-p's bin and before the draw's bins b0 .. b1
@@ -1044,17 +1047,16 @@ __global__ __launch_bounds__(RS_T) void k_rows_topk(RowsK a) {
     append(L.list, &L.nlist, ok && row_bin(a, bv, v) == bin, composite(v, i));
   });
   __syncthreads();
-  put_list(L, L.list, L.nlist, h.list[CUT_K], RS_CAP, &h.nlist[CUT_K], &h.slow[0]);
+  put_list(L, L.list, L.nlist, h.list[CUT_K], RS_LIST, &h.nlist[CUT_K], &h.slow[0]);
 }
 
-// The weight that the top-k cut leaves, from its list.
-__device__ __forceinline__ uint64_t topk_mass(const RowsK &a, PickLds &L, const RowHist &h, float bv) {
+// The weight that the top-k cut leaves, from its list (*ok as cut_list's).
+__device__ __forceinline__ uint64_t topk_mass(const RowsK &a, PickLds &L, const RowHist &h, float bv, bool *ok) {
   uint64_t m;
   find_cross(L, a.top_k, ~0ull);
-  const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[CUT_K], RS_CAP);
+  const uint32_t bin = L.x_bin, before = L.x_count, n = min(h.nlist[CUT_K], RS_LIST);
   const uint64_t mbefore = L.x_mass;
-  bool ok;  // the list is no longer than cut_list takes
-  cut_list(a, L, bv, h.list[CUT_K], n, bin, bin, before, mbefore, a.top_k, ~0ull, &m, &ok);
+  cut_list(a, L, bv, h.list[CUT_K], n, bin, bin, before, mbefore, a.top_k, ~0ull, &m, ok);
   return m;
 }
 
@@ -1072,7 +1074,12 @@ __global__ __launch_bounds__(RS_T) void k_rows_cuts(RowsK a) {
   if (!finite || h.slow[0] || !(u > 0.0 && u < 1.0)) return;  // slow[0]: of the launch before
   const float bv = comp_value(best);
   load_hist(L, h);
-  const uint64_t S = a.top_k && a.top_k < finite ? topk_mass(a, L, h, bv) : L.mass[RS_BINS - 1];
+  bool ok = true;
+  const uint64_t S = a.top_k && a.top_k < finite ? topk_mass(a, L, h, bv, &ok) : L.mass[RS_BINS - 1];
+  if (!ok) {  // as every workgroup of the row finds
+    if (threadIdx.x == 0) h.slow[1] = 1;
+    return;
+  }
   uint64_t least = S, most = S, pmass = 0;  // of the weight that top-p keeps; before its bin
   uint32_t pbin = RS_BINS;                  // none
   if (a.top_p < 1.0) {
@@ -1104,8 +1111,8 @@ __global__ __launch_bounds__(RS_T) void k_rows_cuts(RowsK a) {
     append(L.part, &L.npart, b >= b0 && b <= b1, composite(v, i));
   });
   __syncthreads();
-  put_list(L, L.list, L.nlist, h.list[CUT_P], RS_CAP, &h.nlist[CUT_P], &h.slow[1]);
-  put_list(L, L.part, L.npart, h.draw, RS_DRAW, &h.nlist[CUT_DRAW], &h.slow[1]);
+  put_list(L, L.list, L.nlist, h.list[CUT_P], RS_LIST, &h.nlist[CUT_P], &h.slow[1]);
+  put_list(L, L.part, L.npart, h.list[CUT_DRAW], RS_LIST, &h.nlist[CUT_DRAW], &h.slow[1]);
 }
 
 // The token: the best where nothing is drawn, else from the lists.
@@ -1124,14 +1131,17 @@ __global__ __launch_bounds__(RS_T) void k_rows_last(RowsK a, uint32_t drawn) {
     bool slow = h.slow[0] || h.slow[1];
     if (!slow) {
       uint64_t R = h.s, unused;
-      bool ok;
-      if (a.top_p < 1.0)  // (its list is no longer than cut_list takes)
-        cut_list(a, L, bv, h.list[CUT_P], min(h.nlist[CUT_P], RS_CAP), h.pbin, h.pbin, 0, h.pmass, ~0ull, at_least(a.top_p * (double)R, R), &R, &ok);
-      R = min(R, h.minp);
-      const uint64_t c = cut_list(a, L, bv, h.draw, min(h.nlist[CUT_DRAW], RS_DRAW), h.b0, h.b1, 0, h.dmass, ~0ull, at_least(u * (double)R, R),
-                                  &unused, &ok);
+      bool ok = true;
+      if (a.top_p < 1.0)
+        cut_list(a, L, bv, h.list[CUT_P], min(h.nlist[CUT_P], RS_LIST), h.pbin, h.pbin, 0, h.pmass, ~0ull, at_least(a.top_p * (double)R, R), &R, &ok);
       slow = !ok;
-      token = (int32_t)comp_index(c);
+      if (!slow) {
+        R = min(R, h.minp);
+        const uint64_t c = cut_list(a, L, bv, h.list[CUT_DRAW], min(h.nlist[CUT_DRAW], RS_LIST), h.b0, h.b1, 0, h.dmass, ~0ull,
+                                    at_least(u * (double)R, R), &unused, &ok);
+        slow = !ok;
+        token = (int32_t)comp_index(c);
+      }
     }
     if (slow) {
       row_hist(a, L, h, a.logits + blockIdx.x * a.stride, bv);
