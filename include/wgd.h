@@ -237,23 +237,27 @@ int wgd_embed(wgd_context *ctx, int32_t type, const wgd_buffer *table, const wgd
  *   a = positions[t] * scale * theta^(-2j/rot) / factors[j].
  * positions is int32[batch], factors f32[rot/2] or NULL for ones; linear, NTK, by-parts (YaRN)
  * and Llama 3 scaling are factors and a magnitude (webgpu_amd/rope.py makes them). Angles are
- * formed and reduced in f64, and the tail of a head is left as it is. Query and key heads that
- * lie side by side in a row are one call. For models with Q/K norm run wgd_norm with n =
- * head_dim first. */
+ * formed and reduced in f64, their cosine and sine are off by at most 2^-29 before they are rounded
+ * to f32, and the tail of a head is left as it is. Query and key heads that lie side by side in
+ * a row are one call. For models with Q/K norm run wgd_norm with n = head_dim first. */
 int wgd_rope_at(wgd_context *ctx, wgd_buffer *x, const wgd_buffer *positions, const wgd_buffer *factors,
                 uint32_t heads, uint32_t head_dim, float theta, float scale, float magnitude, uint32_t rotary_dim,
                 uint32_t stride, uint64_t offset, int32_t adjacent, uint32_t batch);
 /* Attention of every node of a drafted tree: query q[i][h] over the cached keys t in
  * (position_i - window, start), at ring slot t % capacity as in wgd_attention, and over i itself
  * and its ancestors within the window; y[i][h] = softmax(scale * q.k) V, zeros for padding. A
- * node outside i's ancestors never reaches y[i], whatever its K/V hold. Needs nodes <=
+ * node outside i's ancestors never reaches y[i], whatever its K/V hold; NaN and infinities there
+ * have the rows that share a workgroup with them formed again, some hundred times slower. Needs nodes <=
  * WGD_TREE_MAX, head_dim <= 512, start < 2^31, heads <= 2^20, nodes * heads < 2^26, nodes * heads /
  * kv_heads <= 1048560 and a ring that holds every key that some node sees, min(start, window - 1) + nodes
  * <= capacity. */
 int wgd_attention_tree(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *y,
                        const wgd_buffer *parents, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t start,
                        float scale, uint32_t window, uint32_t capacity, uint32_t nodes);
-/* The same over f16 rings (wgd_attention_f16kv's): scores, softmax and sums stay f32. */
+/* The same over f16 rings (wgd_attention_f16kv's). Scores, maxima, sums and outputs are f32; with a head_dim
+ * that is a multiple of 8, up to 256, queries and weights enter the products as two f16 each: an
+ * entry of a query is off by 2^-22 of itself and 2^-39 of the row's largest, a weight by 2^-22 of
+ * itself and 2^-36 of the largest one. */
 int wgd_attention_tree_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v,
                              wgd_buffer *y, const wgd_buffer *parents, uint32_t heads, uint32_t kv_heads,
                              uint32_t head_dim, uint32_t start, float scale, uint32_t window, uint32_t capacity,
@@ -264,9 +268,9 @@ int wgd_attention_tree_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_bu
  * exp((l - best) / temperature); kept are the top_k first (0: all of them), of these the
  * shortest prefix whose share of their weight reaches top_p, and of these the ones with a weight
  * of min_p or more; the token is the first whose running sum reaches uniform * (the kept
- * weight). With min_p 0 that is wgd_sample's rule. Weights and sums are integers of
- * 2^-min(51, 62 - ceil(log2 n)) of the largest weight, so a draw does not depend on the order of
- * the sums.
+ * weight). With min_p 0 that is wgd_sample's rule. Weights are formed to 2^-46 of themselves; they and
+ * their sums are integers of 2^-min(51, 62 - ceil(log2 n)) of the largest weight, so a draw does not
+ * depend on the order of the sums.
  * Temperature 0 takes the best; so does a uniform outside [0, 1). A row without a finite logit
  * gets -1. temperature <= 2, 0 < top_p <= 1, 0 <= min_p <= 1 (WGD_E_INVALID otherwise). */
 int wgd_sample_rows(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, uint32_t rows, uint32_t stride,

@@ -75,3 +75,61 @@ def test_rows_formed_again_hold_the_formula(gpu, up, case, bad):  # noqa: F811
         got = run_tree(gpu, up, q, k1, v1, parents, start, scale, window)
         assert tree_dense.within(got[free], want[free], S, keys, most), (np.abs(got - want)[free].max(), tree_dense.bounds(want[free], S, keys, most))
         assert not np.isfinite(got[seen]).any()
+
+
+# ------------------------------------------------------------------------------- what f16 rings round
+#
+# Over f16 rings, head dims that are multiples of 8 up to 256, a query is held as two f16: off by 2^-22 of itself and 2^-39
+# of the row's largest |q|, Q. So are the weights, by 2^-22 of themselves and 2^-36 of the largest; their sum has them
+# in f32. With e = 2^-24 a score (2 hd products of f16 added in f32) is off by
+#   d = scale ((2^-22 + (2 hd + 8) e) sum|q k| + 2^-39 Q sum|k|) + e (|s| + 32),
+# a weight by r = 2 d + 2^-21 of itself, sums of n terms by n e, and an output by
+#   (sum w |v| (r + n e) + 2^-36 sum|v|) / sum w + |y| (r + n e).
+# f32 rings: without the terms of 2^-39 and 2^-36.
+
+def rounding(q, k, v, scale, half):
+    """Exact outputs of one query and their bounds: q [hd], k and v [n][hd]."""
+    q, k, v = (a.astype(np.float64) for a in (q, k, v))
+    n, hd, e = len(k), len(q), 2.0 ** -24
+    s = k @ q * scale
+    w = np.exp(s - s.max())
+    d = scale * ((2.0 ** -22 + (2 * hd + 8) * e) * (np.abs(k) @ np.abs(q)).max() + (2.0 ** -39 * np.abs(q).max() * np.abs(k).sum(1).max() if half else 0))
+    r = 2 * (d + e * (np.abs(s).max() + 32)) + 2.0 ** -21
+    y = w @ v / w.sum()
+    grid = 2.0 ** -36 * np.abs(v).sum(0) if half else 0
+    return y, (w @ np.abs(v) * (r + n * e) + grid) / w.sum() + np.abs(y) * (r + n * e)
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
+@pytest.mark.parametrize("hd,heads,start", [(64, 1, 900), (128, 1, 900), (256, 1, 900), (72, 1, 900), (64, 64, 8500), (128, 64, 8500), (256, 64, 8500)])
+@pytest.mark.parametrize("faint", [-12.0, -18.3, -25.4, -31.7, -40.2])
+def test_faint_weights(gpu, up, hd, heads, start, faint, kv):  # noqa: F811
+    """A first key that takes nearly all the weight and whose value is 0, beside keys of weight 2^faint."""
+    half = kv == "f16"
+    q = np.zeros((1, heads, hd), np.float32)
+    q[..., 0] = 1
+    k, v = np.zeros((start + 1, 1, hd), np.float32), np.ones((start + 1, 1, hd), np.float32)
+    k[0, 0, 0], v[0] = 16, 0
+    v[1:] += 0.25 * (np.arange(hd) % 3)
+    dtype = np.float16 if half else np.float32
+    k, v, scale = k.astype(dtype), v.astype(dtype), -faint * math.log(2) / 16
+    want, bound = rounding(q[0, 0], k[:, 0], v[:, 0], scale, half)
+    got = run_tree(gpu, up, q, k, v, np.array([-1], np.int32), start, scale, NO_WINDOW)
+    assert np.all(np.abs(got[0] - want) <= bound), (np.abs(got[0] - want).max() / want.max(), (bound / want).max())
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
+@pytest.mark.parametrize("hd,heads,start", [(64, 1, 900), (128, 1, 900), (256, 1, 900), (72, 1, 900), (64, 64, 8500), (128, 64, 8500), (256, 64, 8500)])
+@pytest.mark.parametrize("largest", [2.0 ** 12, 2.0 ** 18, 2.0 ** 24])
+def test_queries_with_one_large_entry(gpu, up, hd, heads, start, largest, kv):  # noqa: F811
+    """Where the keys are 0: the scores come from the small entries."""
+    half = kv == "f16"
+    rng = np.random.default_rng(hd)
+    q = rng.standard_normal((1, heads, hd)).astype(np.float32)
+    q[..., 3] = largest
+    k, v = (rng.standard_normal((start + 1, 1, hd)).astype(np.float16 if half else np.float32) for _ in range(2))
+    k[..., 3] = 0
+    got = run_tree(gpu, up, q, k, v, np.array([-1], np.int32), start, 1 / math.sqrt(hd), NO_WINDOW)
+    for h in range(heads):
+        want, bound = rounding(q[0, h], k[:, 0], v[:, 0], 1 / math.sqrt(hd), half)
+        assert np.all(np.abs(got[0, h] - want) <= bound), (h, np.abs(got[0, h] - want).max(), bound.max())

@@ -271,7 +271,11 @@ __global__ __launch_bounds__(256) void k_attn_tree_any(TreeK a) {
 // O^T += V^T P^T.
 //   f16 rings (v_mfma_f32_16x16x32_f16): K and V are operands as they are, exact. The queries (times
 //     scale log2 e) are split into f16 hi + lo with a power of two per row, the probabilities with a
-//     factor of 2^11: 22 bits each, two products in place of one. Lane (g, c) loads VE values d = VE c of
+//     factor of 2^11: two products of f16 in place of one of f32, whose rate is an eighth. Each is off by 2^-22 of
+//     itself (f32: 2^-24) and by half of f16's least step, 2^-25: below 2^-39 of a row's largest query entry, which
+//     lies in [2^14, 2^15), and 2^-36 of its largest weight, 2^11 at least. A weight below 2^-36 of the largest is in the
+//     sum, which has them in f32, and not in the outputs: n such keys are n 2^-36 of the largest value at
+//     most, where f32 sums of n terms may be off by n 2^-24. Lane (g, c) loads VE values d = VE c of
 //     its eight keys and picks the d-th halves of the eight with v_perm: output tile (x, e) is
 //     the dims 16 VE x + VE m + e.
 //   f32 rings (v_mfma_f32_16x16x4_f32): f32 products and sums.
