@@ -737,8 +737,8 @@ __global__ __launch_bounds__((tree_threads<HD>())) void k_attn_tree(TreeK a, Tre
 // stage of SK keys into LDS once, straight from memory (no registers), while they work on the one before; a
 // wavefront's blocks of 32 keys are its slice's. K rows and V rows lie in 16-byte chunks; chunk i of key k
 // at place i ^ swizzle(k), so that the 16 keys of a K operand, and the 16-bit transposing reads that make V
-// operands (4 keys of one dim per lane), meet all banks evenly. 64 nodes, 32 heads on 8 of 128, 31000 keys: 75 us (direct
-// 112), 433 TFLOP/s counted once, twice that with the split operands. Matrix products take 36% of the cycles and the issue of
+// operands (4 keys of one dim per lane), meet all banks evenly. 64 nodes, 32 heads on 8 of 128, 31000 keys: 75 us (k_attn_tree
+// 158), 433 TFLOP/s counted once, twice that with the split operands. Matrix products take 36% of the cycles and the issue of
 // vector instructions 39%; a wavefront is at waits for LDS, loads and the others of its stage 37% of its life, two to a SIMD.
 // Two V operands at LDS addresses `at`: dims in transposing reads of keys 0 .. 4 and, OFF bytes on, 16 .. 20 of each lane
 // group. The builtin of this read waits for every load from memory into LDS that is under way, the next
@@ -957,8 +957,9 @@ __global__ __launch_bounds__(256) void k_attn_tree_join(const float *part, float
 
 static uint32_t tree_first(const TreeAttnArgs &in) { return in.start - std::min(in.start, in.window - 1); }
 
-// mfma: the kernel for head dims 64, 128 and 256; RT tiles of 16 rows per wavefront, rw groups of them
-// and `waves` wavefronts per workgroup.
+// mfma: a kernel of matrix products, for head dims that are multiples of 8 up to 256, padded to HD = 64, 128 or 256;
+// RT tiles of 16 rows per wavefront (two in the staged kernel up to 128, one else), rw groups of them and `waves`
+// wavefronts per workgroup.
 struct TreePlan { bool mfma, staged; uint32_t HD, T, RT, rw, waves, per, blocks, nsplit; };
 static TreePlan tree_plan(const TreeAttnArgs &in) {
   TreePlan p{};
@@ -971,7 +972,8 @@ static TreePlan tree_plan(const TreeAttnArgs &in) {
     const uint32_t tiles = (rows + 15) / 16, unit = in.kv16 ? 32 : 16;
     // Staged from where its reuse of the keys outweighs its slower start. us, direct against staged, 8 kv heads:
     //   hd 128, 4 tiles, 16000 keys 29.4 / 28.0 (4000: 17.2 / 22.9); 8 tiles, 4000 keys 20.1 / 20.6 (1000: 14.1 / 17.5);
-    //   16 tiles, 4000 keys 28.6 / 24.6 (1000: 16.3 / 18.9), 16000 keys 80 / 47; hd 256, 8 tiles, 4000 keys 32.5 / 28.4.
+    //   16 tiles, 4000 keys 28.6 / 24.6 (1000: 16.3 / 18.9), 16000 keys 80 / 47; hd 256, 8 tiles, 4000 keys 32.5 / 28.4
+    //   (with two row groups: a stage of 64 keys is two blocks then, for four slices, so half of the wavefronts have none).
     p.staged = in.kv16 && in.hd == p.HD && tiles >= 4 && (uint64_t)tiles * keys >= (p.HD == 256 ? 16000 : 32000);
     p.RT = p.staged && p.HD <= 128 ? 2 : 1;
     p.waves = p.staged || p.HD <= 128 ? 8 : 4;
@@ -980,7 +982,9 @@ static TreePlan tree_plan(const TreeAttnArgs &in) {
     // ends in 4.5 and works 2.1 (f16) or 3.1 (f32) for a block of each slice; the join adds 3.3. hd 128, 8 kv heads, one
     // node: f16 300 keys 8.9 in one split, 11.3 in two; 1000 keys 14.9 and 13.7, 11.9 in four; f32 300 keys 13.2
     // in one, 12.3 in three; f32 1071 keys of 16 kv heads, 6 tiles: 24.4 us with one row group in two splits, 22.7 with two
-    // in five.
+    // in five. All of it is measured at hd 128 with up to five splits: hd 64 and 256 go by the same figures, a staged block by
+    // the direct kernel's, and the join of a few hundred splits takes longer than 3.3 (8 nodes, 8 heads on one of 256, 31000 keys:
+    // 243 splits, 50 us in all).
     const uint32_t kb = (keys + unit - 1) / unit;
     const double block = in.kv16 ? 2.1 : 3.1;
     uint32_t want = 1;
