@@ -268,7 +268,7 @@ int wgd_attention_tree_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_bu
  * exp((l - best) / temperature); kept are the top_k first (0: all of them), of these the
  * shortest prefix whose share of their weight reaches top_p, and of these the ones with a weight
  * of min_p or more; the token is the first whose running sum reaches uniform * (the kept
- * weight). With min_p 0 that is wgd_sample's rule. Weights are formed to 2^-46 of themselves; they and
+ * weight). With min_p 0 that is wgd_sample's rule. Weights are formed to 2^-45 of themselves; they and
  * their sums are integers of 2^-min(51, 62 - ceil(log2 n)) of the largest weight, so a draw does not
  * depend on the order of the sums.
  * Temperature 0 takes the best; so does a uniform outside [0, 1). A row without a finite logit

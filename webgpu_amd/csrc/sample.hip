@@ -518,9 +518,9 @@ struct RowsK {
 __device__ __forceinline__ uint32_t row_bin(const RowsK &a, float best, float l) {
   return (uint32_t)fminf((best - l) * a.bins, (float)(RS_BINS - 1));
 }
-// exp((l - best) / T) to 2^-46 of it, well below the grid of all but the largest weights: 2^k times the Taylor sum of the rest r,
-// |r| <= ln 2 / 2, whose next term is below 7e-15; the quotient and the rest round as much again. More terms would
-// lengthen a chain that bounds k_rows_hist as it is.
+// exp((l - best) / T) to 2^-45 of it, which is finer than the grid of all but the largest weights: 2^k times the Taylor sum of the
+// rest r, |r| <= ln 2 / 2. The next term is below 9e-15 of it, the roundings of 1 / T, of the quotient and of r add up to 1.1e-14
+// at 48; measured 1.33e-14. More terms would lengthen a chain that bounds k_rows_hist as it is.
 // Below 2^-70 it is 0: less than half of the least integer below, whatever n.
 __device__ __forceinline__ double row_weight(const RowsK &a, float best, float l) {
   const double x = fmax(((double)l - (double)best) * a.inv_t, -64.0);
