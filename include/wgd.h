@@ -292,6 +292,92 @@ int wgd_tree_accept(wgd_context *ctx, const wgd_buffer *parents, const wgd_buffe
 int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, const wgd_buffer *path,
                   uint64_t row_bytes, uint32_t start, uint32_t capacity, uint32_t nodes);
 
+/* ---------------------------------------------------------------- many requests
+ * A step of a batch of requests (no reference counterpart). Their keys and values lie in pages: of one
+ * K and one V pool per layer, [pages][page][kv_heads][head_dim] in f32 or f16, page `table[r * max_pages + c]` holds
+ * the tokens c * page .. + page of request r (int32[requests][max_pages]); lengths[r] (int32) is how many tokens it has
+ * and refs[p] (int32[pages]) how many rows of the table hold page p; 0 or less is a free page. Zero-filled buffers are the empty
+ * state. A host that keeps pages itself adds to their refs. The page is a power of two up to WGD_PAGE_MAX; requests <=
+ * WGD_REQUESTS_MAX; max_pages * page and pages * page are below 2^31. Lengths outside [0, max_pages * page] count as
+ * the nearest end. These launches wait for nothing, and their choices do not depend on the order of threads. They
+ * allocate nothing once a call of the same sizes has run (WGD_E_STATE where a capture would have to). Buffers that a call writes
+ * are others than those that it reads, unless it says so. */
+#define WGD_REQUESTS_MAX 1024
+#define WGD_PAGE_MAX 1024
+
+/* Places for counts[r] (int32[requests], in [0, tokens]; NULL: `tokens` each) new tokens of every request: in the
+ * order of requests, each takes the lowest free pages that it needs beyond those it has, or where fewer are left none
+ * at all: then, and where the tokens do not fit max_pages or counts[r] lies outside, added[r] (int32[requests]) becomes -1
+ * and the request stays as it was, while later ones may still fit. Else added[r] = counts[r], which is what lengths[r] grows
+ * by; positions[r * tokens + t] (for wgd_rope_at) and slots[r * tokens + t] (page * id + place, for wgd_pages_store) are
+ * those of its t-th new token, and -1 where there is none (both int32[requests * tokens]). requests * tokens <= 2^24. */
+int wgd_pages_extend(wgd_context *ctx, wgd_buffer *table, wgd_buffer *lengths, wgd_buffer *refs, const wgd_buffer *counts,
+                     wgd_buffer *added, wgd_buffer *positions, wgd_buffer *slots, uint32_t requests, uint32_t tokens,
+                     uint32_t page, uint32_t max_pages, uint32_t pages);
+/* Requests that fork, end or lose their last tokens: request r becomes the first keep[r] tokens (NULL, or more than
+ * there are: all) of what request origin[r] was (both int32[requests]); an origin outside [0, requests) leaves it empty. So
+ * origin[r] = r keeps r (cut to keep[r]), another one makes r its copy, -1 frees it. Full pages are shared. A last page that is not
+ * full belongs to one request alone: if nobody else holds it, it stays with the lowest of those that end in it; the
+ * others, in order, get the lowest free pages, and copies (int32[2 * requests + 1]) becomes the number of these and their
+ * (source, target) pairs, -1 behind them: run wgd_pages_copy with it on the pools of all layers before anything is
+ * written to them. Pages that are no longer held are free. Where the free pages do not suffice nothing changes and copies[0] is
+ * -1. Columns behind a changed request's last page become -1. */
+int wgd_pages_fork(wgd_context *ctx, wgd_buffer *table, wgd_buffer *lengths, wgd_buffer *refs, const wgd_buffer *origin,
+                   const wgd_buffer *keep, wgd_buffer *copies, uint32_t requests, uint32_t page, uint32_t max_pages,
+                   uint32_t pages);
+/* Compaction: with n pages in use, the j-th used one at n or above moves to the j-th free one below n, so that the used
+ * pages are the first n. moved (int32[pages]) becomes every used page's new number, -1 for free ones; copies (int32[2 *
+ * (pages / 2) + 1]) the number of moves and their (source, target) pairs, -1 behind them, for wgd_pages_copy. table_to and
+ * refs_to are the table and counts afterwards; they may be table and refs themselves. Without that the old ones stay
+ * valid until a page is written. Entries of the table outside [0, pages) stay. */
+int wgd_pages_compact(wgd_context *ctx, const wgd_buffer *table, const wgd_buffer *refs, wgd_buffer *table_to,
+                      wgd_buffer *refs_to, wgd_buffer *moved, wgd_buffer *copies, uint32_t requests, uint32_t max_pages,
+                      uint32_t pages);
+/* Page copies[1 + 2 i] to page copies[2 + 2 i] for i < copies[0] <= most, in every one of `count` distinct pools (a host
+ * array, at most 65536; copies as the calls above write it: targets differ from one another and from all sources) of [pages][page_bytes],
+ * page_bytes a multiple of 2 up to 2^30. Pairs with a number outside [0, pages) move nothing. */
+int wgd_pages_copy(wgd_context *ctx, wgd_buffer *const *pools, uint32_t count, const wgd_buffer *copies, uint32_t most,
+                   uint64_t page_bytes, uint32_t pages);
+/* K and V rows of new tokens into the pools: row t < rows, `row` = kv_heads * head_dim floats at k + k_offset + t * stride
+ * and v + v_offset + t * stride (floats; stride 0: row; k and v may be one buffer), to slot slots[t] of pools of
+ * slots_in_pool = pages * page rows. Slots are distinct; those outside [0, slots_in_pool) store nothing. */
+int wgd_pages_store(wgd_context *ctx, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *k_pool, wgd_buffer *v_pool,
+                    const wgd_buffer *slots, uint32_t row, uint32_t rows, uint32_t stride, uint64_t k_offset,
+                    uint64_t v_offset, uint32_t slots_in_pool);
+/* The same into pools of halves, rounded to nearest (ties to even). */
+int wgd_pages_store_f16kv(wgd_context *ctx, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *k_pool,
+                          wgd_buffer *v_pool, const wgd_buffer *slots, uint32_t row, uint32_t rows, uint32_t stride,
+                          uint64_t k_offset, uint64_t v_offset, uint32_t slots_in_pool);
+/* Attention of the last counts[r] tokens of every request (int32[requests], as `added` of wgd_pages_extend; NULL:
+ * `tokens`; none where it is 0 or less, at most `tokens` and lengths[r]): q[r][t][h] at the position p = lengths[r] - counts[r] + t
+ * sees the keys (p - window, p] of its request; y[r][t][h] = softmax(scale * q.k) V, zeros for t >= counts[r]. q and
+ * y are [requests][tokens][heads][head_dim], the keys of these tokens are stored already. Keys on pages outside [0, pages)
+ * are not seen, and a row that sees none gets zeros. What a row does not see never reaches it, whatever its K/V hold.
+ * shared > 0 (a multiple of page): requests that hold the same page in column shared / page - 1 as request `owner` hold the
+ * same ones in all columns before it, as wgd_pages_fork makes them; their first `shared` tokens are then computed together, for requests
+ * with new tokens, all of them behind the prefix, that the window does not cut. Results are the formula's either way.
+ * head_dim <= 512, heads <= 2^20, requests * tokens * heads <= 2^25, tokens * heads / kv_heads <= 2^20. */
+int wgd_attention_pages(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k_pool, const wgd_buffer *v_pool,
+                        wgd_buffer *y, const wgd_buffer *table, const wgd_buffer *lengths, const wgd_buffer *counts,
+                        uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale, uint32_t window, uint32_t page,
+                        uint32_t max_pages, uint32_t pages, uint32_t requests, uint32_t tokens, uint32_t shared,
+                        uint32_t owner);
+/* The same over pools of halves. */
+int wgd_attention_pages_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k_pool, const wgd_buffer *v_pool,
+                              wgd_buffer *y, const wgd_buffer *table, const wgd_buffer *lengths, const wgd_buffer *counts,
+                              uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale, uint32_t window,
+                              uint32_t page, uint32_t max_pages, uint32_t pages, uint32_t requests, uint32_t tokens,
+                              uint32_t shared, uint32_t owner);
+/* Low-rank adapters beside a projection (run it with wgd_matmul first): for rows t < batch with the adapter w =
+ * which[t] (int32[batch]),
+ *   y[t * stride + row_base + r] += scales[w] * sum_k B[w][r][k] (sum_c A[w][k][c] x[t][c]),  r < rows, k < rank, c < cols;
+ * rows with w outside [0, adapters) stay as they are, as does what lies around them. a is [adapters][rank][cols] and b
+ * [adapters][rows][rank], both F32 or F16 (`type`; GGUF's lora_a and lora_b as they are), lower ranks filled up with zeros;
+ * scales f32[adapters] (alpha / rank). Products and sums are f32. rank <= 1024. */
+int wgd_adapters(wgd_context *ctx, int32_t type, const wgd_buffer *a, const wgd_buffer *b, const wgd_buffer *which,
+                 const wgd_buffer *scales, const wgd_buffer *x, wgd_buffer *y, uint32_t cols, uint32_t rows, uint32_t rank,
+                 uint32_t adapters, uint32_t stride, uint32_t row_base, uint32_t batch);
+
 /* ---------------------------------------------------------------- measurement
  * No reference counterpart: `launches` back-to-back plain streaming reads of `bytes`
  * (multiple of 16), launch i reading copy i % copies of src (copies laid out `bytes`

@@ -1351,3 +1351,4 @@ hipError_t decode_attention(hipStream_t s, const DecodeAttnArgs &in) {
 }  // namespace wgd
 
 #include "attention_tree.h"
+#include "attention_pages.h"

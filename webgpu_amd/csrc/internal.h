@@ -238,6 +238,52 @@ hipError_t tree_accept(hipStream_t s, const int32_t *parents, const int32_t *dra
                        uint32_t nodes);
 hipError_t kv_commit(hipStream_t s, void *const *rings, uint32_t count, const int32_t *path, uint64_t row_bytes,
                      uint32_t start, uint32_t capacity, uint32_t nodes);
+// ---------------------------------------------------------------- pages and adapters (include/wgd.h)
+// A page has 2^shift tokens; max_pages << shift and pages << shift are below 2^31.
+struct PagesExtendArgs {
+  int32_t *table, *lengths, *refs; const int32_t *counts;  // counts may be null: `tokens` each
+  int32_t *added, *positions, *slots;
+  uint32_t requests, tokens, shift, max_pages, pages;
+};
+hipError_t pages_extend(hipStream_t s, const PagesExtendArgs &a);
+struct PagesForkArgs {
+  int32_t *table, *lengths, *refs; const int32_t *origin, *keep;  // keep may be null: whole rows
+  int32_t *copies;
+  uint32_t requests, shift, max_pages, pages;
+  int32_t *rows = nullptr, *settled = nullptr;  // rows: pages_fork_scratch_bytes(), settled lies behind
+};
+uint64_t pages_fork_scratch_bytes(const PagesForkArgs &a);
+hipError_t pages_fork(hipStream_t s, const PagesForkArgs &a);
+struct PagesCompactArgs {
+  const int32_t *table, *refs; int32_t *table_to, *refs_to, *moved, *copies;
+  uint32_t requests, max_pages, pages;
+};
+hipError_t pages_compact(hipStream_t s, const PagesCompactArgs &a);
+hipError_t pages_copy(hipStream_t s, void *const *pools, uint32_t count, const int32_t *copies, uint32_t most, uint64_t page_bytes,
+                      uint32_t pages);
+struct PagesStoreArgs {
+  const float *k, *v; void *k_pool, *v_pool; const int32_t *slots;
+  uint32_t row, rows; uint64_t stride; uint32_t slots_in_pool;
+  bool kv16 = false;
+};
+hipError_t pages_store(hipStream_t s, const PagesStoreArgs &a);
+struct PagesAttnArgs {
+  const float *q; const void *k, *v; float *y; const int32_t *table, *lengths, *counts;  // counts may be null
+  uint32_t heads, kv_heads, hd, window, shift, max_pages, pages, requests, tokens, shared, owner;
+  float scale;
+  bool kv16 = false;
+  float *partial = nullptr; uint64_t partial_floats = 0;  // at least attention_pages_scratch_floats()
+};
+uint64_t attention_pages_scratch_floats(const PagesAttnArgs &a);
+hipError_t attention_pages(hipStream_t s, const PagesAttnArgs &a);
+struct AdaptersArgs {
+  const void *a, *b; const int32_t *which; const float *scales, *x; float *y;
+  uint32_t cols, rows, rank, adapters, batch; uint64_t stride;
+  bool half = false;
+  float *partial = nullptr;  // adapters_scratch_floats()
+};
+uint64_t adapters_scratch_floats(const AdaptersArgs &a);
+hipError_t adapters(hipStream_t s, const AdaptersArgs &a);
 hipError_t add(hipStream_t s, const float *delta, float *state, uint32_t n);
 hipError_t glu(hipStream_t s, const float *gate, const float *up, float *y, uint32_t n, int act);
 // glu() over [batch][cols] that also writes y in the prompt GEMM's split form (cols % 64 == 0).

@@ -32,7 +32,7 @@ struct wgd_context {
   int32_t *sample_result = nullptr;            // the token of wgd_sample, in pinned host memory
   void *sample_scratch = nullptr;              // its slices' candidates
   uint64_t sample_scratch_bytes = 0;
-  void *tree_scratch = nullptr;                // of the drafted-tree launchers (tree_workspace in runtime.hip)
+  void *tree_scratch = nullptr;                // of the launchers of trees and of many requests (tree_workspace in runtime.hip)
   uint64_t tree_scratch_bytes = 0;
   bool tree_scratch_captured = false;          // a graph holds its address
 };

@@ -848,3 +848,6 @@ hipError_t argmax(hipStream_t s, const float *logits, uint32_t n, int32_t *out) 
 }
 
 }  // namespace wgd
+
+#include "pages.h"
+#include "adapters.h"

@@ -680,7 +680,7 @@ int wgd_sample(wgd_context *ctx, const wgd_buffer *logits, uint32_t n, double te
 
 // ---------------------------------------------------------------- drafted trees
 
-// Scratch of the drafted-tree launchers, grown by doubling and kept with the context. A captured
+// Scratch of the launchers of drafted trees and of many requests, grown by doubling and kept with the context. A captured
 // graph keeps its address: nothing is allocated during a capture, and a block that a graph may
 // hold is kept until the context ends when a larger one takes its place.
 static int tree_workspace(wgd_context *ctx, uint64_t need, const char *what, void **out) {
@@ -695,7 +695,7 @@ static int tree_workspace(wgd_context *ctx, uint64_t need, const char *what, voi
     uint64_t size = std::max(need, 2 * ctx->tree_scratch_bytes);
     ctx->tree_scratch = nullptr; ctx->tree_scratch_bytes = 0;
     if (ctx->allocated + size > ctx->limit) size = need;
-    int rc = ctx_alloc(ctx, size, "drafted-tree scratch", &ctx->tree_scratch);
+    int rc = ctx_alloc(ctx, size, "scratch of trees and batches", &ctx->tree_scratch);
     if (rc) return rc;
     ctx->tree_scratch_bytes = size;
     ctx->tree_scratch_captured = false;
@@ -831,6 +831,245 @@ int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, co
   if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
     return fail(ctx, WGD_E_INVALID, "kv_commit: a ring is given twice, or is the path");
   return ctx_check(ctx, kv_commit(ctx->stream, at.data(), count, (const int32_t *)path->ptr, row_bytes, start, capacity, nodes), "kv_commit");
+}
+
+// ---------------------------------------------------------------- many requests
+
+// The shape of a paged cache.
+static int pages_shape(wgd_context *ctx, const char *what, uint32_t requests, uint32_t page, uint32_t max_pages, uint32_t pages) {
+  if (requests > WGD_REQUESTS_MAX) return fail(ctx, WGD_E_INVALID, "%s: %u requests, a batch has at most %u", what, requests, WGD_REQUESTS_MAX);
+  if (!page || (page & (page - 1)) || page > WGD_PAGE_MAX) return fail(ctx, WGD_E_INVALID, "%s: pages of %u tokens; a power of two up to %u", what, page, WGD_PAGE_MAX);
+  if (!max_pages || !pages || (uint64_t)max_pages * page > 0x7FFFFFFFu || (uint64_t)pages * page > 0x7FFFFFFFu)
+    return fail(ctx, WGD_E_INVALID, "%s: %u pages, %u a request, of %u tokens", what, pages, max_pages, page);
+  return WGD_OK;
+}
+static uint32_t page_shift(uint32_t page) { return (uint32_t)__builtin_ctz(page); }
+// Written buffers are distinct, and none of those read.
+static bool apart(std::initializer_list<const wgd_buffer *> written, std::initializer_list<const wgd_buffer *> read) {
+  for (auto w = written.begin(); w != written.end(); ++w) {
+    if (std::find(w + 1, written.end(), *w) != written.end()) return false;
+    if (std::find(read.begin(), read.end(), *w) != read.end()) return false;
+  }
+  return true;
+}
+#define NEED_APART(ctx, what, written, read) do { if (!apart(written, read)) return fail(ctx, WGD_E_INVALID, "%s: what is written needs buffers of its own", what); } while (0)
+#define SET(...) {__VA_ARGS__}
+
+int wgd_pages_extend(wgd_context *ctx, wgd_buffer *table, wgd_buffer *lengths, wgd_buffer *refs, const wgd_buffer *counts,
+                     wgd_buffer *added, wgd_buffer *positions, wgd_buffer *slots, uint32_t requests, uint32_t tokens,
+                     uint32_t page, uint32_t max_pages, uint32_t pages) {
+  const char *what = "pages_extend";
+  NEED_CTX(ctx);
+  for (const wgd_buffer *b : {table, lengths, refs, added, positions, slots}) NEED_BUF(ctx, b, what);
+  if (counts) NEED_BUF(ctx, counts, what);
+  int rc = pages_shape(ctx, what, requests, page, max_pages, pages);
+  if (rc) return rc;
+  if (!tokens || (uint64_t)requests * tokens > (1u << 24))
+    return fail(ctx, WGD_E_INVALID, "%s: %u tokens for each of %u requests; 1 to 2^24 together", what, tokens, requests);
+  NEED_APART(ctx, what, SET(table, lengths, refs, added, positions, slots), SET(counts));
+  NEED_FIT(ctx, table, (uint64_t)requests * max_pages * 4, "page table");
+  NEED_FIT(ctx, lengths, (uint64_t)requests * 4, "lengths");
+  NEED_FIT(ctx, refs, (uint64_t)pages * 4, "page counts");
+  if (counts) NEED_FIT(ctx, counts, (uint64_t)requests * 4, "counts of new tokens");
+  NEED_FIT(ctx, added, (uint64_t)requests * 4, "added tokens");
+  NEED_FIT(ctx, positions, (uint64_t)requests * tokens * 4, "positions");
+  NEED_FIT(ctx, slots, (uint64_t)requests * tokens * 4, "slots");
+  PagesExtendArgs a{};
+  a.table = (int32_t *)table->ptr; a.lengths = (int32_t *)lengths->ptr; a.refs = (int32_t *)refs->ptr;
+  a.counts = counts ? (const int32_t *)counts->ptr : nullptr;
+  a.added = (int32_t *)added->ptr; a.positions = (int32_t *)positions->ptr; a.slots = (int32_t *)slots->ptr;
+  a.requests = requests; a.tokens = tokens; a.shift = page_shift(page); a.max_pages = max_pages; a.pages = pages;
+  return ctx_check(ctx, pages_extend(ctx->stream, a), what);
+}
+
+int wgd_pages_fork(wgd_context *ctx, wgd_buffer *table, wgd_buffer *lengths, wgd_buffer *refs, const wgd_buffer *origin,
+                   const wgd_buffer *keep, wgd_buffer *copies, uint32_t requests, uint32_t page, uint32_t max_pages,
+                   uint32_t pages) {
+  const char *what = "pages_fork";
+  NEED_CTX(ctx);
+  for (const wgd_buffer *b : {(const wgd_buffer *)table, (const wgd_buffer *)lengths, (const wgd_buffer *)refs, origin, (const wgd_buffer *)copies}) NEED_BUF(ctx, b, what);
+  if (keep) NEED_BUF(ctx, keep, what);
+  int rc = pages_shape(ctx, what, requests, page, max_pages, pages);
+  if (rc) return rc;
+  NEED_APART(ctx, what, SET(table, lengths, refs, copies), SET(origin, keep));
+  NEED_FIT(ctx, table, (uint64_t)requests * max_pages * 4, "page table");
+  NEED_FIT(ctx, lengths, (uint64_t)requests * 4, "lengths");
+  NEED_FIT(ctx, refs, (uint64_t)pages * 4, "page counts");
+  NEED_FIT(ctx, origin, (uint64_t)requests * 4, "origins");
+  if (keep) NEED_FIT(ctx, keep, (uint64_t)requests * 4, "kept tokens");
+  NEED_FIT(ctx, copies, ((uint64_t)requests * 2 + 1) * 4, "page copies");
+  PagesForkArgs a{};
+  a.table = (int32_t *)table->ptr; a.lengths = (int32_t *)lengths->ptr; a.refs = (int32_t *)refs->ptr;
+  a.origin = (const int32_t *)origin->ptr; a.keep = keep ? (const int32_t *)keep->ptr : nullptr; a.copies = (int32_t *)copies->ptr;
+  a.requests = requests; a.shift = page_shift(page); a.max_pages = max_pages; a.pages = pages;
+  rc = tree_workspace(ctx, pages_fork_scratch_bytes(a), what, (void **)&a.rows);
+  if (rc) return rc;
+  return ctx_check(ctx, pages_fork(ctx->stream, a), what);
+}
+
+int wgd_pages_compact(wgd_context *ctx, const wgd_buffer *table, const wgd_buffer *refs, wgd_buffer *table_to,
+                      wgd_buffer *refs_to, wgd_buffer *moved, wgd_buffer *copies, uint32_t requests, uint32_t max_pages,
+                      uint32_t pages) {
+  const char *what = "pages_compact";
+  NEED_CTX(ctx);
+  for (const wgd_buffer *b : {table, refs, (const wgd_buffer *)table_to, (const wgd_buffer *)refs_to, (const wgd_buffer *)moved, (const wgd_buffer *)copies}) NEED_BUF(ctx, b, what);
+  int rc = pages_shape(ctx, what, requests, 1, max_pages, pages);
+  if (rc) return rc;
+  if (!apart({table_to, refs_to, moved, copies}, {}) || table_to == refs || refs_to == table || !apart({moved, copies}, {table, refs}))
+    return fail(ctx, WGD_E_INVALID, "%s: what is written needs buffers of its own", what);
+  NEED_FIT(ctx, table, (uint64_t)requests * max_pages * 4, "page table");
+  NEED_FIT(ctx, table_to, (uint64_t)requests * max_pages * 4, "page table");
+  NEED_FIT(ctx, refs, (uint64_t)pages * 4, "page counts");
+  NEED_FIT(ctx, refs_to, (uint64_t)pages * 4, "page counts");
+  NEED_FIT(ctx, moved, (uint64_t)pages * 4, "moved pages");
+  NEED_FIT(ctx, copies, ((uint64_t)(pages / 2) * 2 + 1) * 4, "page copies");
+  PagesCompactArgs a{};
+  a.table = (const int32_t *)table->ptr; a.refs = (const int32_t *)refs->ptr; a.table_to = (int32_t *)table_to->ptr;
+  a.refs_to = (int32_t *)refs_to->ptr; a.moved = (int32_t *)moved->ptr; a.copies = (int32_t *)copies->ptr;
+  a.requests = requests; a.max_pages = max_pages; a.pages = pages;
+  return ctx_check(ctx, pages_compact(ctx->stream, a), what);
+}
+
+int wgd_pages_copy(wgd_context *ctx, wgd_buffer *const *pools, uint32_t count, const wgd_buffer *copies, uint32_t most,
+                   uint64_t page_bytes, uint32_t pages) {
+  NEED_CTX(ctx); NEED_BUF(ctx, copies, "pages_copy");
+  if (!pages || pages > 0x7FFFFFFFu || !page_bytes || page_bytes % 2 || page_bytes > (1u << 30) || most > (1u << 30))
+    return fail(ctx, WGD_E_INVALID, "pages_copy: %u of %u pages of %llu bytes", most, pages, (unsigned long long)page_bytes);
+  NEED_FIT(ctx, copies, ((uint64_t)most * 2 + 1) * 4, "page copies");
+  if (!count) return WGD_OK;
+  if (!pools || count > 65536) return fail(ctx, WGD_E_INVALID, pools ? "pages_copy: %u pools, at most 65536 in one call" : "pages_copy: NULL pools", count);
+  std::vector<void *> at(count);
+  for (uint32_t i = 0; i < count; i++) {
+    NEED_BUF(ctx, pools[i], "pages_copy");
+    NEED_FIT(ctx, pools[i], (uint64_t)pages * page_bytes, "pages_copy pool");
+    at[i] = pools[i]->ptr;
+  }
+  std::vector<void *> sorted = at;
+  sorted.push_back(copies->ptr);
+  std::sort(sorted.begin(), sorted.end());
+  if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+    return fail(ctx, WGD_E_INVALID, "pages_copy: a pool is given twice, or is the list of copies");
+  return ctx_check(ctx, pages_copy(ctx->stream, at.data(), count, (const int32_t *)copies->ptr, most, page_bytes, pages), "pages_copy");
+}
+
+static int pages_store_common(wgd_context *ctx, const char *what, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *k_pool,
+                              wgd_buffer *v_pool, const wgd_buffer *slots, uint32_t row, uint32_t rows, uint32_t stride,
+                              uint64_t k_offset, uint64_t v_offset, uint32_t slots_in_pool, bool kv16) {
+  NEED_CTX(ctx);
+  for (const wgd_buffer *b : {k, v, (const wgd_buffer *)k_pool, (const wgd_buffer *)v_pool, slots}) NEED_BUF(ctx, b, what);
+  if (!row || (stride && stride < row) || slots_in_pool > 0x7FFFFFFFu)
+    return fail(ctx, WGD_E_INVALID, "%s: rows of %u floats, %u apart, into %u slots", what, row, stride, slots_in_pool);
+  NEED_APART(ctx, what, SET(k_pool, v_pool), SET(k, v, slots));
+  if (!rows) return WGD_OK;
+  PagesStoreArgs a{};
+  a.row = row; a.rows = rows; a.stride = stride ? stride : row; a.slots_in_pool = slots_in_pool; a.kv16 = kv16;
+  const uint64_t floats = (uint64_t)(rows - 1) * a.stride + row;
+  if (k_offset > k->size / 4 || v_offset > v->size / 4) return fail(ctx, WGD_E_INVALID, "%s: offsets outside the rows' buffers", what);
+  NEED_FLOATS(ctx, k, k_offset, floats, "keys to store");
+  NEED_FLOATS(ctx, v, v_offset, floats, "values to store");
+  NEED_FIT(ctx, slots, (uint64_t)rows * 4, "slots");
+  if ((uint64_t)slots_in_pool * row > (kv16 ? k_pool->size / 2 : k_pool->size / 4) || (uint64_t)slots_in_pool * row > (kv16 ? v_pool->size / 2 : v_pool->size / 4))
+    return fail(ctx, WGD_E_INVALID, "%s: %u slots of %u elements do not fit the pools", what, slots_in_pool, row);
+  a.k = (const float *)k->ptr + k_offset; a.v = (const float *)v->ptr + v_offset; a.k_pool = k_pool->ptr; a.v_pool = v_pool->ptr;
+  a.slots = (const int32_t *)slots->ptr;
+  return ctx_check(ctx, pages_store(ctx->stream, a), what);
+}
+
+int wgd_pages_store(wgd_context *ctx, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *k_pool, wgd_buffer *v_pool,
+                    const wgd_buffer *slots, uint32_t row, uint32_t rows, uint32_t stride, uint64_t k_offset,
+                    uint64_t v_offset, uint32_t slots_in_pool) {
+  return pages_store_common(ctx, "pages_store", k, v, k_pool, v_pool, slots, row, rows, stride, k_offset, v_offset, slots_in_pool, false);
+}
+
+int wgd_pages_store_f16kv(wgd_context *ctx, const wgd_buffer *k, const wgd_buffer *v, wgd_buffer *k_pool,
+                          wgd_buffer *v_pool, const wgd_buffer *slots, uint32_t row, uint32_t rows, uint32_t stride,
+                          uint64_t k_offset, uint64_t v_offset, uint32_t slots_in_pool) {
+  return pages_store_common(ctx, "pages_store_f16kv", k, v, k_pool, v_pool, slots, row, rows, stride, k_offset, v_offset, slots_in_pool, true);
+}
+
+static int attention_pages_common(wgd_context *ctx, const char *what, const wgd_buffer *q, const wgd_buffer *k, const wgd_buffer *v,
+                                  wgd_buffer *y, const wgd_buffer *table, const wgd_buffer *lengths, const wgd_buffer *counts,
+                                  uint32_t heads, uint32_t kv_heads, uint32_t hd, float scale, uint32_t window, uint32_t page,
+                                  uint32_t max_pages, uint32_t pages, uint32_t requests, uint32_t tokens, uint32_t shared,
+                                  uint32_t owner, bool kv16) {
+  NEED_CTX(ctx);
+  for (const wgd_buffer *b : {q, k, v, (const wgd_buffer *)y, table, lengths}) NEED_BUF(ctx, b, what);
+  if (counts) NEED_BUF(ctx, counts, what);
+  int rc = pages_shape(ctx, what, requests, page, max_pages, pages);
+  if (rc) return rc;
+  if (!kv_heads || !heads || heads % kv_heads || !hd || hd > 512 || !window || !tokens)
+    return fail(ctx, WGD_E_INVALID, "%s: invalid heads %u/%u, head_dim %u, window %u or tokens %u", what, heads, kv_heads, hd, window, tokens);
+  const uint64_t rows = (uint64_t)requests * tokens * heads;
+  if (heads > (1u << 20) || tokens > (1u << 20) || rows > (1u << 25) || (uint64_t)tokens * (heads / kv_heads) > (1u << 20))
+    return fail(ctx, WGD_E_INVALID, "%s: %u heads on %u for %u tokens of each of %u requests are more than a launch takes", what, heads, kv_heads, tokens, requests);
+  if (shared % page || shared / page > max_pages || (shared && owner >= requests))
+    return fail(ctx, WGD_E_INVALID, "%s: a prefix of %u tokens of request %u is no whole number of its pages", what, shared, owner);
+  if (!apart({y}, {q, k, v, table, lengths, counts})) return fail(ctx, WGD_E_INVALID, "%s: the output needs a buffer of its own", what);
+  if (!requests) return WGD_OK;
+  const uint64_t row = (uint64_t)kv_heads * hd, pool = (kv16 ? std::min(k->size, v->size) / 2 : std::min(k->size, v->size) / 4);
+  if ((uint64_t)pages * page > pool / row) return fail(ctx, WGD_E_INVALID, "%s: %u pages of %u tokens do not fit the pools", what, pages, page);
+  NEED_FIT(ctx, q, rows * hd * 4, "attention queries");
+  NEED_FIT(ctx, y, rows * hd * 4, "attention output");
+  NEED_FIT(ctx, table, (uint64_t)requests * max_pages * 4, "page table");
+  NEED_FIT(ctx, lengths, (uint64_t)requests * 4, "lengths");
+  if (counts) NEED_FIT(ctx, counts, (uint64_t)requests * 4, "counts of new tokens");
+  PagesAttnArgs a{};
+  a.q = (const float *)q->ptr; a.k = k->ptr; a.v = v->ptr; a.y = (float *)y->ptr; a.table = (const int32_t *)table->ptr;
+  a.lengths = (const int32_t *)lengths->ptr; a.counts = counts ? (const int32_t *)counts->ptr : nullptr;
+  a.heads = heads; a.kv_heads = kv_heads; a.hd = hd; a.window = window; a.shift = page_shift(page); a.max_pages = max_pages;
+  a.pages = pages; a.requests = requests; a.tokens = tokens; a.shared = shared; a.owner = owner; a.scale = scale; a.kv16 = kv16;
+  a.partial_floats = attention_pages_scratch_floats(a);
+  rc = tree_workspace(ctx, a.partial_floats * 4, what, (void **)&a.partial);
+  if (rc) return rc;
+  return ctx_check(ctx, attention_pages(ctx->stream, a), what);
+}
+
+int wgd_attention_pages(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k_pool, const wgd_buffer *v_pool,
+                        wgd_buffer *y, const wgd_buffer *table, const wgd_buffer *lengths, const wgd_buffer *counts,
+                        uint32_t heads, uint32_t kv_heads, uint32_t hd, float scale, uint32_t window, uint32_t page,
+                        uint32_t max_pages, uint32_t pages, uint32_t requests, uint32_t tokens, uint32_t shared,
+                        uint32_t owner) {
+  return attention_pages_common(ctx, "attention_pages", q, k_pool, v_pool, y, table, lengths, counts, heads, kv_heads, hd, scale,
+                                window, page, max_pages, pages, requests, tokens, shared, owner, false);
+}
+
+int wgd_attention_pages_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k_pool, const wgd_buffer *v_pool,
+                              wgd_buffer *y, const wgd_buffer *table, const wgd_buffer *lengths, const wgd_buffer *counts,
+                              uint32_t heads, uint32_t kv_heads, uint32_t hd, float scale, uint32_t window, uint32_t page,
+                              uint32_t max_pages, uint32_t pages, uint32_t requests, uint32_t tokens, uint32_t shared,
+                              uint32_t owner) {
+  return attention_pages_common(ctx, "attention_pages_f16kv", q, k_pool, v_pool, y, table, lengths, counts, heads, kv_heads, hd, scale,
+                                window, page, max_pages, pages, requests, tokens, shared, owner, true);
+}
+
+int wgd_adapters(wgd_context *ctx, int32_t type, const wgd_buffer *a, const wgd_buffer *b, const wgd_buffer *which,
+                 const wgd_buffer *scales, const wgd_buffer *x, wgd_buffer *y, uint32_t cols, uint32_t rows, uint32_t rank,
+                 uint32_t adapters_, uint32_t stride, uint32_t row_base, uint32_t batch) {
+  const char *what = "adapters";
+  NEED_CTX(ctx);
+  for (const wgd_buffer *p : {a, b, which, scales, x, (const wgd_buffer *)y}) NEED_BUF(ctx, p, what);
+  if (type != F32 && type != F16) return fail(ctx, WGD_E_INVALID, "%s: type %d; F32 and F16 are supported", what, type);
+  for (const wgd_buffer *p : {a, b})
+    if (p->layout != LAYOUT_GGUF || (p->type >= 0 && p->type != type)) return fail(ctx, WGD_E_INVALID, "%s: weights %s were uploaded as type %d", what, p->label.c_str(), p->type);
+  if (!cols || !rows || !rank || rank > 1024 || !adapters_ || adapters_ > 0x7FFFFFFFu || batch > (1u << 24))
+    return fail(ctx, WGD_E_INVALID, "%s: %u adapters of rank %u, %u x %u, for %u rows", what, adapters_, rank, rows, cols, batch);
+  if (batch > 1 && stride < (uint64_t)row_base + rows) return fail(ctx, WGD_E_INVALID, "%s: stride %u < rowBase + rows", what, stride);
+  if (!apart({y}, {a, b, which, scales, x})) return fail(ctx, WGD_E_INVALID, "%s: the output needs a buffer of its own", what);
+  if (!batch) return WGD_OK;
+  const uint64_t e = type == F16 ? 2 : 4;
+  if ((uint64_t)adapters_ * rank > a->size / e / cols || (uint64_t)adapters_ * rank > b->size / e / rows)
+    return fail(ctx, WGD_E_INVALID, "%s: %u adapters of rank %u do not fit the weights' buffers", what, adapters_, rank);
+  NEED_FIT(ctx, which, (uint64_t)batch * 4, "adapters of the rows");
+  NEED_FIT(ctx, scales, (uint64_t)adapters_ * 4, "scales of the adapters");
+  NEED_FIT(ctx, x, (uint64_t)batch * cols * 4, "adapters input");
+  NEED_FLOATS(ctx, y, 0, (uint64_t)(batch - 1) * stride + row_base + rows, "adapters output");
+  AdaptersArgs p{};
+  p.a = a->ptr; p.b = b->ptr; p.which = (const int32_t *)which->ptr; p.scales = (const float *)scales->ptr; p.x = (const float *)x->ptr;
+  p.y = (float *)y->ptr + row_base; p.cols = cols; p.rows = rows; p.rank = rank; p.adapters = adapters_; p.batch = batch; p.stride = stride;
+  p.half = type == F16;
+  int rc = tree_workspace(ctx, adapters_scratch_floats(p) * 4, what, (void **)&p.partial);
+  if (rc) return rc;
+  return ctx_check(ctx, adapters(ctx->stream, p), what);
 }
 
 int wgd_embed(wgd_context *ctx, int32_t type, const wgd_buffer *table, const wgd_buffer *ids, wgd_buffer *out,

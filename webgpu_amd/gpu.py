@@ -61,6 +61,15 @@ SIGNATURES = {
     "wgd_sample_rows": (C.c_int, [_P, _P, _U32, _U32, _U32, _P, _P, _D, _U32, _D, _D]),
     "wgd_tree_accept": (C.c_int, [_P, _P, _P, _P, _P, _U32]),
     "wgd_kv_commit": (C.c_int, [_P, _P, _U32, _P, _U64, _U32, _U32, _U32]),
+    "wgd_pages_extend": (C.c_int, [_P] * 8 + [_U32] * 5),
+    "wgd_pages_fork": (C.c_int, [_P] * 7 + [_U32] * 4),
+    "wgd_pages_compact": (C.c_int, [_P] * 7 + [_U32] * 3),
+    "wgd_pages_copy": (C.c_int, [_P, _P, _U32, _P, _U32, _U64, _U32]),
+    "wgd_pages_store": (C.c_int, [_P] * 6 + [_U32, _U32, _U32, _U64, _U64, _U32]),
+    "wgd_pages_store_f16kv": (C.c_int, [_P] * 6 + [_U32, _U32, _U32, _U64, _U64, _U32]),
+    "wgd_attention_pages": (C.c_int, [_P] * 8 + [_U32, _U32, _U32, _F] + [_U32] * 8),
+    "wgd_attention_pages_f16kv": (C.c_int, [_P] * 8 + [_U32, _U32, _U32, _F] + [_U32] * 8),
+    "wgd_adapters": (C.c_int, [_P, _I32] + [_P] * 6 + [_U32] * 7),
     "wgd_probe_read": (C.c_int, [_P, _P, _U64, _U32, _U32, _U32, _U32, _U32, _P, _U32]),
     "wgd_add": (C.c_int, [_P, _P, _P, _U32]),
     "wgd_silu": (C.c_int, [_P, _P, _P, _P, _U32]),
@@ -359,6 +368,68 @@ class Compute:
         """Moves the path's rows of every ring (K and V of any layers) to the slots they keep."""
         ptrs = array("Q", [r.ptr for r in rings])
         self.check(lib().wgd_kv_commit(self.ctx, ptrs.buffer_info()[0], len(ptrs), path.ptr, row_bytes, start, capacity, nodes))
+
+    # -- many requests (include/wgd.h) -------------------------------------------------
+    def pages_extend(self, table: Buffer, lengths: Buffer, refs: Buffer, added: Buffer, positions: Buffer, slots: Buffer,
+                     requests: int, tokens: int, page: int, max_pages: int, pages: int,
+                     counts: Optional[Buffer] = None) -> None:
+        """Places for counts[r] (``tokens`` without) new tokens of every request, with their positions and slots."""
+        self.check(lib().wgd_pages_extend(self.ctx, table.ptr, lengths.ptr, refs.ptr, counts.ptr if counts is not None else None,
+                                          added.ptr, positions.ptr, slots.ptr, requests, tokens, page, max_pages, pages))
+
+    def pages_fork(self, table: Buffer, lengths: Buffer, refs: Buffer, origin: Buffer, copies: Buffer, requests: int, page: int,
+                   max_pages: int, pages: int, keep: Optional[Buffer] = None) -> None:
+        """Request r becomes the first keep[r] tokens (all without) of what request origin[r] was, empty for -1;
+        the pages that this asks to be copied go to ``copies`` (for ``pages_copy``)."""
+        self.check(lib().wgd_pages_fork(self.ctx, table.ptr, lengths.ptr, refs.ptr, origin.ptr, keep.ptr if keep is not None else None,
+                                        copies.ptr, requests, page, max_pages, pages))
+
+    def pages_compact(self, table: Buffer, refs: Buffer, table_to: Buffer, refs_to: Buffer, moved: Buffer, copies: Buffer,
+                      requests: int, max_pages: int, pages: int) -> None:
+        """Numbers the used pages 0 .. n: the table and counts afterwards, every page's new number and the copies."""
+        self.check(lib().wgd_pages_compact(self.ctx, table.ptr, refs.ptr, table_to.ptr, refs_to.ptr, moved.ptr, copies.ptr, requests,
+                                           max_pages, pages))
+
+    def pages_copy(self, pools, copies: Buffer, most: int, page_bytes: int, pages: int) -> None:
+        """Carries out ``copies`` (at most ``most``) in every pool."""
+        ptrs = array("Q", [p.ptr for p in pools])
+        self.check(lib().wgd_pages_copy(self.ctx, ptrs.buffer_info()[0], len(ptrs), copies.ptr, most, page_bytes, pages))
+
+    def pages_store(self, k: Buffer, v: Buffer, k_pool: Buffer, v_pool: Buffer, slots: Buffer, row: int, rows: int,
+                    slots_in_pool: int, stride: int = 0, k_offset: int = 0, v_offset: int = 0) -> None:
+        """K and V rows of new tokens into their slots of f32 pools."""
+        self.check(lib().wgd_pages_store(self.ctx, k.ptr, v.ptr, k_pool.ptr, v_pool.ptr, slots.ptr, row, rows, stride, k_offset,
+                                         v_offset, slots_in_pool))
+
+    def pages_store_f16kv(self, k: Buffer, v: Buffer, k_pool: Buffer, v_pool: Buffer, slots: Buffer, row: int, rows: int,
+                          slots_in_pool: int, stride: int = 0, k_offset: int = 0, v_offset: int = 0) -> None:
+        """pages_store() into pools of f16 elements, rounded to nearest even."""
+        self.check(lib().wgd_pages_store_f16kv(self.ctx, k.ptr, v.ptr, k_pool.ptr, v_pool.ptr, slots.ptr, row, rows, stride, k_offset,
+                                               v_offset, slots_in_pool))
+
+    def attention_pages(self, q: Buffer, k_pool: Buffer, v_pool: Buffer, y: Buffer, table: Buffer, lengths: Buffer, heads: int,
+                        kv_heads: int, hd: int, scale: float, window: int, page: int, max_pages: int, pages: int, requests: int,
+                        tokens: int = 1, counts: Optional[Buffer] = None, shared: int = 0, owner: int = 0) -> None:
+        """Attention of the newest tokens of every request over its pages; a prefix of ``shared`` tokens of request ``owner`` is
+        computed once for all that hold it."""
+        self.check(lib().wgd_attention_pages(self.ctx, q.ptr, k_pool.ptr, v_pool.ptr, y.ptr, table.ptr, lengths.ptr,
+                                             counts.ptr if counts is not None else None, heads, kv_heads, hd, scale, window, page,
+                                             max_pages, pages, requests, tokens, shared, owner))
+
+    def attention_pages_f16kv(self, q: Buffer, k_pool: Buffer, v_pool: Buffer, y: Buffer, table: Buffer, lengths: Buffer,
+                              heads: int, kv_heads: int, hd: int, scale: float, window: int, page: int, max_pages: int, pages: int,
+                              requests: int, tokens: int = 1, counts: Optional[Buffer] = None, shared: int = 0,
+                              owner: int = 0) -> None:
+        """attention_pages() over pools of f16 elements."""
+        self.check(lib().wgd_attention_pages_f16kv(self.ctx, q.ptr, k_pool.ptr, v_pool.ptr, y.ptr, table.ptr, lengths.ptr,
+                                                   counts.ptr if counts is not None else None, heads, kv_heads, hd, scale, window,
+                                                   page, max_pages, pages, requests, tokens, shared, owner))
+
+    def adapters(self, type_: int, a: Buffer, b: Buffer, which: Buffer, scales: Buffer, x: Buffer, y: Buffer, cols: int, rows: int,
+                 rank: int, adapters: int, stride: int, row_base: int, batch: int = 1) -> None:
+        """y[t] += scales[w] B[w] (A[w] x[t]) for every row t with an adapter w = which[t]."""
+        self.check(lib().wgd_adapters(self.ctx, type_, a.ptr, b.ptr, which.ptr, scales.ptr, x.ptr, y.ptr, cols, rows, rank, adapters,
+                                      stride, row_base, batch))
 
     def embed(self, type_: int, table: Buffer, ids: Buffer, out: Buffer, hidden: int, n: int, scale: float = 1.0) -> None:
         self.check(lib().wgd_embed(self.ctx, type_, table.ptr, ids.ptr, out.ptr, hidden, n, scale))
