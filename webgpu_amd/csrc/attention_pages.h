@@ -4,8 +4,8 @@
 // most `tokens`) with a query each: query t has the position p = lengths[r] - n_r + t and sees the keys (p - window, p]:
 //   y = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m),  s_k = scale q . k_k,  m = max s_k.
 // The lengths are on the device, so the work is shared out there: every wavefront forms the same plan from them.
-// A request's keys are cut into chunks of the same length for all, about `target` of them together; a workgroup has one
-// chunk, one kv head and some of the rows, the (query, head of the group) pairs that share the head's keys.
+// The keys of the requests are cut into about `target` chunks of similar length; a workgroup has one chunk, one kv head and
+// some of the rows, the (query, head of the group) pairs that share the head's keys.
 // Requests whose first `shared` tokens are the owner's have these computed together: the rows of all of them
 // against the owner's keys, in `nprefix` parts. The parts of a row meet in k_pages_join, as (max, sum, weighted values).
 #pragma once
@@ -17,7 +17,6 @@ struct PagesK {
   uint32_t heads, kvh, group, hd, window, shift, max_pages, pages, requests, tokens, shared, owner;
   uint32_t unit, least, target, slots;  // keys of a unit; least units of a chunk; chunks wanted, and at most
   uint32_t nprefix, per;                // parts of the prefix, keys of each
-  uint32_t blocks;                      // row blocks of a request (of all of them, in the prefix)
   float scale;
 };
 
@@ -37,6 +36,7 @@ __device__ __forceinline__ PagesRequest pages_request(const PagesK &a, uint32_t 
   q.n = min(q.len, a.counts ? (uint32_t)min(max(a.counts[r], 0), (int32_t)a.tokens) : a.tokens);
   const uint32_t first = q.len - q.n + 1;  // keys up to the first query's own
   q.lo = first > a.window ? first - a.window : 0;
+  if (a.shift >= 4) q.lo &= ~15u;  // whole halves of blocks, on the same page; nothing before the first key is read
   if (a.shared) {
     const uint32_t c = (a.shared >> a.shift) - 1;
     const bool owned = min((uint32_t)max(a.lengths[a.owner], 0), a.max_pages << a.shift) >= a.shared;
@@ -104,7 +104,7 @@ __device__ __forceinline__ PagesChunks pages_chunks(const PagesK &a, const Pages
 // A workgroup's part of the work: rows of kv head kv against the keys [lo, hi) of one row of the table. Row i of the part is
 // (request, query, head): of one request, or of those that share the prefix (`list`, in LDS).
 struct PagesPart {
-  uint32_t kv, row0, nrows, lo, hi;
+  uint32_t kv, row0, nrows, lo, hi, seen;  // seen: the first key that a row sees, if that lies behind lo
   uint32_t r, n, end0;       // own chunks: the request, its queries, lengths - n + 1 (what query 0 sees of it)
   const int32_t *table;
   const uint16_t *list;      // the prefix: null otherwise
@@ -270,7 +270,7 @@ __device__ __forceinline__ bool pages_part(const PagesK &a, uint32_t rows, uint1
     p.nrows = n * a.tokens * a.group;
     p.lo = min(blockIdx.y * a.per, a.shared);
     p.hi = min(p.lo + a.per, a.shared);
-    p.r = a.owner; p.n = a.tokens; p.end0 = 0;
+    p.r = a.owner; p.n = a.tokens; p.end0 = 0; p.seen = 0;
     p.table = a.table + (uint64_t)a.owner * a.max_pages;
     p.list = list;
     p.direct = false;
@@ -281,11 +281,12 @@ __device__ __forceinline__ bool pages_part(const PagesK &a, uint32_t rows, uint1
   } else {
     const PagesChunks c = pages_chunks<false>(a, plan, blockIdx.y);
     if (c.r == 0xFFFFFFFFu) return false;
-    const uint32_t at = blockIdx.y - c.first, keys = plan.chunk * a.unit;  // (chunks behind the first have keys: at * keys < len)
+    const uint32_t at = blockIdx.y - c.first, units = c.n ? (c.len - c.lo + a.unit - 1) / a.unit : 0;  // no fewer than chunks, or 0
     p.nrows = c.n * a.group;
-    p.lo = c.lo + at * keys;
-    p.hi = c.len - p.lo < keys ? c.len : p.lo + keys;
+    p.lo = c.lo + (uint32_t)((uint64_t)units * at / c.count) * a.unit;
+    p.hi = at + 1 == c.count ? c.len : c.lo + (uint32_t)((uint64_t)units * (at + 1) / c.count) * a.unit;
     p.r = c.r; p.n = c.n; p.end0 = c.len - c.n + 1;
+    p.seen = p.end0 > a.window ? p.end0 - a.window : 0;
     p.table = a.table + (uint64_t)c.r * a.max_pages;
     p.list = nullptr;
     p.direct = c.count == 1 && !c.shares;
@@ -307,6 +308,285 @@ __global__ __launch_bounds__(256) void k_pages_any(PagesK a, uint32_t T) {
   PagesPart p;
   if (!pages_part<PREFIX, 256>(a, TREE_R, list, p)) return;
   pages_any<E, 256>(a, lds, T, p, p.row0);
+}
+
+// ------------------------------------------------------------------ head dims up to 256, multiples of 8
+//
+// The page numbers of a workgroup's keys lie in LDS, PAGES_IDS at a time; blocks of keys go from the pages straight into matrix
+// operands, as those of k_attn_tree do from a ring, each wavefront with its tile of 16 rows and every slices-th block. Pages
+// of 16 tokens or more have the 16 keys of a half block one behind the other (all ranges begin at a multiple of 16 there): one
+// number, a scalar, for the lot.
+// A masked key's weight is exactly 0, but 0 times what is not finite is NaN, and the split operands turn infinities into it: a workgroup that
+// ends with anything not finite, or that has a page that is none, forms its rows again with pages_any.
+constexpr uint32_t PAGES_IDS = 1024;
+
+// Which of the keys t0 .. + 32 (below hi) a row sees, as bits.
+__device__ __forceinline__ uint32_t pages_mask(uint32_t begin, uint32_t end, uint32_t t0) {
+  auto below = [&](uint32_t t) { return t <= t0 ? 0u : t - t0 >= 32 ? ~0u : (1u << (t - t0)) - 1; };
+  return below(end) & ~below(begin);
+}
+
+// The numbers of the pages of [k0, k1) into ids; true in all threads if one of them is none.
+template <uint32_t NT>
+__device__ __forceinline__ bool pages_ids(const PagesK &a, const PagesPart &p, uint32_t *ids, uint32_t k0, uint32_t k1) {
+  const uint32_t first = k0 >> a.shift, n = ((k1 - 1) >> a.shift) + 1 - first;
+  bool none = false;
+  for (uint32_t i = threadIdx.x; i < n; i += NT) {
+    const int32_t id = p.table[first + i];
+    const bool ok = id >= 0 && (uint32_t)id < a.pages;
+    none |= !ok;
+    ids[i] = ok ? (uint32_t)id : 0;
+  }
+  return __syncthreads_or(none);
+}
+
+template <uint32_t HD, class E, bool FULL>
+struct PagesWave : TreeWave<HD, E, FULL> {
+  typedef TreeWave<HD, E, FULL> Wave;
+  using Wave::NB, Wave::KT, Wave::VK, Wave::KEYS, Wave::NX, Wave::k, Wave::v, Wave::rowb, Wave::hi, Wave::k_piece, Wave::v_piece, Wave::k_row,
+      Wave::v_row, Wave::kr;
+  typedef typename Wave::vpiece vpiece;
+  const uint32_t *ids;  // from page `first` on
+  uint32_t first, shift, seen;
+
+  __device__ __forceinline__ uint64_t at(uint32_t t) const {  // of one key, the nearest of [seen, hi)
+    t = min(max(t, seen), hi - 1);
+    return (((uint64_t)ids[(t >> shift) - first] << shift) + (t & ((1u << shift) - 1))) * rowb;
+  }
+  __device__ __forceinline__ uint64_t half(uint32_t t) const {  // of 16 keys side by side
+    const uint32_t id = __builtin_amdgcn_readfirstlane(ids[(t >> shift) - first]);
+    return (((uint64_t)id << shift) + (t & ((1u << shift) - 1))) * rowb;
+  }
+  __device__ __forceinline__ bool whole(uint32_t t) const { return shift >= 4 && t >= seen && t + KEYS <= hi; }
+  __device__ __forceinline__ void load_k(uint32_t t) {
+    const uint32_t c = threadIdx.x & 15;
+    if (whole(t)) {
+#pragma unroll
+      for (uint32_t b = 0; b < NB; b++) {
+        const uint8_t *row = k + half(t + 16 * b);
+#pragma unroll
+        for (uint32_t u = 0; u < KT; u++) kr[b][u] = *(const u32x4 *)(row + (k_row + k_piece[u]));
+      }
+    } else {
+#pragma unroll
+      for (uint32_t b = 0; b < NB; b++) {
+        const uint8_t *row = k + at(t + 16 * b + c);
+#pragma unroll
+        for (uint32_t u = 0; u < KT; u++) kr[b][u] = *(const u32x4 *)(row + k_piece[u]);
+      }
+    }
+  }
+  // Keys [t0, hi) in steps of `step`; the row sees [begin, end), all rows of the wavefront [all_begin, all_end).
+  __device__ __forceinline__ void walk(uint32_t t0, uint32_t step, uint32_t begin, uint32_t end, uint32_t all_begin, uint32_t all_end) {
+    const uint32_t g = (threadIdx.x & 63) >> 4;
+    if (t0 < hi) load_k(t0);
+    for (; t0 < hi; t0 += step) {
+      vpiece vr[VK][NX];
+      if (whole(t0)) {
+#pragma unroll
+        for (uint32_t b = 0; b < NB; b++) {
+          const uint8_t *rows = v + half(t0 + 16 * b);
+#pragma unroll
+          for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+            for (uint32_t x = 0; x < NX; x++) vr[4 * b + j][x] = *(const vpiece *)(rows + j * rowb + (v_row + v_piece[x]));
+        }
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < VK; j++) {
+          const uint8_t *row = v + at(t0 + 16 * (j / 4) + 4 * g + j % 4);
+#pragma unroll
+          for (uint32_t x = 0; x < NX; x++) vr[j][x] = *(const vpiece *)(row + v_piece[x]);
+        }
+      }
+      f32x4 s[NB];
+      this->scores(s);
+      if (t0 + step < hi) load_k(t0 + step);
+      const bool masked = t0 + KEYS > min(hi, all_end) || t0 < all_begin;
+      this->weigh(0, s, this->qs, masked, masked ? pages_mask(begin, min(end, hi), t0) : 0);
+      this->values(vr, s);
+    }
+  }
+};
+
+// The end of a workgroup: the slices of its wavefronts merge in LDS, and the rows go to y or to their parts. wave w has the rows row0 + (w % rw) *
+// 16 RT .. and the slice w / rw. With anything not finite, or `again`, the rows are formed again.
+template <uint32_t HD, class E, uint32_t RT, uint32_t NT, class Rows>
+__device__ __forceinline__ void pages_end(const PagesK &a, uint32_t rw, float *lds, const PagesPart &p, const Rows &s, bool again) {
+  constexpr uint32_t VE = Rows::VE, NX = Rows::NX, OS = HD + 4, WS = RT * 16 * (OS + 2);
+  const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15, slices = NT / 64 / rw;
+  if (__syncthreads_or(again || !s.finite())) {
+    for (uint32_t i = 0; i < rw * RT; i++)
+      if (p.row0 + 16 * i < p.nrows) pages_any<E, NT>(a, lds, tree_any_tile(HD), p, p.row0 + 16 * i);
+    return;
+  }
+  // ---- to LDS: [row] max, sum; [row][HD]
+  float *mine = lds + (tid >> 6) * WS;
+#pragma unroll
+  for (uint32_t rt = 0; rt < RT; rt++) {
+    float l = s.l[rt];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) { mine[2 * (16 * rt + c)] = s.m[rt]; mine[2 * (16 * rt + c) + 1] = l; }
+    float *row = mine + RT * 32 + (16 * rt + c) * OS;
+#pragma unroll
+    for (uint32_t x = 0; x < NX; x++) {
+      if constexpr (VE == 1) {
+        *(f32x4 *)(row + 16 * x + 4 * g) = s.o[rt][x][0];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (uint32_t e = 0; e < VE; e += 4)
+            *(f32x4 *)(row + 16 * VE * x + 4 * VE * g + VE * r + e) =
+                f32x4{s.o[rt][x][e][r], s.o[rt][x][e + 1][r], s.o[rt][x][e + 2][r], s.o[rt][x][e + 3][r]};
+      }
+    }
+  }
+  __syncthreads();
+  // ---- the slices in order, eight dims of a row per thread
+  const uint64_t pairs = pages_pairs(pages_part_rows(a.slots, a.nprefix, a.requests, (uint64_t)a.tokens * a.heads), a.hd);
+  for (uint32_t i = tid; i < rw * RT * 16 * (HD / 8); i += NT) {
+    const uint32_t d = i % (HD / 8) * 8, lr = i / (HD / 8) % (RT * 16), rg = i / (HD / 8) / (RT * 16);
+    const PagesRow w = pages_row(a, p, p.row0 + rg * RT * 16 + lr);
+    if (!w.valid || d >= a.hd) continue;
+    float M = -INFINITY, l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (uint32_t u = 0; u < slices; u++) M = fmaxf(M, lds[(u * rw + rg) * WS + 2 * lr]);
+    for (uint32_t u = 0; u < slices; u++) {
+      const float *at = lds + (u * rw + rg) * WS;
+      if (at[2 * lr + 1] == 0.f) continue;  // nothing seen
+      const float f = at[2 * lr] == M ? 1.f : __builtin_amdgcn_exp2f(at[2 * lr] - M);
+      l += at[2 * lr + 1] * f;
+      const f32x4 x0 = *(const f32x4 *)(at + RT * 32 + lr * OS + d), x1 = *(const f32x4 *)(at + RT * 32 + lr * OS + d + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) { y[e] += x0[e] * f; y[4 + e] += x1[e] * f; }
+    }
+    float *to = a.y + w.row * a.hd + d, inv = 1.f;
+    if (p.direct) {
+      inv = 1.f / l;  // (a row sees its own key at least)
+    } else {
+      const uint64_t at = pages_at(a, p, w);
+      to = a.part + at * a.hd + d;
+      if (d == 0) *(float2 *)(a.part + pairs + 2 * at) = make_float2(M - TREE_BIAS, w.begin < p.hi && w.end > p.lo ? l : -1.f);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) *(f32x4 *)(to + e) = f32x4{y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv};
+  }
+}
+
+// What a lane's row sees, and all rows of its wavefront.
+struct PagesSees { uint32_t begin, end, all_begin, all_end; };
+__device__ __forceinline__ PagesSees pages_sees(const PagesRow &w) {
+  PagesSees s = {w.valid ? w.begin : 0u, w.valid ? w.end : 0u, w.valid ? w.begin : 0u, w.valid ? w.end : ~0u};
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    s.all_begin = max(s.all_begin, (uint32_t)__shfl_xor((int)s.all_begin, o, 64));
+    s.all_end = min(s.all_end, (uint32_t)__shfl_xor((int)s.all_end, o, 64));
+  }
+  s.all_begin = __builtin_amdgcn_readfirstlane(s.all_begin);
+  s.all_end = __builtin_amdgcn_readfirstlane(s.all_end);
+  return s;
+}
+
+template <uint32_t HD, class E, bool FULL, bool PREFIX>
+__global__ __launch_bounds__((tree_threads<HD>())) void k_pages(PagesK a, uint32_t rw) {
+  constexpr uint32_t NT = tree_threads<HD>();
+  typedef PagesWave<HD, E, FULL> Wave;
+  extern __shared__ float lds[];
+  __shared__ uint16_t list[PREFIX ? WGD_REQUESTS_MAX : 1];
+  __shared__ uint32_t ids[PAGES_IDS];
+  PagesPart p;
+  if (!pages_part<PREFIX, NT>(a, 16 * rw, list, p)) return;
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = w / rw, wrow = p.row0 + w % rw * 16;
+  const PagesRow row = pages_row(a, p, wrow + (threadIdx.x & 15));
+  const PagesSees sees = pages_sees(row);
+  Wave s;
+  s.place(a.k, a.v, a.kvh, a.hd, p.kv);
+  s.load_q(a.scale, a.hd, a.q + row.row * a.hd, row.valid);
+  s.clear();
+  s.ids = ids; s.shift = a.shift; s.seen = p.seen;
+  bool none = false;
+  for (uint32_t k0 = p.lo; k0 < p.hi && !none; k0 = s.hi) {
+    s.first = k0 >> a.shift;
+    s.hi = min((uint64_t)p.hi, (uint64_t)(s.first + PAGES_IDS) << a.shift);
+    if (k0 > p.lo) __syncthreads();
+    none = pages_ids<NT>(a, p, ids, k0, s.hi);
+    if (!none && wrow < p.nrows) s.walk(k0 + slice * Wave::KEYS, NT / 64 / rw * Wave::KEYS, sees.begin, sees.end, sees.all_begin, sees.all_end);
+  }
+  pages_end<HD, E, 1, NT>(a, rw, lds, p, s, none);
+}
+
+// ------------------------------------------------------------------ many rows over halves: keys staged in LDS
+// As k_attn_tree_staged: eight wavefronts load stages of SK keys into LDS while they work on the one before.
+template <uint32_t HD, uint32_t RT, uint32_t SK, bool PREFIX>
+__global__ __launch_bounds__(TREE_STAGED_NT) void k_pages_staged(PagesK a, uint32_t rw) {
+  typedef TreeStaged<HD, RT> Wave;
+  constexpr uint32_t ROW = Wave::ROW, CH = Wave::CH, NT = TREE_STAGED_NT, STEP = NT / CH;
+  extern __shared__ float lds[];
+  __shared__ uint16_t list[PREFIX ? WGD_REQUESTS_MAX : 1];
+  __shared__ uint32_t ids[PAGES_IDS];
+  PagesPart p;
+  if (!pages_part<PREFIX, NT>(a, 16 * RT * rw, list, p)) return;
+  const uint32_t tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), slice = w / rw, slices = NT / 64 / rw;
+  const uint32_t wrow = p.row0 + w % rw * 16 * RT, pg = (1u << a.shift) - 1;
+  uint8_t *stages = (uint8_t *)lds;
+  const uint64_t rowb = (uint64_t)a.kvh * ROW, head = (uint64_t)p.kv * ROW;
+  const uint8_t *k = (const uint8_t *)a.k + head, *v = (const uint8_t *)a.v + head;
+  const uint32_t key0 = tid / CH, k_place = (tid % CH ^ Wave::k_swizzle(key0)) * 16, v_place = (tid % CH ^ Wave::v_swizzle(key0)) * 16;
+  static_assert(STEP % 16 == 0, "the swizzles repeat after 16 keys");
+  uint32_t first = 0, hi = 0;
+  auto load = [&](uint32_t t0, uint32_t s) {
+    uint8_t *K = stages + s * 2 * SK * ROW + 1024 * w, *V = K + SK * ROW;
+    auto put = [](const uint8_t *from, uint8_t *to) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+    };
+    uint64_t at[SK / STEP];
+#pragma unroll
+    for (uint32_t n = 0; n < SK / STEP; n++) {
+      const uint32_t t = min(max(t0 + key0 + n * STEP, p.seen), hi - 1);
+      at[n] = (((uint64_t)ids[(t >> a.shift) - first] << a.shift) + (t & pg)) * rowb;
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < SK / STEP; n++) {
+      put(k + at[n] + k_place, K + n * STEP * ROW);
+      put(v + at[n] + v_place, V + n * STEP * ROW);
+    }
+  };
+  PagesSees sees[RT];
+  Wave s;
+  s.clear();
+#pragma unroll
+  for (uint32_t rt = 0; rt < RT; rt++) {
+    const PagesRow row = pages_row(a, p, wrow + 16 * rt + (tid & 15));
+    sees[rt] = pages_sees(row);
+    s.qs[rt] = tree_query<Wave::KT>(a.q + row.row * HD, HD, a.scale * TREE_LOG2E, row.valid, s.qh[rt], s.ql[rt]);
+  }
+  uint32_t all_begin = 0, all_end = ~0u;
+#pragma unroll
+  for (uint32_t rt = 0; rt < RT; rt++) { all_begin = max(all_begin, sees[rt].all_begin); all_end = min(all_end, sees[rt].all_end); }
+  bool none = false;
+  for (uint32_t k0 = p.lo; k0 < p.hi && !none; k0 = hi) {
+    if (k0 > p.lo) __syncthreads();  // the numbers and both stages are no longer read
+    first = k0 >> a.shift;
+    hi = min((uint64_t)p.hi, (uint64_t)(first + PAGES_IDS) << a.shift);
+    none = pages_ids<NT>(a, p, ids, k0, hi);
+    if (none) break;
+    load(k0, 0);
+    uint32_t stage = 0;
+    for (uint32_t t0 = k0; t0 < hi; t0 += SK, stage ^= 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's loads into the stage
+      __syncthreads();                                   // everyone's; and the other stage is no longer read
+      if (t0 + SK < hi) load(t0 + SK, stage ^ 1);
+      const uint8_t *K = stages + stage * 2 * SK * ROW, *V = K + SK * ROW;
+      if (wrow < p.nrows)
+        for (uint32_t b = slice; b < SK / 32 && t0 + 32 * b < hi; b += slices) {
+          const uint32_t t = t0 + 32 * b;
+          s.block(K + 32 * b * ROW, V + 32 * b * ROW, t + 32 > min(hi, all_end) || t < all_begin,
+                  [&](uint32_t rt) { return pages_mask(sees[rt].begin, min(sees[rt].end, hi), t); });
+        }
+    }
+  }
+  pages_end<HD, _Float16, RT, NT>(a, rw, lds, p, s, none);
 }
 
 // ------------------------------------------------------------------ the parts of a row
@@ -351,24 +631,46 @@ __global__ __launch_bounds__(256) void k_pages_join(PagesK a) {
   }
 }
 
-struct PagesLaunch { uint32_t T, rows, blocks, pblocks, unit, least, target, slots, nprefix, per; };
+// The kernels of a call. mfma: matrix products; HD: the head dim padded to 64, 128 or 256; rows: of a workgroup, blocks and pblocks how
+// many that makes of a request and of all of them together.
+struct PagesLaunch { bool mfma, staged, pstaged; uint32_t HD, T, rw, prw, rows, prows, blocks, pblocks, unit, least, target, slots, nprefix, per; };
 static PagesLaunch pages_launch(const PagesAttnArgs &in) {
   PagesLaunch p{};
-  const uint32_t group = in.heads / in.kv_heads, cus = (uint32_t)device_cu_count();
+  const uint32_t group = in.heads / in.kv_heads, cus = (uint32_t)device_cu_count(), nrows = in.tokens * group;
+  const uint64_t longest = (uint64_t)in.max_pages << in.shift, prows = (uint64_t)in.requests * nrows;
+  // (a lane's offsets within 16 rows of a page are 32-bit)
+  p.mfma = in.hd % 8 == 0 && in.hd <= 256 && (uint64_t)in.kv_heads * in.hd * 4 < (1u << 27);
+  p.HD = in.hd <= 64 ? 64 : in.hd <= 128 ? 128 : 256;
+  const bool can_stage = p.mfma && in.kv16 && in.hd == p.HD;
+  auto shape = [&](uint64_t n, bool &staged, uint32_t &rw, uint32_t &rows) {
+    if (!p.mfma) { rows = TREE_R; rw = 1; return; }
+    const uint64_t tiles = (n + 15) / 16;
+    staged = can_stage && tiles >= 8;
+    const uint32_t RT = staged && p.HD <= 128 ? 2 : 1;
+    const uint64_t groups = (tiles + RT - 1) / RT;
+    rw = groups >= 4 ? 4 : groups >= 2 ? 2 : 1;
+    rows = 16 * RT * rw;
+  };
+  shape(nrows, p.staged, p.rw, p.rows);
+  p.blocks = (nrows + p.rows - 1) / p.rows;
+  const uint32_t waves = p.staged || p.HD <= 128 ? 8 : 4;
   p.T = tree_any_tile(in.hd);
-  p.rows = TREE_R;
-  p.unit = p.T; p.least = 4;
-  p.blocks = (in.tokens * group + p.rows - 1) / p.rows;
-  const uint64_t longest = (uint64_t)in.max_pages << in.shift;
+  p.unit = !p.mfma ? p.T : (in.kv16 ? 32 : 16) * (waves / p.rw);
+  if (p.staged) p.unit = std::max(p.unit, 128u);
+  p.least = p.mfma ? 2 : 4;
   const uint32_t wgs = in.kv_heads * p.blocks;
-  p.target = std::max(1u, std::min(4 * cus / std::max(1u, wgs), PAGES_TARGET));
+  p.target = std::max(1u, std::min((p.mfma ? 2 : 4) * cus / std::max(1u, wgs), PAGES_TARGET));
   // no request is cut where the longest is one chunk
   const uint64_t chunks = std::min<uint64_t>(p.target, (uint64_t)in.requests * ((longest + p.unit * p.least - 1) / (p.unit * p.least)));
   p.slots = (uint32_t)chunks + in.requests;
   if (in.shared && in.requests > 1) {
-    p.pblocks = (uint32_t)(((uint64_t)in.requests * in.tokens * group + p.rows - 1) / p.rows);
-    const uint32_t want = std::max(1u, std::min({4 * cus / std::max(1u, in.kv_heads * p.pblocks), in.shared / (p.unit * p.least) + 1, PAGES_PREFIX}));
-    p.per = ((in.shared + want - 1) / want + p.unit - 1) / p.unit * p.unit;
+    shape(prows, p.pstaged, p.prw, p.prows);
+    p.pblocks = (uint32_t)((prows + p.prows - 1) / p.prows);
+    const uint32_t pw = p.pstaged || p.HD <= 128 ? 8 : 4;
+    uint32_t unit = !p.mfma ? 4 * p.T : p.pstaged ? (p.HD == 256 ? 64 : 128) : (in.kv16 ? 32 : 16) * (pw / p.prw);
+    unit = std::max(unit, 1u << in.shift);
+    const uint32_t want = std::max(1u, std::min({(p.mfma ? 1 : 4) * cus / std::max(1u, in.kv_heads * p.pblocks), (in.shared + unit - 1) / unit, PAGES_PREFIX}));
+    p.per = ((in.shared + want - 1) / want + unit - 1) / unit * unit;
     p.nprefix = (in.shared + p.per - 1) / p.per;
   }
   return p;
@@ -386,6 +688,45 @@ uint64_t attention_pages_scratch_floats(const PagesAttnArgs &in) {
   return pages_pairs(rows, in.hd) + 2 * rows;
 }
 
+template <bool PREFIX, class E>
+static void launch_pages_any(hipStream_t s, const PagesK &a, const PagesLaunch &p) {
+  const size_t lds = tree_any_lds(a.hd, p.T);
+  if (lds > 50000) lds_opt_in_bytes((const void *)k_pages_any<E, PREFIX>, 100000);
+  hipLaunchKernelGGL((k_pages_any<E, PREFIX>), dim3(a.kvh * (PREFIX ? p.pblocks : p.blocks), PREFIX ? p.nprefix : p.slots), dim3(256), lds, s, a, p.T);
+}
+template <uint32_t HD, class E, bool FULL, bool PREFIX>
+static void launch_pages_direct(hipStream_t s, const PagesK &a, const PagesLaunch &p) {
+  constexpr uint32_t waves = tree_threads<HD>() / 64;
+  constexpr size_t lds = std::max(tree_wave_lds<HD, 1>() * waves, tree_any_lds(HD, tree_any_tile(HD)));
+  static_assert(lds + 4 * PAGES_IDS + 2 * WGD_REQUESTS_MAX + 1024 <= LDS_MAX, "the wavefronts' outputs fit LDS");
+  lds_opt_in_bytes((const void *)k_pages<HD, E, FULL, PREFIX>, (uint32_t)lds);
+  hipLaunchKernelGGL((k_pages<HD, E, FULL, PREFIX>), dim3(a.kvh * (PREFIX ? p.pblocks : p.blocks), PREFIX ? p.nprefix : p.slots), dim3(64 * waves), lds, s,
+                     a, PREFIX ? p.prw : p.rw);
+}
+template <uint32_t HD, bool PREFIX>
+static void launch_pages_staged(hipStream_t s, const PagesK &a, const PagesLaunch &p) {
+  constexpr uint32_t RT = HD == 256 ? 1 : 2, SK = HD == 256 ? 64 : 128, waves = TREE_STAGED_NT / 64;
+  constexpr size_t lds = std::max({tree_wave_lds<HD, RT>() * waves, tree_any_lds(HD, tree_any_tile(HD)), (size_t)4 * SK * 2 * HD});
+  static_assert(lds + 4 * PAGES_IDS + 2 * WGD_REQUESTS_MAX + 1024 <= LDS_MAX, "two stages, and the wavefronts' outputs, fit LDS");
+  lds_opt_in_bytes((const void *)k_pages_staged<HD, RT, SK, PREFIX>, (uint32_t)lds);
+  hipLaunchKernelGGL((k_pages_staged<HD, RT, SK, PREFIX>), dim3(a.kvh * (PREFIX ? p.pblocks : p.blocks), PREFIX ? p.nprefix : p.slots), dim3(TREE_STAGED_NT),
+                     lds, s, a, PREFIX ? p.prw : p.rw);
+}
+template <uint32_t HD, class E, bool PREFIX>
+static void launch_pages_hd(hipStream_t s, const PagesK &a, const PagesLaunch &p) {
+  if (a.hd < HD) return launch_pages_direct<HD, E, false, PREFIX>(s, a, p);
+  if constexpr (sizeof(E) == 2)
+    if (PREFIX ? p.pstaged : p.staged) return launch_pages_staged<HD, PREFIX>(s, a, p);
+  launch_pages_direct<HD, E, true, PREFIX>(s, a, p);
+}
+template <class E, bool PREFIX>
+static void launch_pages(hipStream_t s, const PagesK &a, const PagesLaunch &p) {
+  if (!p.mfma) launch_pages_any<PREFIX, E>(s, a, p);
+  else if (p.HD == 64) launch_pages_hd<64, E, PREFIX>(s, a, p);
+  else if (p.HD == 128) launch_pages_hd<128, E, PREFIX>(s, a, p);
+  else launch_pages_hd<256, E, PREFIX>(s, a, p);
+}
+
 hipError_t attention_pages(hipStream_t s, const PagesAttnArgs &in) {
   if (!in.requests) return hipSuccess;
   if (!in.kv_heads || in.heads % in.kv_heads || !in.hd || in.hd > 512 || !in.window || !in.tokens || in.requests > WGD_REQUESTS_MAX ||
@@ -397,20 +738,13 @@ hipError_t attention_pages(hipStream_t s, const PagesAttnArgs &in) {
   a.heads = in.heads; a.kvh = in.kv_heads; a.group = in.heads / in.kv_heads; a.hd = in.hd; a.window = in.window; a.shift = in.shift;
   a.max_pages = in.max_pages; a.pages = in.pages; a.requests = in.requests; a.tokens = in.tokens;
   a.shared = p.nprefix ? in.shared : 0; a.owner = in.owner;
-  a.unit = p.unit; a.least = p.least; a.target = p.target; a.slots = p.slots; a.nprefix = p.nprefix; a.per = p.per; a.blocks = p.blocks;
+  a.unit = p.unit; a.least = p.least; a.target = p.target; a.slots = p.slots; a.nprefix = p.nprefix; a.per = p.per;
   a.scale = in.scale;
-  const size_t lds = tree_any_lds(in.hd, p.T);
-  auto any = [&](auto kernel, uint32_t x, uint32_t y) {
-    if (lds > 50000) lds_opt_in_bytes((const void *)kernel, 100000);
-    hipLaunchKernelGGL(kernel, dim3(x, y), dim3(256), lds, s, a, p.T);
-  };
   if (p.nprefix) {
-    if (in.kv16) any(k_pages_any<_Float16, true>, in.kv_heads * p.pblocks, p.nprefix);
-    else any(k_pages_any<float, true>, in.kv_heads * p.pblocks, p.nprefix);
+    in.kv16 ? launch_pages<_Float16, true>(s, a, p) : launch_pages<float, true>(s, a, p);
     WGD_HIP(hipGetLastError());
   }
-  if (in.kv16) any(k_pages_any<_Float16, false>, in.kv_heads * p.blocks, p.slots);
-  else any(k_pages_any<float, false>, in.kv_heads * p.blocks, p.slots);
+  in.kv16 ? launch_pages<_Float16, false>(s, a, p) : launch_pages<float, false>(s, a, p);
   WGD_HIP(hipGetLastError());
   if (!pages_joins(in, p)) return hipSuccess;
   const uint64_t rows = (uint64_t)in.requests * in.tokens * in.heads;

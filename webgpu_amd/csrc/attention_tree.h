@@ -482,13 +482,12 @@ struct TreeWave : TreeRows<HD, 1, tree_nb<E>(), tree_ve<HD, E>()> {
       }
     }
   }
-  // The first block's keys, asked for before anything else.
-  __device__ __forceinline__ void begin(const TreeK &a, uint32_t kv, uint32_t t0, uint32_t end) {
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, bytes = (FULL ? HD : a.hd) * sizeof(E);
-    k = (const uint8_t *)a.k + (uint64_t)kv * bytes;
-    v = (const uint8_t *)a.v + (uint64_t)kv * bytes;
-    rowb = (uint64_t)a.kvh * bytes;  // below 2^27 (tree_plan)
-    cap = a.capacity; hi = end;
+  // Kv head kv of caches of `heads`, and this lane's offsets in their rows.
+  __device__ __forceinline__ void place(const void *keys, const void *values, uint32_t heads, uint32_t hd, uint32_t kv) {
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, bytes = (FULL ? HD : hd) * sizeof(E);
+    k = (const uint8_t *)keys + (uint64_t)kv * bytes;
+    v = (const uint8_t *)values + (uint64_t)kv * bytes;
+    rowb = (uint64_t)heads * bytes;  // below 2^27 (tree_plan)
     k_row = c * (uint32_t)rowb;
     v_row = 4 * g * (uint32_t)rowb;
 #pragma unroll
@@ -498,24 +497,76 @@ struct TreeWave : TreeRows<HD, 1, tree_nb<E>(), tree_ve<HD, E>()> {
       v_piece[x] = (16 * x + c) * (uint32_t)sizeof(vpiece);
       if (!FULL) v_piece[x] = min(v_piece[x], bytes - (uint32_t)sizeof(vpiece));
     }
+  }
+  // The first block's keys, asked for before anything else.
+  __device__ __forceinline__ void begin(const TreeK &a, uint32_t kv, uint32_t t0, uint32_t end) {
+    place(a.k, a.v, a.kvh, a.hd, kv);
+    cap = a.capacity; hi = end;
     if (t0 >= hi) return;
     base = t0 % cap;
     load_k(t0);
   }
 
   // The row's query times scale log2 e as operand.
-  __device__ __forceinline__ void load_q(const TreeK &a, const float *q, bool ok) {
-    const float f = a.scale * TREE_LOG2E;
+  __device__ __forceinline__ void load_q(float scale, uint32_t hd, const float *q, bool ok) {
+    const float f = scale * TREE_LOG2E;
     if constexpr (!HALF) {
       const uint32_t g = (threadIdx.x & 63) >> 4;
 #pragma unroll
       for (uint32_t t = 0; t < KT; t++) {
-        const f32x4 x = ok && (FULL || 16 * t + 4 * g < a.hd) ? *(const f32x4 *)(q + 16 * t + 4 * g) : f32x4{0, 0, 0, 0};
+        const f32x4 x = ok && (FULL || 16 * t + 4 * g < hd) ? *(const f32x4 *)(q + 16 * t + 4 * g) : f32x4{0, 0, 0, 0};
         qh[t] = __builtin_bit_cast(u32x4, f32x4{x.x * f, x.y * f, x.z * f, x.w * f});
       }
       qs = 1.f;
     } else {
-      qs = tree_query<KT>(q, FULL ? HD : a.hd, f, ok, qh, ql);
+      qs = tree_query<KT>(q, FULL ? HD : hd, f, ok, qh, ql);
+    }
+  }
+  // The scores of the block in kr, over qs.
+  __device__ __forceinline__ void scores(f32x4 (&s)[NB]) const {
+#pragma unroll
+    for (uint32_t b = 0; b < NB; b++) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (uint32_t t = 0; t < KT; t++) {
+        if constexpr (HALF) {
+          const f16x8 kf = __builtin_bit_cast(f16x8, kr[b][t]);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, qh[t]), acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, ql[t]), acc, 0, 0, 0);
+        } else {
+          const f32x4 kf = __builtin_bit_cast(f32x4, kr[b][t]), qf = __builtin_bit_cast(f32x4, qh[t]);
+#pragma unroll
+          for (int u = 0; u < 4; u++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[u], qf[u], acc, 0, 0, 0);
+        }
+      }
+      s[b] = acc;
+    }
+  }
+  // The values of a block times its weights s.
+  __device__ __forceinline__ void values(const vpiece (&vr)[VK][NX], const f32x4 (&s)[NB]) {
+    if constexpr (HALF) {
+      f16x8 ph, pl;
+      tree_split(s, ph, pl);
+#pragma unroll
+      for (uint32_t x = 0; x < NX; x++)
+#pragma unroll
+        for (uint32_t e = 0; e < VE; e++) {
+          u32x4 f;  // half e of the eight keys
+#pragma unroll
+          for (uint32_t i = 0; i < 4; i++)
+            f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][x][e / 2], vr[2 * i][x][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+          const f16x8 vf = __builtin_bit_cast(f16x8, f);
+          o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[0][x][e], 0, 0, 0);
+          o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[0][x][e], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 4; i++)
+#pragma unroll
+        for (uint32_t x = 0; x < NX; x++)
+#pragma unroll
+          for (uint32_t e = 0; e < VE; e++)
+            o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i][x][e]), s[0][i], o[0][x][e], 0, 0, 0);
     }
   }
 
@@ -541,56 +592,15 @@ struct TreeWave : TreeRows<HD, 1, tree_nb<E>(), tree_ve<HD, E>()> {
           for (uint32_t x = 0; x < NX; x++) vr[j][x] = *(const vpiece *)(row + v_piece[x]);
         }
       }
-      // ---- scores
       f32x4 s[NB];
-#pragma unroll
-      for (uint32_t b = 0; b < NB; b++) {
-        f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t t = 0; t < KT; t++) {
-          if constexpr (HALF) {
-            const f16x8 kf = __builtin_bit_cast(f16x8, kr[b][t]);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, qh[t]), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, __builtin_bit_cast(f16x8, ql[t]), acc, 0, 0, 0);
-          } else {
-            const f32x4 kf = __builtin_bit_cast(f32x4, kr[b][t]), qf = __builtin_bit_cast(f32x4, qh[t]);
-#pragma unroll
-            for (int u = 0; u < 4; u++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[u], qf[u], acc, 0, 0, 0);
-          }
-        }
-        s[b] = acc;
-      }
+      scores(s);
       base += step;
       if (base >= cap) base %= cap;
       if (t0 + step < hi) load_k(t0 + step);
-      // ---- weights, in place of the scores
+      // weights, in place of the scores
       const bool masked = t0 + KEYS > min(hi, a.start) || t0 < masked_below;
       this->weigh(0, s, qs, masked, masked ? tree_sees(a, L, seen, t0, hi) : 0);
-      // ---- values
-      if constexpr (HALF) {
-        f16x8 ph, pl;
-        tree_split(s, ph, pl);
-#pragma unroll
-        for (uint32_t x = 0; x < NX; x++)
-#pragma unroll
-          for (uint32_t e = 0; e < VE; e++) {
-            u32x4 f;  // half e of the eight keys
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++)
-              f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][x][e / 2], vr[2 * i][x][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
-            const f16x8 vf = __builtin_bit_cast(f16x8, f);
-            o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[0][x][e], 0, 0, 0);
-            o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[0][x][e], 0, 0, 0);
-          }
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++)
-#pragma unroll
-          for (uint32_t x = 0; x < NX; x++)
-#pragma unroll
-            for (uint32_t e = 0; e < VE; e++)
-              o[0][x][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i][x][e]), s[0][i], o[0][x][e], 0, 0, 0);
-      }
+      values(vr, s);
     }
   }
 };
@@ -725,7 +735,7 @@ __global__ __launch_bounds__((tree_threads<HD>())) void k_attn_tree(TreeK a, Tre
   uint32_t row[1];
   TreeSeen seen[1];
   tree_rows<1>(a, L, p, row, seen);
-  s.load_q(a, a.q + tree_row(a, p.kv, row[0]) * a.hd, p.wrow + (threadIdx.x & 15) < p.nrows);
+  s.load_q(a.scale, a.hd, a.q + tree_row(a, p.kv, row[0]) * a.hd, p.wrow + (threadIdx.x & 15) < p.nrows);
   s.walk(a, L, seen[0], from, p.slices * Wave::KEYS, p.masked_below);
   tree_end<HD, E, 1, tree_threads<HD>()>(a, gr, L, lds, p, s, seen);
 }
@@ -767,9 +777,9 @@ struct TreeStaged : TreeRows<HD, RT, 2, 1> {
   u32x4 qh[RT][KT], ql[RT][KT];
   float qs[RT];
 
-  // A block of 32 keys: its K and V rows in LDS, the first key t0; keys end at hi.
-  __device__ __forceinline__ void block(const TreeK &a, const TreeLds &L, const TreeSeen (&seen)[RT], const uint8_t *K, const uint8_t *V,
-                                        uint32_t t0, uint32_t hi, uint32_t masked_below) {
+  // A block of 32 keys: its K and V rows in LDS. With `masked`, sees(rt) has the keys that the lane's row of tile rt sees, as bits.
+  template <class F>
+  __device__ __forceinline__ void block(const uint8_t *K, const uint8_t *V, bool masked, F &&sees) {
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     f32x4 s[RT][2];
 #pragma unroll
@@ -788,11 +798,10 @@ struct TreeStaged : TreeRows<HD, RT, 2, 1> {
           s[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t], __builtin_bit_cast(f16x8, ql[rt][t]), s[rt][b], 0, 0, 0);
         }
     }
-    const bool masked = t0 + 32 > min(hi, a.start) || t0 < masked_below;
     f16x8 ph[RT], pl[RT];
 #pragma unroll
     for (uint32_t rt = 0; rt < RT; rt++) {
-      this->weigh(rt, s[rt], qs[rt], masked, masked ? tree_sees(a, L, seen[rt], t0, hi) : 0);
+      this->weigh(rt, s[rt], qs[rt], masked, masked ? sees(rt) : 0);
       tree_split(s[rt], ph[rt], pl[rt]);
     }
     // lane (g, i) reads dims 4 (i % 4) .. + 4 of key 4 g + i / 4 and receives dim i of keys 4 g .. + 4
@@ -880,8 +889,11 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_attn_tree_staged(TreeK a, Tr
     if (t0 + SK < p.hi) load(t0 + SK, stage ^ 1);
     const uint8_t *K = stages + stage * 2 * SK * ROW, *V = K + SK * ROW;
     if (p.wrow < p.nrows)
-      for (uint32_t b = p.slice; b < SK / 32 && t0 + 32 * b < p.hi; b += p.slices)
-        s.block(a, L, seen, K + 32 * b * ROW, V + 32 * b * ROW, t0 + 32 * b, p.hi, p.masked_below);
+      for (uint32_t b = p.slice; b < SK / 32 && t0 + 32 * b < p.hi; b += p.slices) {
+        const uint32_t t = t0 + 32 * b;
+        s.block(K + 32 * b * ROW, V + 32 * b * ROW, t + 32 > min(p.hi, a.start) || t < p.masked_below,
+                [&](uint32_t rt) { return tree_sees(a, L, seen[rt], t, p.hi); });
+      }
   }
   tree_end<HD, _Float16, RT, TREE_STAGED_NT>(a, gr, L, lds, p, s, seen);
 }
