@@ -1051,7 +1051,7 @@ int wgd_adapters(wgd_context *ctx, int32_t type, const wgd_buffer *a, const wgd_
   if (type != F32 && type != F16) return fail(ctx, WGD_E_INVALID, "%s: type %d; F32 and F16 are supported", what, type);
   for (const wgd_buffer *p : {a, b})
     if (p->layout != LAYOUT_GGUF || (p->type >= 0 && p->type != type)) return fail(ctx, WGD_E_INVALID, "%s: weights %s were uploaded as type %d", what, p->label.c_str(), p->type);
-  if (!cols || !rows || !rank || rank > 1024 || !adapters_ || adapters_ > 0x7FFFFFFFu || batch > (1u << 24))
+  if (!cols || !rows || cols > 0x7FFFFFFFu || rows > 0x7FFFFFFFu || !rank || rank > 1024 || !adapters_ || adapters_ > 0x7FFFFFFFu || batch > (1u << 24))
     return fail(ctx, WGD_E_INVALID, "%s: %u adapters of rank %u, %u x %u, for %u rows", what, adapters_, rank, rows, cols, batch);
   if (batch > 1 && stride < (uint64_t)row_base + rows) return fail(ctx, WGD_E_INVALID, "%s: stride %u < rowBase + rows", what, stride);
   if (!apart({y}, {a, b, which, scales, x})) return fail(ctx, WGD_E_INVALID, "%s: the output needs a buffer of its own", what);
