@@ -373,7 +373,8 @@ int wgd_attention_pages_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_b
  *   y[t * stride + row_base + r] += scales[w] * sum_k B[w][r][k] (sum_c A[w][k][c] x[t][c]),  r < rows, k < rank, c < cols;
  * rows with w outside [0, adapters) stay as they are, as does what lies around them. a is [adapters][rank][cols] and b
  * [adapters][rows][rank], both F32 or F16 (`type`; GGUF's lora_a and lora_b as they are), lower ranks filled up with zeros;
- * scales f32[adapters] (alpha / rank). Products and sums are f32. rank <= 1024, cols and rows < 2^31, batch <= 2^24. */
+ * scales f32[adapters] (alpha / rank). Sums are f32, and products too with F32 weights; with F16 ones x and the inner sums enter
+ * them as two f16 each: an entry is off by 2^-22 of itself and 2^-39 of its row's largest (64 inner sums at a time), and an infinity beside a weight may become NaN. rank <= 1024, cols and rows < 2^31, batch <= 2^24. */
 int wgd_adapters(wgd_context *ctx, int32_t type, const wgd_buffer *a, const wgd_buffer *b, const wgd_buffer *which,
                  const wgd_buffer *scales, const wgd_buffer *x, wgd_buffer *y, uint32_t cols, uint32_t rows, uint32_t rank,
                  uint32_t adapters, uint32_t stride, uint32_t row_base, uint32_t batch);
