@@ -15,7 +15,8 @@ namespace wgd {
 struct PagesK {
   const float *q; const void *k, *v; float *y, *part; const int32_t *table, *lengths, *counts;
   uint32_t heads, kvh, group, hd, window, shift, max_pages, pages, requests, tokens, shared, owner;
-  uint32_t unit, least, target, slots;  // keys of a unit; least units of a chunk; chunks wanted, and at most
+  uint32_t unit, least, slots;          // keys of a unit (1 << unit); least units of a chunk; chunks at most
+  float per_target;                     // 1 / the chunks wanted, rounded up
   uint32_t nprefix, per;                // parts of the prefix, keys of each
   float scale;
 };
@@ -31,44 +32,62 @@ __host__ __device__ __forceinline__ uint64_t pages_pairs(uint64_t part_rows, uin
 struct PagesRequest { uint32_t len, n, lo; bool shares; };  // its keys start at lo where it shares nothing
 __device__ __forceinline__ PagesRequest pages_request(const PagesK &a, uint32_t r) {
   PagesRequest q = {0, 0, 0, false};
+  const uint32_t at = min(r, a.requests - 1), cap = a.max_pages << a.shift;
+  // (all loads before any of them is waited for)
+  const int32_t len = a.lengths[at], count = a.counts ? a.counts[at] : (int32_t)a.tokens;
+  int32_t owner_len = 0, page = -1, owner_page = -2;
+  if (a.shared) {
+    const uint32_t c = (a.shared >> a.shift) - 1;
+    owner_len = a.lengths[a.owner];
+    page = a.table[(uint64_t)at * a.max_pages + c];
+    owner_page = a.table[(uint64_t)a.owner * a.max_pages + c];
+  }
   if (r >= a.requests) return q;
-  q.len = min((uint32_t)max(a.lengths[r], 0), a.max_pages << a.shift);
-  q.n = min(q.len, a.counts ? (uint32_t)min(max(a.counts[r], 0), (int32_t)a.tokens) : a.tokens);
+  q.len = min((uint32_t)max(len, 0), cap);
+  q.n = min(q.len, (uint32_t)min(max(count, 0), (int32_t)a.tokens));
   const uint32_t first = q.len - q.n + 1;  // keys up to the first query's own
   q.lo = first > a.window ? first - a.window : 0;
   if (a.shift >= 4) q.lo &= ~15u;  // whole halves of blocks, on the same page; nothing before the first key is read
-  if (a.shared) {
-    const uint32_t c = (a.shared >> a.shift) - 1;
-    const bool owned = min((uint32_t)max(a.lengths[a.owner], 0), a.max_pages << a.shift) >= a.shared;
-    q.shares = owned && q.n && q.len - q.n >= a.shared && q.len <= a.window &&
-               a.table[(uint64_t)r * a.max_pages + c] == a.table[(uint64_t)a.owner * a.max_pages + c];
-  }
+  q.shares = a.shared && min((uint32_t)max(owner_len, 0), cap) >= a.shared && q.n && q.len - q.n >= a.shared && q.len <= a.window && page == owner_page;
   return q;
 }
 __device__ __forceinline__ uint32_t pages_units(const PagesK &a, const PagesRequest &q, bool sharing) {
   const uint32_t lo = sharing && q.shares ? a.shared : q.lo;
-  return q.n ? (q.len - lo + a.unit - 1) / a.unit : 0;
+  return q.n ? (q.len - lo + (1u << a.unit) - 1) >> a.unit : 0;
 }
+// Sums over the lanes up to this one.
+__device__ __forceinline__ uint32_t pages_sums(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast15 into rows 1 and 3
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // row_bcast31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ uint32_t pages_lane(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
 
-// The plan of all requests: whether a prefix is shared (by two or more), and the units of a chunk.
-struct PagesPlan { bool sharing; uint32_t chunk; };
+// The plan of all requests: whether a prefix is shared (by two or more), and the units of a chunk. `first` has the first 64 requests.
+struct PagesPlan { bool sharing; uint32_t chunk; PagesRequest first; };
 __device__ __forceinline__ PagesPlan pages_plan(const PagesK &a) {
   const uint32_t lane = threadIdx.x & 63;
-  uint64_t alone = 0, apart = 0;
+  PagesPlan p = {false, 0, {0, 0, 0, false}};
+  float alone = 0.f, apart = 0.f;  // units; below 2^-20 off, which per_target makes up for
   uint32_t sharers = 0;
   for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
     const PagesRequest q = pages_request(a, r0 + lane);
-    alone += pages_units(a, q, false);
-    apart += pages_units(a, q, true);
-    sharers += (uint32_t)__popcll(__ballot(q.shares));
+    if (r0 == 0) p.first = q;
+    alone += wave_total((float)pages_units(a, q, false));
+    if (a.shared) {
+      apart += wave_total((float)pages_units(a, q, true));
+      sharers += (uint32_t)__popcll(__ballot(q.shares));
+    }
   }
-  const bool sharing = sharers > 1;
-  uint64_t sum = sharing ? apart : alone;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor((unsigned long long)sum, o, 64);
-  const uint64_t even = (sum + a.target - 1) / a.target;
-  const uint32_t whole = 0x7FFFFFFFu / a.unit + 1;  // the longest request
-  return PagesPlan{sharing, max(even < whole ? (uint32_t)even : whole, a.least)};
+  p.sharing = sharers > 1;
+  // rounded up, so that there are no more chunks than wanted, and one for each request
+  const float even = ceilf((p.sharing ? apart : alone) * a.per_target);
+  p.chunk = (uint32_t)__builtin_amdgcn_readfirstlane((int)max((uint32_t)fminf(even, 0x1p30f), a.least));
+  return p;
 }
 
 // One request in the plan: the slot of its first chunk, their number, its keys [lo, len). It is the one that has the slot `find`,
@@ -79,24 +98,19 @@ __device__ __forceinline__ PagesChunks pages_chunks(const PagesK &a, const Pages
   const uint32_t lane = threadIdx.x & 63;
   uint32_t before = 0;
   for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
-    const PagesRequest q = pages_request(a, r0 + lane);
+    const PagesRequest q = r0 ? pages_request(a, r0 + lane) : plan.first;
     const uint32_t units = pages_units(a, q, plan.sharing);
     const uint32_t mine = r0 + lane < a.requests ? max(1u, (units + plan.chunk - 1) / plan.chunk) : 0;
-    uint32_t s = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const uint32_t u = (uint32_t)__shfl_up((int)s, o, 64);
-      if (lane >= (uint32_t)o) s += u;
+    const uint32_t s = pages_sums(mine) + before;
+    const uint64_t here = __ballot(BY_REQUEST ? r0 + lane == find : find < s);  // the first of these
+    if (here && (BY_REQUEST || find < pages_lane(s, 63))) {
+      const uint32_t at = (uint32_t)__ffsll((unsigned long long)here) - 1;
+      const bool shares = plan.sharing && (__ballot(q.shares) >> at & 1);
+      const uint32_t count = pages_lane(mine, at);
+      return PagesChunks{r0 + at, pages_lane(s, at) - count, count, shares ? a.shared : pages_lane(q.lo, at), pages_lane(q.len, at),
+                         pages_lane(q.n, at), shares};
     }
-    const uint64_t here = __ballot(BY_REQUEST ? r0 + lane == find : mine && find >= before + s - mine && find < before + s);
-    if (here) {
-      const int at = (int)__ffsll((unsigned long long)here) - 1;
-      const bool shares = plan.sharing && q.shares;
-      return PagesChunks{r0 + (uint32_t)at, before + (uint32_t)__shfl((int)(s - mine), at, 64), (uint32_t)__shfl((int)mine, at, 64),
-                         (uint32_t)__shfl((int)(shares ? a.shared : q.lo), at, 64), (uint32_t)__shfl((int)q.len, at, 64),
-                         (uint32_t)__shfl((int)q.n, at, 64), (bool)__shfl((int)shares, at, 64)};
-    }
-    before += (uint32_t)__shfl((int)s, 63, 64);
+    before = pages_lane(s, 63);
   }
   return PagesChunks{0xFFFFFFFFu, 0, 0, 0, 0, 0, false};
 }
@@ -111,14 +125,23 @@ struct PagesPart {
   bool direct;               // the only part of its rows: to y
   uint64_t part;             // else the first row of its part
 };
+// i / d by its reciprocal, for i < 2^25.
+__device__ __forceinline__ uint32_t pages_div(uint32_t i, uint32_t d) {
+  if (d == 1) return i;
+  uint32_t q = (uint32_t)((float)i * __builtin_amdgcn_rcpf((float)d));
+  q -= q * d > i;
+  return q + ((q + 1) * d <= i);
+}
 struct PagesRow { bool valid; uint64_t row; uint32_t request, query, begin, end; };  // row of q and y; keys [begin, end)
 __device__ __forceinline__ PagesRow pages_row(const PagesK &a, const PagesPart &p, uint32_t i) {
   PagesRow w = {i < p.nrows, 0, p.r, 0, 0, 0};
   if (!w.valid) return w;
-  uint32_t t = i / a.group;
+  const uint32_t at = !p.list && a.tokens == 1 ? 0 : pages_div(i, a.group), head = i - at * a.group;
+  uint32_t t = at;
   if (p.list) {
-    w.request = p.list[t / a.tokens];
-    t %= a.tokens;
+    const uint32_t u = pages_div(at, a.tokens);
+    w.request = p.list[u];
+    t = at - u * a.tokens;
     w.end = p.hi;
     w.valid = !a.counts || (int32_t)t < a.counts[w.request];
   } else {
@@ -127,7 +150,7 @@ __device__ __forceinline__ PagesRow pages_row(const PagesK &a, const PagesPart &
     w.valid = t < p.n;
   }
   w.query = t;
-  w.row = ((uint64_t)w.request * a.tokens + t) * a.heads + p.kv * a.group + i % a.group;
+  w.row = ((uint64_t)w.request * a.tokens + t) * a.heads + p.kv * a.group + head;
   return w;
 }
 // Where a part keeps row w: own parts have the rows of one request, those of the prefix all of them.
@@ -281,10 +304,11 @@ __device__ __forceinline__ bool pages_part(const PagesK &a, uint32_t rows, uint1
   } else {
     const PagesChunks c = pages_chunks<false>(a, plan, blockIdx.y);
     if (c.r == 0xFFFFFFFFu) return false;
-    const uint32_t at = blockIdx.y - c.first, units = c.n ? (c.len - c.lo + a.unit - 1) / a.unit : 0;  // no fewer than chunks, or 0
+    const uint32_t at = blockIdx.y - c.first, units = c.n ? (c.len - c.lo + (1u << a.unit) - 1) >> a.unit : 0;  // no fewer than chunks, or 0
+    const uint32_t each = units / c.count, more = units - each * c.count;  // the first `more` chunks have one unit more
     p.nrows = c.n * a.group;
-    p.lo = c.lo + (uint32_t)((uint64_t)units * at / c.count) * a.unit;
-    p.hi = at + 1 == c.count ? c.len : c.lo + (uint32_t)((uint64_t)units * (at + 1) / c.count) * a.unit;
+    p.lo = c.lo + ((at * each + min(at, more)) << a.unit);
+    p.hi = at + 1 == c.count ? c.len : c.lo + (((at + 1) * each + min(at + 1, more)) << a.unit);
     p.r = c.r; p.n = c.n; p.end0 = c.len - c.n + 1;
     p.seen = p.end0 > a.window ? p.end0 - a.window : 0;
     p.table = a.table + (uint64_t)c.r * a.max_pages;
@@ -330,13 +354,18 @@ __device__ __forceinline__ uint32_t pages_mask(uint32_t begin, uint32_t end, uin
 template <uint32_t NT>
 __device__ __forceinline__ bool pages_ids(const PagesK &a, const PagesPart &p, uint32_t *ids, uint32_t k0, uint32_t k1) {
   const uint32_t first = k0 >> a.shift, n = ((k1 - 1) >> a.shift) + 1 - first;
+  int32_t id[PAGES_IDS / NT];
+#pragma unroll
+  for (uint32_t e = 0; e < PAGES_IDS / NT; e++)
+    if (e == 0 || e * NT < n) id[e] = p.table[first + min(threadIdx.x + e * NT, n - 1)];
   bool none = false;
-  for (uint32_t i = threadIdx.x; i < n; i += NT) {
-    const int32_t id = p.table[first + i];
-    const bool ok = id >= 0 && (uint32_t)id < a.pages;
-    none |= !ok;
-    ids[i] = ok ? (uint32_t)id : 0;
-  }
+#pragma unroll
+  for (uint32_t e = 0; e < PAGES_IDS / NT; e++)
+    if (threadIdx.x + e * NT < n) {
+      const bool ok = id[e] >= 0 && (uint32_t)id[e] < a.pages;
+      none |= !ok;
+      ids[threadIdx.x + e * NT] = ok ? (uint32_t)id[e] : 0;
+    }
   return __syncthreads_or(none);
 }
 
@@ -348,6 +377,7 @@ struct PagesWave : TreeWave<HD, E, FULL> {
   typedef typename Wave::vpiece vpiece;
   const uint32_t *ids;  // from page `first` on
   uint32_t first, shift, seen;
+  vpiece vr[VK][NX];
 
   __device__ __forceinline__ uint64_t at(uint32_t t) const {  // of one key, the nearest of [seen, hi)
     t = min(max(t, seen), hi - 1);
@@ -357,54 +387,101 @@ struct PagesWave : TreeWave<HD, E, FULL> {
     const uint32_t id = __builtin_amdgcn_readfirstlane(ids[(t >> shift) - first]);
     return (((uint64_t)id << shift) + (t & ((1u << shift) - 1))) * rowb;
   }
-  __device__ __forceinline__ bool whole(uint32_t t) const { return shift >= 4 && t >= seen && t + KEYS <= hi; }
+  // Blocks of keys one behind the other, all there: 16 keys at a time on one page.
   __device__ __forceinline__ void load_k(uint32_t t) {
-    const uint32_t c = threadIdx.x & 15;
-    if (whole(t)) {
 #pragma unroll
-      for (uint32_t b = 0; b < NB; b++) {
-        const uint8_t *row = k + half(t + 16 * b);
+    for (uint32_t b = 0; b < NB; b++) {
+      const uint8_t *row = k + half(t + 16 * b);
 #pragma unroll
-        for (uint32_t u = 0; u < KT; u++) kr[b][u] = *(const u32x4 *)(row + (k_row + k_piece[u]));
-      }
+      for (uint32_t u = 0; u < KT; u++) kr[b][u] = *(const u32x4 *)(row + (k_row + k_piece[u]));
+    }
+  }
+  __device__ __forceinline__ void load_v(uint32_t t) {
+#pragma unroll
+    for (uint32_t b = 0; b < NB; b++) {
+      const uint8_t *rows = v + half(t + 16 * b);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+        for (uint32_t x = 0; x < NX; x++) vr[4 * b + j][x] = *(const vpiece *)(rows + j * rowb + (v_row + v_piece[x]));
+    }
+  }
+  // A block of any keys.
+  __device__ __forceinline__ void load_any(uint32_t t) {
+    const uint32_t c = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; b++) {
+      const uint8_t *row = k + at(t + 16 * b + c);
+#pragma unroll
+      for (uint32_t u = 0; u < KT; u++) kr[b][u] = *(const u32x4 *)(row + k_piece[u]);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < VK; j++) {
+      const uint8_t *row = v + at(t + 16 * (j / 4) + 4 * g + j % 4);
+#pragma unroll
+      for (uint32_t x = 0; x < NX; x++) vr[j][x] = *(const vpiece *)(row + v_piece[x]);
+    }
+  }
+  // A query's dims as the operands need them, zero where ok is off (the place is there all the same).
+  static constexpr uint32_t QN = Wave::HALF ? 2 * KT : KT;
+  __device__ __forceinline__ void ask_q(const float *q, uint32_t hd, f32x4 (&x)[QN]) const {
+    const uint32_t g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (uint32_t t = 0; t < QN; t++) x[t] = *(const f32x4 *)(q + piece(t, g, FULL ? HD : hd));
+  }
+  static __device__ __forceinline__ uint32_t piece(uint32_t t, uint32_t g, uint32_t hd) {
+    const uint32_t d = Wave::HALF ? 32 * (t / 2) + 8 * g + 4 * (t % 2) : 16 * t + 4 * g;
+    return FULL ? d : min(d, hd - 4);
+  }
+  __device__ __forceinline__ void take_q(f32x4 (&x)[QN], float scale, uint32_t hd, bool ok) {
+    const uint32_t g = (threadIdx.x & 63) >> 4;
+    const float f = scale * TREE_LOG2E;
+#pragma unroll
+    for (uint32_t t = 0; t < QN; t++) {
+      const bool there = ok && (FULL || piece(t, g, hd) == (Wave::HALF ? 32 * (t / 2) + 8 * g + 4 * (t % 2) : 16 * t + 4 * g));
+      x[t] = there ? x[t] : f32x4{0, 0, 0, 0};
+    }
+    if constexpr (Wave::HALF) {
+      this->qs = tree_query_of<KT>(x, f, this->qh, this->ql);
     } else {
 #pragma unroll
-      for (uint32_t b = 0; b < NB; b++) {
-        const uint8_t *row = k + at(t + 16 * b + c);
-#pragma unroll
-        for (uint32_t u = 0; u < KT; u++) kr[b][u] = *(const u32x4 *)(row + k_piece[u]);
-      }
+      for (uint32_t t = 0; t < KT; t++) this->qh[t] = __builtin_bit_cast(u32x4, f32x4{x[t].x * f, x[t].y * f, x[t].z * f, x[t].w * f});
+      this->qs = 1.f;
+    }
+  }
+  __device__ __forceinline__ bool whole(uint32_t t) const { return shift >= 4 && t >= seen && t + KEYS <= hi; }
+  // Asks for the block at t0.
+  __device__ __forceinline__ void start(uint32_t t0) {
+    if (whole(t0)) {
+      load_k(t0);
+      load_v(t0);
+    } else {
+      load_any(t0);
     }
   }
   // Keys [t0, hi) in steps of `step`; the row sees [begin, end), all rows of the wavefront [all_begin, all_end).
+  // The keys and values of a block are asked for while the one before is at work, with no load behind a branch: what waits for one
+  // would wait for all.
   __device__ __forceinline__ void walk(uint32_t t0, uint32_t step, uint32_t begin, uint32_t end, uint32_t all_begin, uint32_t all_end) {
-    const uint32_t g = (threadIdx.x & 63) >> 4;
-    if (t0 < hi) load_k(t0);
-    for (; t0 < hi; t0 += step) {
-      vpiece vr[VK][NX];
-      if (whole(t0)) {
-#pragma unroll
-        for (uint32_t b = 0; b < NB; b++) {
-          const uint8_t *rows = v + half(t0 + 16 * b);
-#pragma unroll
-          for (uint32_t j = 0; j < 4; j++)
-#pragma unroll
-            for (uint32_t x = 0; x < NX; x++) vr[4 * b + j][x] = *(const vpiece *)(rows + j * rowb + (v_row + v_piece[x]));
-        }
-      } else {
-#pragma unroll
-        for (uint32_t j = 0; j < VK; j++) {
-          const uint8_t *row = v + at(t0 + 16 * (j / 4) + 4 * g + j % 4);
-#pragma unroll
-          for (uint32_t x = 0; x < NX; x++) vr[j][x] = *(const vpiece *)(row + v_piece[x]);
-        }
+    f32x4 s[NB];
+    auto weights = [&](uint32_t t) {
+      const bool masked = t + KEYS > min(hi, all_end) || t < all_begin;
+      this->weigh(0, s, this->qs, masked, masked ? pages_mask(begin, min(end, hi), t) : 0);
+    };
+    while (t0 < hi) {
+      start(t0);
+      const uint32_t last = whole(t0) ? t0 + (hi - KEYS - t0) / step * step : t0;
+      for (; t0 < last; t0 += step) {
+        this->scores(s);
+        load_k(t0 + step);
+        weights(t0);
+        this->values(vr, s);
+        load_v(t0 + step);
       }
-      f32x4 s[NB];
       this->scores(s);
-      if (t0 + step < hi) load_k(t0 + step);
-      const bool masked = t0 + KEYS > min(hi, all_end) || t0 < all_begin;
-      this->weigh(0, s, this->qs, masked, masked ? pages_mask(begin, min(end, hi), t0) : 0);
+      weights(t0);
       this->values(vr, s);
+      t0 += step;
     }
   }
 };
@@ -501,17 +578,25 @@ __global__ __launch_bounds__((tree_threads<HD>())) void k_pages(PagesK a, uint32
   const PagesRow row = pages_row(a, p, wrow + (threadIdx.x & 15));
   const PagesSees sees = pages_sees(row);
   Wave s;
+  f32x4 q[Wave::QN];
+  s.ask_q(a.q + row.row * a.hd, a.hd, q);
   s.place(a.k, a.v, a.kvh, a.hd, p.kv);
-  s.load_q(a.scale, a.hd, a.q + row.row * a.hd, row.valid);
   s.clear();
   s.ids = ids; s.shift = a.shift; s.seen = p.seen;
-  bool none = false;
-  for (uint32_t k0 = p.lo; k0 < p.hi && !none; k0 = s.hi) {
+  const uint32_t step = NT / 64 / rw * Wave::KEYS;
+  auto numbers = [&](uint32_t k0) {
     s.first = k0 >> a.shift;
     s.hi = min((uint64_t)p.hi, (uint64_t)(s.first + PAGES_IDS) << a.shift);
-    if (k0 > p.lo) __syncthreads();
-    none = pages_ids<NT>(a, p, ids, k0, s.hi);
-    if (!none && wrow < p.nrows) s.walk(k0 + slice * Wave::KEYS, NT / 64 / rw * Wave::KEYS, sees.begin, sees.end, sees.all_begin, sees.all_end);
+    return pages_ids<NT>(a, p, ids, k0, s.hi);
+  };
+  bool none = numbers(p.lo);
+  s.take_q(q, a.scale, a.hd, row.valid);
+  for (uint32_t k0 = p.lo; !none;) {
+    if (wrow < p.nrows) s.walk(k0 + slice * Wave::KEYS, step, sees.begin, sees.end, sees.all_begin, sees.all_end);
+    k0 = s.hi;
+    if (k0 >= p.hi) break;
+    __syncthreads();
+    none = numbers(k0);
   }
   pages_end<HD, E, 1, NT>(a, rw, lds, p, s, none);
 }
@@ -590,30 +675,35 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_pages_staged(PagesK a, uint3
 }
 
 // ------------------------------------------------------------------ the parts of a row
-// A wavefront per row: the weights of its parts go over the lanes and LDS, then lanes take the dims.
+// A wavefront per row: the weights of its parts go over the lanes and LDS, then lane groups of hd / 4 (VEC: hd a power of two from 4) take every
+// (64 / group)-th part, 16 bytes a lane and four loads ahead.
 constexpr uint32_t PAGES_TARGET = 512, PAGES_PREFIX = 256, PAGES_PARTS = PAGES_TARGET + 1 + PAGES_PREFIX;
+template <bool VEC>
 __global__ __launch_bounds__(256) void k_pages_join(PagesK a) {
   __shared__ float weight[4][PAGES_PARTS];
   const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const uint64_t all = (uint64_t)a.tokens * a.heads, row = blockIdx.x * 4ull + wv;
+  const uint32_t all = a.tokens * a.heads, row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wv);
   if (row >= a.requests * all) return;  // (no barriers below)
-  const uint32_t r = (uint32_t)(row / all);
+  const uint32_t r = row / all, within = row - r * all;
   const PagesPlan plan = pages_plan(a);
   const PagesChunks c = pages_chunks<true>(a, plan, r);
-  if (row % all / a.heads >= c.n || (c.count == 1 && !c.shares)) return;
+  if (within >= c.n * a.heads || (c.count == 1 && !c.shares)) return;
   const uint64_t pairs = pages_pairs(pages_part_rows(a.slots, a.nprefix, a.requests, all), a.hd);
   const uint32_t np = c.shares ? a.nprefix : 0, n = np + c.count;
-  auto at = [&](uint32_t i) { return i < np ? a.slots * all + (uint64_t)i * a.requests * all + row : (c.first + i - np) * all + row % all; };
+  auto at = [&](uint32_t i) { return i < np ? (uint64_t)a.slots * all + (uint64_t)i * a.requests * all + row : (uint64_t)(c.first + i - np) * all + within; };
+  float2 mine = make_float2(-INFINITY, -1.f);
+  if (lane < n) mine = *(const float2 *)(a.part + pairs + 2 * at(lane));
+  auto pair = [&](uint32_t i) { return i < 64 ? mine : *(const float2 *)(a.part + pairs + 2 * at(i)); };
   float M = -INFINITY;
   bool seen = false;
   for (uint32_t i = lane; i < n; i += 64) {
-    const float2 s = *(const float2 *)(a.part + pairs + 2 * at(i));
+    const float2 s = pair(i);
     if (!(s.y < 0.f)) { M = fmaxf(M, s.x); seen = true; }
   }
   M = wave_max(M);
   float sum = 0.f;
   for (uint32_t i = lane; i < n; i += 64) {
-    const float2 s = *(const float2 *)(a.part + pairs + 2 * at(i));
+    const float2 s = pair(i);
     // (a sum of 0 is a part without a finite score: it adds nothing, and its values may be NaN)
     const float f = s.y < 0.f || s.y == 0.f ? 0.f : s.x == M ? 1.f : exp2f(s.x - M);
     weight[wv][i] = f;
@@ -623,17 +713,41 @@ __global__ __launch_bounds__(256) void k_pages_join(PagesK a) {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
   const bool none = !__any(seen);
-  for (uint32_t d = lane; d < a.hd; d += 64) {
-    float acc = 0.f;
-    for (uint32_t i = 0; i < n; i++)
-      if (weight[wv][i] != 0.f) acc += a.part[at(i) * a.hd + d] * weight[wv][i];
-    a.y[row * a.hd + d] = none ? 0.f : acc / sum;
+  if constexpr (VEC) {
+    const uint32_t width = a.hd / 4, groups = width < 64 ? 64 / width : 1, per = 64 / groups, z0 = lane / per, d0 = lane % per;  // groups: a power of two
+    for (uint32_t d = 4 * d0; d < a.hd; d += 4 * per) {
+      f32x4 acc = {0, 0, 0, 0};
+      for (uint32_t i0 = z0; i0 < n; i0 += 4 * groups) {
+        f32x4 v[4];
+        float f[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+          const uint32_t i = i0 + e * groups;
+          f[e] = i < n ? weight[wv][i] : 0.f;
+          v[e] = *(const f32x4 *)(a.part + at(min(i, n - 1)) * a.hd + d);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++)
+          if (f[e] != 0.f) acc += v[e] * f[e];
+      }
+      for (uint32_t o = per; o < 64; o *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], o, 64);
+      if (z0 == 0) *(f32x4 *)(a.y + (uint64_t)row * a.hd + d) = none ? f32x4{0, 0, 0, 0} : f32x4{acc.x / sum, acc.y / sum, acc.z / sum, acc.w / sum};
+    }
+  } else {
+    for (uint32_t d = lane; d < a.hd; d += 64) {
+      float acc = 0.f;
+      for (uint32_t i = 0; i < n; i++)
+        if (weight[wv][i] != 0.f) acc += a.part[at(i) * a.hd + d] * weight[wv][i];
+      a.y[(uint64_t)row * a.hd + d] = none ? 0.f : acc / sum;
+    }
   }
 }
 
 // The kernels of a call. mfma: matrix products; HD: the head dim padded to 64, 128 or 256; rows: of a workgroup, blocks and pblocks how
 // many that makes of a request and of all of them together.
-struct PagesLaunch { bool mfma, staged, pstaged; uint32_t HD, T, rw, prw, rows, prows, blocks, pblocks, unit, least, target, slots, nprefix, per; };
+struct PagesLaunch { bool mfma, staged, pstaged; uint32_t HD, T, rw, prw, rows, prows, blocks, pblocks, unit, least, target, slots, nprefix, per; };  // unit: keys
 static PagesLaunch pages_launch(const PagesAttnArgs &in) {
   PagesLaunch p{};
   const uint32_t group = in.heads / in.kv_heads, cus = (uint32_t)device_cu_count(), nrows = in.tokens * group;
@@ -738,7 +852,8 @@ hipError_t attention_pages(hipStream_t s, const PagesAttnArgs &in) {
   a.heads = in.heads; a.kvh = in.kv_heads; a.group = in.heads / in.kv_heads; a.hd = in.hd; a.window = in.window; a.shift = in.shift;
   a.max_pages = in.max_pages; a.pages = in.pages; a.requests = in.requests; a.tokens = in.tokens;
   a.shared = p.nprefix ? in.shared : 0; a.owner = in.owner;
-  a.unit = p.unit; a.least = p.least; a.target = p.target; a.slots = p.slots; a.nprefix = p.nprefix; a.per = p.per;
+  a.unit = (uint32_t)__builtin_ctz(p.unit); a.least = p.least; a.slots = p.slots; a.nprefix = p.nprefix; a.per = p.per;
+  a.per_target = (float)((1.0 + 0x1p-20) / p.target);
   a.scale = in.scale;
   if (p.nprefix) {
     in.kv16 ? launch_pages<_Float16, true>(s, a, p) : launch_pages<float, true>(s, a, p);
@@ -748,7 +863,9 @@ hipError_t attention_pages(hipStream_t s, const PagesAttnArgs &in) {
   WGD_HIP(hipGetLastError());
   if (!pages_joins(in, p)) return hipSuccess;
   const uint64_t rows = (uint64_t)in.requests * in.tokens * in.heads;
-  hipLaunchKernelGGL(k_pages_join, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a);
+  const dim3 grid((uint32_t)((rows + 3) / 4));
+  if (in.hd >= 4 && (in.hd & (in.hd - 1)) == 0) hipLaunchKernelGGL(k_pages_join<true>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(k_pages_join<false>, grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -401,21 +401,18 @@ __device__ __forceinline__ void tree_split(const f32x4 (&p)[2], f16x8 &hi, f16x8
   lo = __builtin_bit_cast(f16x8, l);
 }
 
-// A row's query times scale log2 e as f16 operands hi and lo of KT steps of 32 dims, over the power of two returned,
-// which puts its largest magnitude into [2^14, 2^15). Zero past hd, and where ok is off.
+// A row's query (x: its dims 32 t + 8 g .. + 8) times f as f16 operands hi and lo of KT steps of 32 dims, over the power of two returned,
+// which puts its largest magnitude into [2^14, 2^15).
 template <uint32_t KT>
-__device__ __forceinline__ float tree_query(const float *q, uint32_t hd, float f, bool ok, u32x4 (&hi)[KT], u32x4 (&lo)[KT]) {
-  const uint32_t g = (threadIdx.x & 63) >> 4;
-  auto four = [&](uint32_t d) { return ok && d < hd ? *(const f32x4 *)(q + d) : f32x4{0, 0, 0, 0}; };
+__device__ __forceinline__ float tree_query_of(const f32x4 (&x)[2 * KT], float f, u32x4 (&hi)[KT], u32x4 (&lo)[KT]) {
   float v[KT][8];
   uint32_t mx = 0;
 #pragma unroll
   for (uint32_t t = 0; t < KT; t++) {
-    const f32x4 x = four(32 * t + 8 * g), y = four(32 * t + 8 * g + 4);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      v[t][e] = x[e] * f;
-      v[t][4 + e] = y[e] * f;
+      v[t][e] = x[2 * t][e] * f;
+      v[t][4 + e] = x[2 * t + 1][e] * f;
       mx = max(mx, max(__float_as_uint(v[t][e]) & 0x7FFFFFFFu, __float_as_uint(v[t][4 + e]) & 0x7FFFFFFFu));
     }
   }
@@ -433,6 +430,19 @@ __device__ __forceinline__ float tree_query(const float *q, uint32_t hd, float f
       lo[t][e] = l;
     }
   return __uint_as_float((ex - 14u) << 23);
+}
+// The same from memory. Zero past hd, and where ok is off.
+template <uint32_t KT>
+__device__ __forceinline__ float tree_query(const float *q, uint32_t hd, float f, bool ok, u32x4 (&hi)[KT], u32x4 (&lo)[KT]) {
+  const uint32_t g = (threadIdx.x & 63) >> 4;
+  auto four = [&](uint32_t d) { return ok && d < hd ? *(const f32x4 *)(q + d) : f32x4{0, 0, 0, 0}; };
+  f32x4 x[2 * KT];
+#pragma unroll
+  for (uint32_t t = 0; t < KT; t++) {
+    x[2 * t] = four(32 * t + 8 * g);
+    x[2 * t + 1] = four(32 * t + 8 * g + 4);
+  }
+  return tree_query_of<KT>(x, f, hi, lo);
 }
 
 // FULL: the head dim is HD itself.
