@@ -28,27 +28,27 @@ __host__ __device__ __forceinline__ uint64_t pages_part_rows(uint32_t slots, uin
 }
 __host__ __device__ __forceinline__ uint64_t pages_pairs(uint64_t part_rows, uint32_t hd) { return (part_rows * hd + 1) / 2 * 2; }
 
-// What lane-wide plans say of one request.
-struct PagesRequest { uint32_t len, n, lo; bool shares; };  // its keys start at lo where it shares nothing
-__device__ __forceinline__ PagesRequest pages_request(const PagesK &a, uint32_t r) {
+// What lane-wide plans say of one request: its keys start at lo where it shares nothing.
+struct PagesRequest { uint32_t len, n, lo; bool shares; };
+struct PagesRaw { int32_t len, count, page; };      // as they are in memory
+struct PagesOwner { uint32_t len; int32_t page; };  // of the prefix: its last page
+__device__ __forceinline__ PagesRaw pages_raw(const PagesK &a, uint32_t r) {
+  const uint32_t at = min(r, a.requests - 1);
+  return PagesRaw{a.lengths[at], a.counts ? a.counts[at] : (int32_t)a.tokens, a.shared ? a.table[(uint64_t)at * a.max_pages + (a.shared >> a.shift) - 1] : 0};
+}
+__device__ __forceinline__ PagesOwner pages_owner(const PagesK &a) {
+  if (!a.shared) return PagesOwner{0, 0};
+  return PagesOwner{min((uint32_t)max(a.lengths[a.owner], 0), a.max_pages << a.shift), a.table[(uint64_t)a.owner * a.max_pages + (a.shared >> a.shift) - 1]};
+}
+__device__ __forceinline__ PagesRequest pages_request(const PagesK &a, const PagesOwner &o, const PagesRaw &raw, uint32_t r) {
   PagesRequest q = {0, 0, 0, false};
-  const uint32_t at = min(r, a.requests - 1), cap = a.max_pages << a.shift;
-  // (all loads before any of them is waited for)
-  const int32_t len = a.lengths[at], count = a.counts ? a.counts[at] : (int32_t)a.tokens;
-  int32_t owner_len = 0, page = -1, owner_page = -2;
-  if (a.shared) {
-    const uint32_t c = (a.shared >> a.shift) - 1;
-    owner_len = a.lengths[a.owner];
-    page = a.table[(uint64_t)at * a.max_pages + c];
-    owner_page = a.table[(uint64_t)a.owner * a.max_pages + c];
-  }
   if (r >= a.requests) return q;
-  q.len = min((uint32_t)max(len, 0), cap);
-  q.n = min(q.len, (uint32_t)min(max(count, 0), (int32_t)a.tokens));
+  q.len = min((uint32_t)max(raw.len, 0), a.max_pages << a.shift);
+  q.n = min(q.len, (uint32_t)min(max(raw.count, 0), (int32_t)a.tokens));
   const uint32_t first = q.len - q.n + 1;  // keys up to the first query's own
   q.lo = first > a.window ? first - a.window : 0;
   if (a.shift >= 4) q.lo &= ~15u;  // whole halves of blocks, on the same page; nothing before the first key is read
-  q.shares = a.shared && min((uint32_t)max(owner_len, 0), cap) >= a.shared && q.n && q.len - q.n >= a.shared && q.len <= a.window && page == owner_page;
+  q.shares = a.shared && o.len >= a.shared && q.n && q.len - q.n >= a.shared && q.len <= a.window && raw.page == o.page;
   return q;
 }
 __device__ __forceinline__ uint32_t pages_units(const PagesK &a, const PagesRequest &q, bool sharing) {
@@ -67,22 +67,42 @@ __device__ __forceinline__ uint32_t pages_sums(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t pages_lane(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
 
-// The plan of all requests: whether a prefix is shared (by two or more), and the units of a chunk. `first` has the first 64 requests.
-struct PagesPlan { bool sharing; uint32_t chunk; PagesRequest first; };
+// The plan of all requests: whether a prefix is shared (by two or more), and the units of a chunk. The first 64 PAGES_HELD requests
+// are held in registers, their loads all under way at once; the others are loaded wherever they are asked for.
+constexpr uint32_t PAGES_HELD = 1;  // (two or four, 128 or 256 requests, made every workgroup's plan 1 us longer)
+struct PagesPlan { bool sharing; uint32_t chunk; PagesOwner owner; PagesRequest held[PAGES_HELD]; };
+// what(r0, requests r0 .. + 64) for all, as long as it returns false.
+template <class F> __device__ __forceinline__ void pages_each(const PagesK &a, const PagesPlan &p, F &&what) {
+  const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+  for (uint32_t e = 0; e < PAGES_HELD; e++) {
+    if (64 * e >= a.requests) return;
+    if (what(64 * e, p.held[e])) return;
+  }
+  for (uint32_t r0 = 64 * PAGES_HELD; r0 < a.requests; r0 += 64)
+    if (what(r0, pages_request(a, p.owner, pages_raw(a, r0 + lane), r0 + lane))) return;
+}
 __device__ __forceinline__ PagesPlan pages_plan(const PagesK &a) {
   const uint32_t lane = threadIdx.x & 63;
-  PagesPlan p = {false, 0, {0, 0, 0, false}};
+  PagesPlan p;
+  PagesRaw raw[PAGES_HELD];
+#pragma unroll
+  for (uint32_t e = 0; e < PAGES_HELD; e++)
+    if (e == 0 || 64 * e < a.requests) raw[e] = pages_raw(a, 64 * e + lane);
+  p.owner = pages_owner(a);
+#pragma unroll
+  for (uint32_t e = 0; e < PAGES_HELD; e++)
+    if (e == 0 || 64 * e < a.requests) p.held[e] = pages_request(a, p.owner, raw[e], 64 * e + lane);
   float alone = 0.f, apart = 0.f;  // units; below 2^-20 off, which per_target makes up for
   uint32_t sharers = 0;
-  for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
-    const PagesRequest q = pages_request(a, r0 + lane);
-    if (r0 == 0) p.first = q;
+  pages_each(a, p, [&](uint32_t, const PagesRequest &q) {
     alone += wave_total((float)pages_units(a, q, false));
     if (a.shared) {
       apart += wave_total((float)pages_units(a, q, true));
       sharers += (uint32_t)__popcll(__ballot(q.shares));
     }
-  }
+    return false;
+  });
   p.sharing = sharers > 1;
   // rounded up, so that there are no more chunks than wanted, and one for each request
   const float even = ceilf((p.sharing ? apart : alone) * a.per_target);
@@ -97,22 +117,25 @@ template <bool BY_REQUEST>
 __device__ __forceinline__ PagesChunks pages_chunks(const PagesK &a, const PagesPlan &plan, uint32_t find) {
   const uint32_t lane = threadIdx.x & 63;
   uint32_t before = 0;
-  for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
-    const PagesRequest q = r0 ? pages_request(a, r0 + lane) : plan.first;
+  PagesChunks c = {0xFFFFFFFFu, 0, 0, 0, 0, 0, false};
+  pages_each(a, plan, [&](uint32_t r0, const PagesRequest &q) {
     const uint32_t units = pages_units(a, q, plan.sharing);
     const uint32_t mine = r0 + lane < a.requests ? max(1u, (units + plan.chunk - 1) / plan.chunk) : 0;
     const uint32_t s = pages_sums(mine) + before;
-    const uint64_t here = __ballot(BY_REQUEST ? r0 + lane == find : find < s);  // the first of these
-    if (here && (BY_REQUEST || find < pages_lane(s, 63))) {
-      const uint32_t at = (uint32_t)__ffsll((unsigned long long)here) - 1;
-      const bool shares = plan.sharing && (__ballot(q.shares) >> at & 1);
-      const uint32_t count = pages_lane(mine, at);
-      return PagesChunks{r0 + at, pages_lane(s, at) - count, count, shares ? a.shared : pages_lane(q.lo, at), pages_lane(q.len, at),
-                         pages_lane(q.n, at), shares};
-    }
     before = pages_lane(s, 63);
-  }
-  return PagesChunks{0xFFFFFFFFu, 0, 0, 0, 0, 0, false};
+    const uint64_t here = __ballot(BY_REQUEST ? r0 + lane == find : find < s);  // the first of these
+    if (!here) return false;
+    const uint32_t at = (uint32_t)__ffsll((unsigned long long)here) - 1;
+    c.r = r0 + at;
+    c.count = pages_lane(mine, at);
+    c.first = pages_lane(s, at) - c.count;
+    c.shares = plan.sharing && (__ballot(q.shares) >> at & 1);
+    c.lo = c.shares ? a.shared : pages_lane(q.lo, at);
+    c.len = pages_lane(q.len, at);
+    c.n = pages_lane(q.n, at);
+    return true;
+  });
+  return c;
 }
 
 // A workgroup's part of the work: rows of kv head kv against the keys [lo, hi) of one row of the table. Row i of the part is
@@ -272,32 +295,34 @@ __device__ __forceinline__ void pages_any(const PagesK &a, float *lds, uint32_t 
   }
 }
 
-// The workgroup's part; false where it has none. PREFIX: blockIdx.y is a part of the prefix, else a slot. `list` has WGD_REQUESTS_MAX
+// The workgroup's part; false where it has none. PREFIX: (kv head, part) and the block of rows, else (kv head, block of rows) and a slot. `list` has WGD_REQUESTS_MAX
 // places in LDS. Queries that a request does not have get zeros here, from its first chunk's workgroups of `rows` rows each.
 template <bool PREFIX, uint32_t NT>
 __device__ __forceinline__ bool pages_part(const PagesK &a, uint32_t rows, uint16_t *list, PagesPart &p) {
   const PagesPlan plan = pages_plan(a);
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const uint64_t all = (uint64_t)a.tokens * a.heads;
+  // (row blocks of the prefix go last: a last one without rows would hold up others where they are dealt out)
   p.kv = blockIdx.x % a.kvh;
-  p.row0 = blockIdx.x / a.kvh * rows;
+  p.row0 = (PREFIX ? blockIdx.y : blockIdx.x / a.kvh) * rows;
   if constexpr (PREFIX) {
+    const uint32_t part = blockIdx.x / a.kvh;
     if (!plan.sharing) return false;
     uint32_t n = 0;
-    for (uint32_t r0 = 0; r0 < a.requests; r0 += 64) {
-      const bool shares = pages_request(a, r0 + lane).shares;
-      const uint64_t m = __ballot(shares);
-      if (tid < 64 && shares) list[n + (uint32_t)__popcll(m & ((1ull << lane) - 1))] = (uint16_t)(r0 + lane);
+    pages_each(a, plan, [&](uint32_t r0, const PagesRequest &q) {
+      const uint64_t m = __ballot(q.shares);
+      if (tid < 64 && q.shares) list[n + (uint32_t)__popcll(m & ((1ull << lane) - 1))] = (uint16_t)(r0 + lane);
       n += (uint32_t)__popcll(m);
-    }
+      return false;
+    });
     p.nrows = n * a.tokens * a.group;
-    p.lo = min(blockIdx.y * a.per, a.shared);
+    p.lo = min(part * a.per, a.shared);
     p.hi = min(p.lo + a.per, a.shared);
     p.r = a.owner; p.n = a.tokens; p.end0 = 0; p.seen = 0;
     p.table = a.table + (uint64_t)a.owner * a.max_pages;
     p.list = list;
     p.direct = false;
-    p.part = a.slots * all + (uint64_t)blockIdx.y * a.requests * all;
+    p.part = a.slots * all + (uint64_t)part * a.requests * all;
     if (p.row0 >= p.nrows) return false;
     __syncthreads();
     return true;
@@ -342,7 +367,7 @@ __global__ __launch_bounds__(256) void k_pages_any(PagesK a, uint32_t T) {
 // number, a scalar, for the lot.
 // A masked key's weight is exactly 0, but 0 times what is not finite is NaN, and the split operands turn infinities into it: a workgroup that
 // ends with anything not finite, or that has a page that is none, forms its rows again with pages_any.
-constexpr uint32_t PAGES_IDS = 1024;
+constexpr uint32_t PAGES_IDS = 1024, PAGES_WG = 256;
 
 // Which of the keys t0 .. + 32 (below hi) a row sees, as bits.
 __device__ __forceinline__ uint32_t pages_mask(uint32_t begin, uint32_t end, uint32_t t0) {
@@ -497,7 +522,17 @@ __device__ __forceinline__ void pages_end(const PagesK &a, uint32_t rw, float *l
       if (p.row0 + 16 * i < p.nrows) pages_any<E, NT>(a, lds, tree_any_tile(HD), p, p.row0 + 16 * i);
     return;
   }
-  // ---- to LDS: [row] max, sum; [row][HD]
+  // ---- to LDS: where the rows go (in floats; ~0: nowhere), and whether they see anything; [row] max, sum; [row][HD]
+  __shared__ uint64_t place[128];
+  __shared__ uint32_t sees_any[4];
+  const uint32_t rows = rw * RT * 16;
+  if (tid < 128) {
+    const PagesRow w = pages_row(a, p, p.row0 + tid);
+    const bool ok = tid < rows && w.valid;
+    place[tid] = ok ? (p.direct ? w.row : pages_at(a, p, w)) : ~0ull;
+    const uint64_t m = __ballot(ok && w.begin < p.hi && w.end > p.lo);
+    if (lane == 0) { sees_any[tid / 32] = (uint32_t)m; sees_any[tid / 32 + 1] = (uint32_t)(m >> 32); }
+  }
   float *mine = lds + (tid >> 6) * WS;
 #pragma unroll
   for (uint32_t rt = 0; rt < RT; rt++) {
@@ -523,10 +558,10 @@ __device__ __forceinline__ void pages_end(const PagesK &a, uint32_t rw, float *l
   __syncthreads();
   // ---- the slices in order, eight dims of a row per thread
   const uint64_t pairs = pages_pairs(pages_part_rows(a.slots, a.nprefix, a.requests, (uint64_t)a.tokens * a.heads), a.hd);
-  for (uint32_t i = tid; i < rw * RT * 16 * (HD / 8); i += NT) {
-    const uint32_t d = i % (HD / 8) * 8, lr = i / (HD / 8) % (RT * 16), rg = i / (HD / 8) / (RT * 16);
-    const PagesRow w = pages_row(a, p, p.row0 + rg * RT * 16 + lr);
-    if (!w.valid || d >= a.hd) continue;
+  for (uint32_t i = tid; i < rows * (HD / 8); i += NT) {
+    const uint32_t d = i % (HD / 8) * 8, at_row = i / (HD / 8), lr = at_row % (RT * 16), rg = at_row / (RT * 16);
+    const uint64_t go = place[at_row];
+    if (go == ~0ull || d >= a.hd) continue;
     float M = -INFINITY, l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (uint32_t u = 0; u < slices; u++) M = fmaxf(M, lds[(u * rw + rg) * WS + 2 * lr]);
     for (uint32_t u = 0; u < slices; u++) {
@@ -538,14 +573,10 @@ __device__ __forceinline__ void pages_end(const PagesK &a, uint32_t rw, float *l
 #pragma unroll
       for (int e = 0; e < 4; e++) { y[e] += x0[e] * f; y[4 + e] += x1[e] * f; }
     }
-    float *to = a.y + w.row * a.hd + d, inv = 1.f;
-    if (p.direct) {
-      inv = 1.f / l;  // (a row sees its own key at least)
-    } else {
-      const uint64_t at = pages_at(a, p, w);
-      to = a.part + at * a.hd + d;
-      if (d == 0) *(float2 *)(a.part + pairs + 2 * at) = make_float2(M - TREE_BIAS, w.begin < p.hi && w.end > p.lo ? l : -1.f);
-    }
+    float *to = (p.direct ? a.y : a.part) + go * a.hd + d;
+    const float inv = p.direct ? 1.f / l : 1.f;  // (a row sees its own key at least)
+    if (!p.direct && d == 0)
+      *(float2 *)(a.part + pairs + 2 * go) = make_float2(M - TREE_BIAS, sees_any[at_row / 32] >> (at_row % 32) & 1 ? l : -1.f);
 #pragma unroll
     for (int e = 0; e < 8; e += 4) *(f32x4 *)(to + e) = f32x4{y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv};
   }
@@ -566,8 +597,8 @@ __device__ __forceinline__ PagesSees pages_sees(const PagesRow &w) {
 }
 
 template <uint32_t HD, class E, bool FULL, bool PREFIX>
-__global__ __launch_bounds__((tree_threads<HD>())) void k_pages(PagesK a, uint32_t rw) {
-  constexpr uint32_t NT = tree_threads<HD>();
+__global__ __launch_bounds__(PAGES_WG, HD == 256 ? 1 : 2) void k_pages(PagesK a, uint32_t rw) {
+  constexpr uint32_t NT = PAGES_WG;
   typedef PagesWave<HD, E, FULL> Wave;
   extern __shared__ float lds[];
   __shared__ uint16_t list[PREFIX ? WGD_REQUESTS_MAX : 1];
@@ -591,12 +622,19 @@ __global__ __launch_bounds__((tree_threads<HD>())) void k_pages(PagesK a, uint32
   };
   bool none = numbers(p.lo);
   s.take_q(q, a.scale, a.hd, row.valid);
-  for (uint32_t k0 = p.lo; !none;) {
+  auto walk = [&](uint32_t k0) {
     if (wrow < p.nrows) s.walk(k0 + slice * Wave::KEYS, step, sees.begin, sees.end, sees.all_begin, sees.all_end);
-    k0 = s.hi;
-    if (k0 >= p.hi) break;
-    __syncthreads();
-    none = numbers(k0);
+  };
+  if constexpr (PREFIX) {  // (the numbers of a part fit, pages_launch())
+    if (!none) walk(p.lo);
+  } else {
+    for (uint32_t k0 = p.lo; !none;) {
+      walk(k0);
+      k0 = s.hi;
+      if (k0 >= p.hi) break;
+      __syncthreads();
+      none = numbers(k0);
+    }
   }
   pages_end<HD, E, 1, NT>(a, rw, lds, p, s, none);
 }
@@ -640,22 +678,32 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_pages_staged(PagesK a, uint3
   PagesSees sees[RT];
   Wave s;
   s.clear();
+  f32x4 q[RT][2 * Wave::KT];
+  bool valid[RT];
 #pragma unroll
   for (uint32_t rt = 0; rt < RT; rt++) {
     const PagesRow row = pages_row(a, p, wrow + 16 * rt + (tid & 15));
     sees[rt] = pages_sees(row);
-    s.qs[rt] = tree_query<Wave::KT>(a.q + row.row * HD, HD, a.scale * TREE_LOG2E, row.valid, s.qh[rt], s.ql[rt]);
+    valid[rt] = row.valid;
+#pragma unroll
+    for (uint32_t t = 0; t < 2 * Wave::KT; t++) q[rt][t] = *(const f32x4 *)(a.q + row.row * HD + 32 * (t / 2) + 8 * ((tid & 63) >> 4) + 4 * (t % 2));
   }
   uint32_t all_begin = 0, all_end = ~0u;
 #pragma unroll
   for (uint32_t rt = 0; rt < RT; rt++) { all_begin = max(all_begin, sees[rt].all_begin); all_end = min(all_end, sees[rt].all_end); }
-  bool none = false;
-  for (uint32_t k0 = p.lo; k0 < p.hi && !none; k0 = hi) {
-    if (k0 > p.lo) __syncthreads();  // the numbers and both stages are no longer read
+  auto numbers = [&](uint32_t k0) {
     first = k0 >> a.shift;
     hi = min((uint64_t)p.hi, (uint64_t)(first + PAGES_IDS) << a.shift);
-    none = pages_ids<NT>(a, p, ids, k0, hi);
-    if (none) break;
+    return pages_ids<NT>(a, p, ids, k0, hi);
+  };
+  bool none = numbers(p.lo);
+#pragma unroll
+  for (uint32_t rt = 0; rt < RT; rt++) {
+#pragma unroll
+    for (uint32_t t = 0; t < 2 * Wave::KT; t++) q[rt][t] = valid[rt] ? q[rt][t] : f32x4{0, 0, 0, 0};
+    s.qs[rt] = tree_query_of<Wave::KT>(q[rt], a.scale * TREE_LOG2E, s.qh[rt], s.ql[rt]);
+  }
+  auto walk = [&](uint32_t k0) {
     load(k0, 0);
     uint32_t stage = 0;
     for (uint32_t t0 = k0; t0 < hi; t0 += SK, stage ^= 1) {
@@ -669,6 +717,17 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_pages_staged(PagesK a, uint3
           s.block(K + 32 * b * ROW, V + 32 * b * ROW, t + 32 > min(hi, all_end) || t < all_begin,
                   [&](uint32_t rt) { return pages_mask(sees[rt].begin, min(sees[rt].end, hi), t); });
         }
+    }
+  };
+  if constexpr (PREFIX) {  // (the numbers of a part fit, pages_launch())
+    if (!none) walk(p.lo);
+  } else {
+    for (uint32_t k0 = p.lo; !none;) {
+      walk(k0);
+      k0 = hi;
+      if (k0 >= p.hi) break;
+      __syncthreads();  // the numbers and both stages are no longer read
+      none = numbers(k0);
     }
   }
   pages_end<HD, _Float16, RT, NT>(a, rw, lds, p, s, none);
@@ -767,25 +826,35 @@ static PagesLaunch pages_launch(const PagesAttnArgs &in) {
   };
   shape(nrows, p.staged, p.rw, p.rows);
   p.blocks = (nrows + p.rows - 1) / p.rows;
-  const uint32_t waves = p.staged || p.HD <= 128 ? 8 : 4;
   p.T = tree_any_tile(in.hd);
-  p.unit = !p.mfma ? p.T : (in.kv16 ? 32 : 16) * (waves / p.rw);
-  if (p.staged) p.unit = std::max(p.unit, 128u);
-  p.least = p.mfma ? 2 : 4;
+  // Chunks: about four workgroups a CU (two are there at a time), of one step of all wavefronts at least. us, 31 requests of 100 to 4000 keys,
+  // 32 heads on 8 of 128, f16, by workgroups wanted a CU: 1: 73, 2: 66, 3: 63, 4: 61, 8: 62; with workgroups of 512 threads 70 to 77, of 128 the
+  // same. Four requests of 40 to 500 f32 keys, 8 kv heads: chunks of one step 9.0, two 10.8, four 13.
+  p.unit = !p.mfma ? p.T : p.staged ? 128 : (in.kv16 ? 32 : 16) * (PAGES_WG / 64 / p.rw);
+  p.least = p.mfma ? 1 : 4;
   const uint32_t wgs = in.kv_heads * p.blocks;
-  p.target = std::max(1u, std::min((p.mfma ? 2 : 4) * cus / std::max(1u, wgs), PAGES_TARGET));
+  p.target = std::max(1u, std::min((p.staged ? 2 : 4) * cus / std::max(1u, wgs), PAGES_TARGET));
   // no request is cut where the longest is one chunk
   const uint64_t chunks = std::min<uint64_t>(p.target, (uint64_t)in.requests * ((longest + p.unit * p.least - 1) / (p.unit * p.least)));
   p.slots = (uint32_t)chunks + in.requests;
   if (in.shared && in.requests > 1) {
     shape(prows, p.pstaged, p.prw, p.prows);
     p.pblocks = (uint32_t)((prows + p.prows - 1) / p.prows);
-    const uint32_t pw = p.pstaged || p.HD <= 128 ? 8 : 4;
-    uint32_t unit = !p.mfma ? 4 * p.T : p.pstaged ? (p.HD == 256 ? 64 : 128) : (in.kv16 ? 32 : 16) * (pw / p.prw);
-    unit = std::max(unit, 1u << in.shift);
-    const uint32_t want = std::max(1u, std::min({(p.mfma ? 1 : 4) * cus / std::max(1u, in.kv_heads * p.pblocks), (in.shared + unit - 1) / unit, PAGES_PREFIX}));
-    p.per = ((in.shared + want - 1) / want + unit - 1) / unit * unit;
-    p.nprefix = (in.shared + p.per - 1) / p.per;
+    // Parts by estimated time, us: a workgroup starts and ends in 4.5 and works 2.1 (f16) or 3.1 (f32) for a block of each slice; a part is
+    // written and read once more. A last block of rows that may have few of them counts as none. 64 of 66 requests, 32 heads on 8 of 128, 8192
+    // keys: 4 parts 75, 8 49, 10 46, 16 36 us (as many workgroups as CUs), 32 73.
+    const uint32_t unit = std::max(!p.mfma ? p.T : p.pstaged ? 128 : (in.kv16 ? 32 : 16) * (PAGES_WG / 64 / p.prw), 1u << in.shift);
+    const uint32_t slices = p.pstaged ? 8 / p.prw : PAGES_WG / 64 / p.prw, block = in.kv16 ? 32 : 16;
+    const uint64_t wgs = in.kv_heads * std::max<uint64_t>(1, (prows + p.prows / 4) / p.prows);
+    const double held = (double)in.requests * in.tokens * in.heads * in.hd * 8 / 4e6;
+    double best = 1e30;
+    for (uint32_t n = 1; n <= PAGES_PREFIX && (uint64_t)(n - 1) * unit < in.shared; n++) {
+      const uint32_t per = ((in.shared + n - 1) / n + unit - 1) / unit * unit, parts = (in.shared + per - 1) / per;
+      if (parts < n || (p.mfma && per >> in.shift >= PAGES_IDS)) continue;  // (too many parts for that: computed apart)
+      const double work = p.mfma ? (in.kv16 ? 2.1 : 3.1) * ((per + block * slices - 1) / (block * slices)) : 0.5 * per;
+      const double t = (double)((wgs * n + (p.pstaged ? 1 : 2) * cus - 1) / ((p.pstaged ? 1 : 2) * cus)) * (4.5 + work) + held * n;
+      if (t < best) { best = t; p.per = per; p.nprefix = parts; }
+    }
   }
   return p;
 }
@@ -802,19 +871,22 @@ uint64_t attention_pages_scratch_floats(const PagesAttnArgs &in) {
   return pages_pairs(rows, in.hd) + 2 * rows;
 }
 
+template <bool PREFIX> static dim3 pages_grid(const PagesK &a, const PagesLaunch &p) {
+  return PREFIX ? dim3(a.kvh * p.nprefix, p.pblocks) : dim3(a.kvh * p.blocks, p.slots);
+}
 template <bool PREFIX, class E>
 static void launch_pages_any(hipStream_t s, const PagesK &a, const PagesLaunch &p) {
   const size_t lds = tree_any_lds(a.hd, p.T);
   if (lds > 50000) lds_opt_in_bytes((const void *)k_pages_any<E, PREFIX>, 100000);
-  hipLaunchKernelGGL((k_pages_any<E, PREFIX>), dim3(a.kvh * (PREFIX ? p.pblocks : p.blocks), PREFIX ? p.nprefix : p.slots), dim3(256), lds, s, a, p.T);
+  hipLaunchKernelGGL((k_pages_any<E, PREFIX>), pages_grid<PREFIX>(a, p), dim3(256), lds, s, a, p.T);
 }
 template <uint32_t HD, class E, bool FULL, bool PREFIX>
 static void launch_pages_direct(hipStream_t s, const PagesK &a, const PagesLaunch &p) {
-  constexpr uint32_t waves = tree_threads<HD>() / 64;
+  constexpr uint32_t waves = PAGES_WG / 64;
   constexpr size_t lds = std::max(tree_wave_lds<HD, 1>() * waves, tree_any_lds(HD, tree_any_tile(HD)));
   static_assert(lds + 4 * PAGES_IDS + 2 * WGD_REQUESTS_MAX + 1024 <= LDS_MAX, "the wavefronts' outputs fit LDS");
   lds_opt_in_bytes((const void *)k_pages<HD, E, FULL, PREFIX>, (uint32_t)lds);
-  hipLaunchKernelGGL((k_pages<HD, E, FULL, PREFIX>), dim3(a.kvh * (PREFIX ? p.pblocks : p.blocks), PREFIX ? p.nprefix : p.slots), dim3(64 * waves), lds, s,
+  hipLaunchKernelGGL((k_pages<HD, E, FULL, PREFIX>), pages_grid<PREFIX>(a, p), dim3(64 * waves), lds, s,
                      a, PREFIX ? p.prw : p.rw);
 }
 template <uint32_t HD, bool PREFIX>
@@ -823,7 +895,7 @@ static void launch_pages_staged(hipStream_t s, const PagesK &a, const PagesLaunc
   constexpr size_t lds = std::max({tree_wave_lds<HD, RT>() * waves, tree_any_lds(HD, tree_any_tile(HD)), (size_t)4 * SK * 2 * HD});
   static_assert(lds + 4 * PAGES_IDS + 2 * WGD_REQUESTS_MAX + 1024 <= LDS_MAX, "two stages, and the wavefronts' outputs, fit LDS");
   lds_opt_in_bytes((const void *)k_pages_staged<HD, RT, SK, PREFIX>, (uint32_t)lds);
-  hipLaunchKernelGGL((k_pages_staged<HD, RT, SK, PREFIX>), dim3(a.kvh * (PREFIX ? p.pblocks : p.blocks), PREFIX ? p.nprefix : p.slots), dim3(TREE_STAGED_NT),
+  hipLaunchKernelGGL((k_pages_staged<HD, RT, SK, PREFIX>), pages_grid<PREFIX>(a, p), dim3(TREE_STAGED_NT),
                      lds, s, a, PREFIX ? p.prw : p.rw);
 }
 template <uint32_t HD, class E, bool PREFIX>
