@@ -199,6 +199,10 @@ def test_pages_that_are_none_are_not_seen(gpu, up, kv):  # noqa: F811
         b.check(b.run(gpu, up, 0.1), 0.1)
         b.table[:, 19] = -1  # its last column
         b.check(b.run(gpu, up, 0.1), 0.1)
+    # a column of the prefix that is none in tables that have nothing else in common
+    b = Batch(rng, 8, 2, 128, 16, [330, 323], kv=kv)
+    b.table[:, 19] = -1
+    b.check(b.run(gpu, up, 0.1, shared=320), 0.1)
 
 
 def test_lengths_beyond_the_table_count_as_its_end(gpu, up):  # noqa: F811
@@ -239,6 +243,29 @@ def test_offsets_pass_32_bits(gpu, up):  # noqa: F811
             b.check(read(gpu, y, b.q.shape, np.float32), 0.1)
     finally:
         gpu.destroy(big)
+
+
+@pytest.mark.parametrize("tokens", [1360, 1400])
+def test_millions_of_rows_of_one_kv_head(gpu, up, tokens):  # noqa: F811
+    """Rows of a shared prefix up to what a launch takes (65535 blocks of 64) and beyond. Zero queries weigh all their keys alike: with V 0 in
+    the prefix and r + 1 in the request's own tokens, query t of request r gives (t + 1) (r + 1) / (16 + t + 1)."""
+    R, heads, hd, page = 1024, 3, 8, 16
+    own = ref.held(tokens, page)
+    pages = 1 + R * own
+    table = np.concatenate([np.zeros((R, 1)), 1 + np.arange(R * own).reshape(R, own)], 1).astype(np.int32)
+    v = np.repeat(np.concatenate([[0], 1 + np.arange(R * own) // own]), page * hd).astype(np.float32)
+    q, y = gpu.buffer(R * tokens * heads * hd * 4), gpu.buffer(R * tokens * heads * hd * 4)
+    try:
+        gpu.attention_pages(q, up(np.zeros_like(v)), up(v), y, up(table), up(np.full(R, 16 + tokens, np.int32)), heads, 1, hd, 0.3, NO_WINDOW, page,
+                            own + 1, pages, R, tokens, shared=16)
+        got = read(gpu, y, (R, tokens, heads * hd), np.float32)
+    finally:
+        gpu.destroy(q)
+        gpu.destroy(y)
+    t, r = np.arange(tokens)[None] + 1.0, np.arange(R)[:, None] + 1.0
+    want = t * r / (16 + t)
+    # equal weights: their sums are whole numbers in f32, the products and the quotient round
+    assert np.abs(got - want[..., None]).max() <= (tokens + 16 + 8) * EPS * R
 
 
 def test_many_requests_repeat_themselves_and_two_contexts_agree(gpu, up):  # noqa: F811

@@ -48,7 +48,7 @@ __device__ __forceinline__ PagesRequest pages_request(const PagesK &a, const Pag
   const uint32_t first = q.len - q.n + 1;  // keys up to the first query's own
   q.lo = first > a.window ? first - a.window : 0;
   if (a.shift >= 4) q.lo &= ~15u;  // whole halves of blocks, on the same page; nothing before the first key is read
-  q.shares = a.shared && o.len >= a.shared && q.n && q.len - q.n >= a.shared && q.len <= a.window && raw.page == o.page;
+  q.shares = a.shared && o.len >= a.shared && q.n && q.len - q.n >= a.shared && q.len <= a.window && raw.page == o.page && o.page >= 0 && (uint32_t)o.page < a.pages;
   return q;
 }
 __device__ __forceinline__ uint32_t pages_units(const PagesK &a, const PagesRequest &q, bool sharing) {
@@ -93,7 +93,7 @@ __device__ __forceinline__ PagesPlan pages_plan(const PagesK &a) {
 #pragma unroll
   for (uint32_t e = 0; e < PAGES_HELD; e++)
     if (e == 0 || 64 * e < a.requests) p.held[e] = pages_request(a, p.owner, raw[e], 64 * e + lane);
-  float alone = 0.f, apart = 0.f;  // units; below 2^-20 off, which per_target makes up for
+  float alone = 0.f, apart = 0.f;  // units; below 2^-19 off, which per_target makes up for
   uint32_t sharers = 0;
   pages_each(a, p, [&](uint32_t, const PagesRequest &q) {
     alone += wave_total((float)pages_units(a, q, false));
@@ -148,12 +148,14 @@ struct PagesPart {
   bool direct;               // the only part of its rows: to y
   uint64_t part;             // else the first row of its part
 };
-// i / d by its reciprocal, for i < 2^25.
+// i / d by its reciprocal, for i <= 2^25 and d <= 2^20: the first estimate is off by 2^25 2^-22 at most, the second by one.
 __device__ __forceinline__ uint32_t pages_div(uint32_t i, uint32_t d) {
   if (d == 1) return i;
-  uint32_t q = (uint32_t)((float)i * __builtin_amdgcn_rcpf((float)d));
-  q -= q * d > i;
-  return q + ((q + 1) * d <= i);
+  const float inv = __builtin_amdgcn_rcpf((float)d);
+  uint32_t q = (uint32_t)((float)i * inv);
+  q += (uint32_t)(int32_t)floorf((float)(int32_t)(i - q * d) * inv);
+  q -= (int32_t)(i - q * d) < 0;
+  return q + ((int32_t)(i - q * d) >= (int32_t)d);
 }
 struct PagesRow { bool valid; uint64_t row; uint32_t request, query, begin, end; };  // row of q and y; keys [begin, end)
 __device__ __forceinline__ PagesRow pages_row(const PagesK &a, const PagesPart &p, uint32_t i) {
@@ -187,7 +189,6 @@ __device__ __forceinline__ uint64_t pages_at(const PagesK &a, const PagesPart &p
 template <class E, uint32_t NT>
 __device__ __forceinline__ void pages_any(const PagesK &a, float *lds, uint32_t T, const PagesPart &p, uint32_t r0) {
   __shared__ uint64_t vis[TREE_R];
-  __shared__ uint32_t there[2];
   __shared__ float mrow[TREE_R], lrow[TREE_R], corr[TREE_R];
   __shared__ uint32_t any[TREE_R];
   const uint32_t hd = a.hd, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, pg = (1u << a.shift) - 1;
@@ -833,7 +834,7 @@ static PagesLaunch pages_launch(const PagesAttnArgs &in) {
   p.unit = !p.mfma ? p.T : p.staged ? 128 : (in.kv16 ? 32 : 16) * (PAGES_WG / 64 / p.rw);
   p.least = p.mfma ? 1 : 4;
   const uint32_t wgs = in.kv_heads * p.blocks;
-  p.target = std::max(1u, std::min((p.staged ? 2 : 4) * cus / std::max(1u, wgs), PAGES_TARGET));
+  p.target = std::max(1u, std::min((p.staged || p.HD == 256 ? 2 : 4) * cus / std::max(1u, wgs), PAGES_TARGET));
   // no request is cut where the longest is one chunk
   const uint64_t chunks = std::min<uint64_t>(p.target, (uint64_t)in.requests * ((longest + p.unit * p.least - 1) / (p.unit * p.least)));
   p.slots = (uint32_t)chunks + in.requests;
@@ -848,7 +849,8 @@ static PagesLaunch pages_launch(const PagesAttnArgs &in) {
     const uint64_t wgs = in.kv_heads * std::max<uint64_t>(1, (prows + p.prows / 4) / p.prows);
     const double held = (double)in.requests * in.tokens * in.heads * in.hd * 8 / 4e6;
     double best = 1e30;
-    for (uint32_t n = 1; n <= PAGES_PREFIX && (uint64_t)(n - 1) * unit < in.shared; n++) {
+    // (a launch has at most 65535 blocks of rows along y)
+    for (uint32_t n = 1; p.pblocks <= 65535 && n <= PAGES_PREFIX && (uint64_t)(n - 1) * unit < in.shared; n++) {
       const uint32_t per = ((in.shared + n - 1) / n + unit - 1) / unit * unit, parts = (in.shared + per - 1) / per;
       if (parts < n || (p.mfma && per >> in.shift >= PAGES_IDS)) continue;  // (too many parts for that: computed apart)
       const double work = p.mfma ? (in.kv16 ? 2.1 : 3.1) * ((per + block * slices - 1) / (block * slices)) : 0.5 * per;
@@ -925,7 +927,7 @@ hipError_t attention_pages(hipStream_t s, const PagesAttnArgs &in) {
   a.max_pages = in.max_pages; a.pages = in.pages; a.requests = in.requests; a.tokens = in.tokens;
   a.shared = p.nprefix ? in.shared : 0; a.owner = in.owner;
   a.unit = (uint32_t)__builtin_ctz(p.unit); a.least = p.least; a.slots = p.slots; a.nprefix = p.nprefix; a.per = p.per;
-  a.per_target = (float)((1.0 + 0x1p-20) / p.target);
+  a.per_target = (float)((1.0 + 0x1p-18) / p.target);
   a.scale = in.scale;
   if (p.nprefix) {
     in.kv16 ? launch_pages<_Float16, true>(s, a, p) : launch_pages<float, true>(s, a, p);
