@@ -362,7 +362,11 @@ int wgd_attention_pages(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer 
                         uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale, uint32_t window, uint32_t page,
                         uint32_t max_pages, uint32_t pages, uint32_t requests, uint32_t tokens, uint32_t shared,
                         uint32_t owner);
-/* The same over pools of halves. */
+/* The same over pools of halves. Scores, maxima, sums and outputs are f32; with a head_dim that is a multiple of 8, up to 256,
+ * queries and weights enter the products as two f16 each: an entry of a query is off by 2^-22 of itself and 2^-39 of its row's largest, a weight
+ * by 2^-22 of itself and 2^-36 of the largest one. Both forms: rows that see a value that is not finite, or a page that is none, have those that
+ * share a workgroup with them formed again one product at a time, some hundred times slower; so are head_dims that
+ * are no multiple of 8 or above 256. */
 int wgd_attention_pages_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_buffer *k_pool, const wgd_buffer *v_pool,
                               wgd_buffer *y, const wgd_buffer *table, const wgd_buffer *lengths, const wgd_buffer *counts,
                               uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale, uint32_t window,
@@ -374,7 +378,8 @@ int wgd_attention_pages_f16kv(wgd_context *ctx, const wgd_buffer *q, const wgd_b
  * rows with w outside [0, adapters) stay as they are, as does what lies around them. a is [adapters][rank][cols] and b
  * [adapters][rows][rank], both F32 or F16 (`type`; GGUF's lora_a and lora_b as they are), lower ranks filled up with zeros;
  * scales f32[adapters] (alpha / rank). Sums are f32, and products too with F32 weights; with F16 ones x and the inner sums enter
- * them as two f16 each: an entry is off by 2^-22 of itself and 2^-39 of its row's largest (64 inner sums at a time), and an infinity beside a weight may become NaN. rank <= 1024, cols and rows < 2^31, batch <= 2^24. */
+ * them as two f16 each: an entry is off by 2^-22 of itself and 2^-39 of its row's largest
+ * (64 inner sums at a time), and an infinity beside a weight may become NaN. rank <= 1024, cols and rows < 2^31, batch <= 2^24. */
 int wgd_adapters(wgd_context *ctx, int32_t type, const wgd_buffer *a, const wgd_buffer *b, const wgd_buffer *which,
                  const wgd_buffer *scales, const wgd_buffer *x, wgd_buffer *y, uint32_t cols, uint32_t rows, uint32_t rank,
                  uint32_t adapters, uint32_t stride, uint32_t row_base, uint32_t batch);

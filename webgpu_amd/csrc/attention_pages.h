@@ -368,6 +368,10 @@ __global__ __launch_bounds__(256) void k_pages_any(PagesK a, uint32_t T) {
 // number, a scalar, for the lot.
 // A masked key's weight is exactly 0, but 0 times what is not finite is NaN, and the split operands turn infinities into it: a workgroup that
 // ends with anything not finite, or that has a page that is none, forms its rows again with pages_any.
+// What bounds k_pages: long caches, the bytes of the keys and values. 31 requests of 100 to 4000 keys, 32 heads on 8 of 128, f16 (271 MB): 61 us,
+// 4.4 TB/s where a large copy has 4.8; 46% of a wavefront's life waits for loads, matrix products are at work for 6% of the cycles. Short
+// ones, latency: 9 us for four requests of 40 to 500 f32 keys. A workgroup there has the plan for 2.8 us (lengths, then the sums over lanes), the
+// page numbers for 1.1, and ends in 2.9.
 constexpr uint32_t PAGES_IDS = 1024, PAGES_WG = 256;
 
 // Which of the keys t0 .. + 32 (below hi) a row sees, as bits.
@@ -641,7 +645,10 @@ __global__ __launch_bounds__(PAGES_WG, HD == 256 ? 1 : 2) void k_pages(PagesK a,
 }
 
 // ------------------------------------------------------------------ many rows over halves: keys staged in LDS
-// As k_attn_tree_staged: eight wavefronts load stages of SK keys into LDS while they work on the one before.
+// As k_attn_tree_staged: eight wavefronts load stages of SK keys into LDS while they work on the one before. For 128 rows of a kv head
+// and more, whose workgroups would each read all keys again. What bounds it: a prefix of 8192 keys under 64 requests, 32 heads on 8 of 128, takes
+// 36 us, 480 TFLOP/s with both products of the split operands; a workgroup's stage of 128 keys takes 4.4 us (a third of it matrix products, then the
+// weights and their split, LDS, the barrier), what comes before its first stage 10 and the end 7.
 template <uint32_t HD, uint32_t RT, uint32_t SK, bool PREFIX>
 __global__ __launch_bounds__(TREE_STAGED_NT) void k_pages_staged(PagesK a, uint32_t rw) {
   typedef TreeStaged<HD, RT> Wave;
@@ -736,7 +743,8 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_pages_staged(PagesK a, uint3
 
 // ------------------------------------------------------------------ the parts of a row
 // A wavefront per row: the weights of its parts go over the lanes and LDS, then lane groups of hd / 4 (VEC: hd a power of two from 4) take every
-// (64 / group)-th part, 16 bytes a lane and four loads ahead.
+// (64 / group)-th part, 16 bytes a lane and four loads ahead. Bound by latency: the plan, the pairs, the values. 4.3 us for 64 rows of 128 and for 1024,
+// 7.9 for 2112 with 16 to 20 parts each.
 constexpr uint32_t PAGES_TARGET = 512, PAGES_PREFIX = 256, PAGES_PARTS = PAGES_TARGET + 1 + PAGES_PREFIX;
 template <bool VEC>
 __global__ __launch_bounds__(256) void k_pages_join(PagesK a) {
@@ -834,7 +842,13 @@ static PagesLaunch pages_launch(const PagesAttnArgs &in) {
   p.unit = !p.mfma ? p.T : p.staged ? 128 : (in.kv16 ? 32 : 16) * (PAGES_WG / 64 / p.rw);
   p.least = p.mfma ? 1 : 4;
   const uint32_t wgs = in.kv_heads * p.blocks;
-  p.target = std::max(1u, std::min((p.staged || p.HD == 256 ? 2 : 4) * cus / std::max(1u, wgs), PAGES_TARGET));
+  // Staged workgroups have a CU to themselves: all of them at once where the requests are few enough for that (every one rounds its
+  // chunks up, by half of one on average). us, times as many as CUs in all, 1: 2: the rule; 32 heads on 8 of 128, 128 tokens of 1 request, 4000 keys,
+  // 36, 51, 36; 4 requests of up to 4000 77, 77, 68; 64 tokens of 8 of up to 8000 142, 140, 116. 128 of 16 of up to 2000 131, 127, 127.
+  const uint32_t at_once = cus / std::max(1u, wgs);
+  if (p.staged) p.target = in.requests <= at_once ? at_once - in.requests / 2 : 2 * cus / std::max(1u, wgs);
+  else p.target = (p.HD == 256 ? 2 : 4) * cus / std::max(1u, wgs);
+  p.target = std::max(1u, std::min(p.target, PAGES_TARGET));
   // no request is cut where the longest is one chunk
   const uint64_t chunks = std::min<uint64_t>(p.target, (uint64_t)in.requests * ((longest + p.unit * p.least - 1) / (p.unit * p.least)));
   p.slots = (uint32_t)chunks + in.requests;

@@ -68,7 +68,7 @@ __device__ __forceinline__ uint32_t pages_free(const int32_t *refs, uint32_t pag
 
 // ------------------------------------------------------------------ places for new tokens
 // A thread per request: what it needs, the sum before it; then the free pages go to the requests in order, a thread per
-// 16 pages. Where pages run short one thread goes through the requests. 
+// 16 pages. Where pages run short one thread goes through the requests. 6.7 us for 4 tokens of 8 requests and 700 pages, 8.7 for 512 tokens of each.
 struct ExtendLds { uint32_t scan[PAGES_NT / 64 + 1]; uint32_t start[PAGES_NT + 1]; int32_t len[PAGES_NT], added[PAGES_NT]; };
 
 __device__ __forceinline__ void extend_place(const PagesExtendArgs &a, uint32_t i, int32_t before, int32_t added) {
@@ -163,6 +163,7 @@ hipError_t pages_extend(hipStream_t s, const PagesExtendArgs &a) {
 // Three steps over the rows that change, an element of the table per thread: their old pages are let go, the full pages
 // of their new rows held, and the new rows set down in scratch; then the last pages that are not full are given to one
 // row each, or copied; then the new rows go to the table. Without enough pages the last step takes the first one back.
+// 6.5 us in one launch for 8 requests of 64 pages; in three 3.6 + 6.8 + 2.5 for 64 requests of 256.
 struct ForkRow { bool changed; uint32_t from, held, kept; };  // pages that the row held; tokens that it keeps
 
 __device__ __forceinline__ uint32_t fork_length(const PagesForkArgs &a, uint32_t r) {
@@ -298,7 +299,8 @@ hipError_t pages_fork(hipStream_t s, const PagesForkArgs &in) {
 // ------------------------------------------------------------------ compaction
 // With `used` pages in use, the free ones below `used` are as many as the used ones from there on: the j-th of
 // these moves to the j-th of those. One workgroup goes through the pages twice, to count and to pair; a hole comes before
-// the page that moves there, so its number is listed when it is asked for.
+// the page that moves there, so its number is listed when it is asked for. 7.8 us for 128 pages, 13.9 for 4000: loads, scans,
+// and 16 pages a thread one after another.
 struct CompactLds { uint32_t scan[PAGES_NT / 64 + 1]; };
 __global__ __launch_bounds__(PAGES_NT) void k_pages_compact(PagesCompactArgs a) {
   __shared__ CompactLds L;
@@ -356,6 +358,8 @@ hipError_t pages_compact(hipStream_t s, const PagesCompactArgs &a) {
 }
 
 // ------------------------------------------------------------------ pages from place to place
+// A workgroup has 256 COPY_AHEAD units of a page, every gridDim.y-th pair and one pool; its loads go ahead of its stores. Bound by the
+// bytes: 1000 moves of 64 KB in two pools, 262 MB read and written, 53 us (4.9 TB/s).
 constexpr uint32_t COPY_POOLS = 64, COPY_AHEAD = 4;
 struct CopyPools { void *p[COPY_POOLS]; };
 typedef uint32_t copy16 __attribute__((ext_vector_type(4)));
@@ -401,7 +405,7 @@ hipError_t pages_copy(hipStream_t s, void *const *pools, uint32_t count, const i
 
 // ------------------------------------------------------------------ K/V rows into their slots
 // A row has `per` threads (a power of two), so that short rows share a workgroup. VEC: four elements a thread, where rows,
-// strides and offsets are whole multiples of four.
+// strides and offsets are whole multiples of four. Bound by the bytes: 2400 rows of 1024 f32 values of K and V each into halves, 30 MB, 7.5 us.
 template <class E, bool VEC>
 __global__ __launch_bounds__(256) void k_pages_store(PagesStoreArgs a, uint32_t per) {
   constexpr uint32_t W = VEC ? 4 : 1;
