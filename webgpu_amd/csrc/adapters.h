@@ -10,7 +10,7 @@
 // The order of the sums depends on the sizes alone.
 // What bounds it: few rows, the latency of two launches, each of loads that depend on which[] (4 rows of rank 8, 1024 x 2048: 3.7 and 5.0 us;
 // 64 rows of 24 adapters of rank 16, 4096 x 14336, 12 MB of weights: 5.9 and 8.6). Many rows, the bytes of x and y: 1536 rows of rank 64, 4096 x
-// 4096: down 14.2 (25 MB), up 17.7 (50 MB), where half of a wavefront's life waits for loads.
+// 4096: down 14.2 (25 MB), up 17.7 (50 MB), where two thirds of a wavefront's life wait for loads.
 #pragma once
 
 namespace wgd {

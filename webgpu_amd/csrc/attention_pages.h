@@ -647,7 +647,7 @@ __global__ __launch_bounds__(PAGES_WG, HD == 256 ? 1 : 2) void k_pages(PagesK a,
 // ------------------------------------------------------------------ many rows over halves: keys staged in LDS
 // As k_attn_tree_staged: eight wavefronts load stages of SK keys into LDS while they work on the one before. For 128 rows of a kv head
 // and more, whose workgroups would each read all keys again. What bounds it: a prefix of 8192 keys under 64 requests, 32 heads on 8 of 128, takes
-// 36 us, 480 TFLOP/s with both products of the split operands; a workgroup's stage of 128 keys takes 4.4 us (a third of it matrix products, then the
+// 36 us, 480 TFLOP/s with both products of the split operands; a workgroup's stage of 128 keys takes 4.4 us (two fifths of it matrix products, then the
 // weights and their split, LDS, the barrier), what comes before its first stage 10 and the end 7.
 template <uint32_t HD, uint32_t RT, uint32_t SK, bool PREFIX>
 __global__ __launch_bounds__(TREE_STAGED_NT) void k_pages_staged(PagesK a, uint32_t rw) {
