@@ -162,6 +162,16 @@ def test_compact(gpu, up, R, width, pages, used, inplace):
     assert read(gpu, moved, pages + 1)[-1] == 77 and np.all(read(gpu, copies, pages // 2 * 2 + 3)[-2:] == 77)
 
 
+@pytest.mark.parametrize("pages", [1024, 1025, 2050, 4095, 4096, 4097, 5001])
+def test_pools_around_the_pages_of_a_thread(gpu, up, pages):
+    """A thread has one page of a pool, four or sixteen: pools at and beside where that changes."""
+    for used in (pages // 2, pages - 1):
+        for inplace in (False, True):
+            test_compact(gpu, up, 8, 200, pages, used, inplace)
+    test_extend(gpu, up, (6, 1000, 1, pages), 0)
+    test_fork(gpu, up, (6, 900, 2, pages), 0)
+
+
 @pytest.mark.parametrize("pools,pages,bytes_,n", [(1, 2, 2, 1), (3, 9, 6, 4), (2, 40, 4100, 17), (130, 12, 64, 5), (2, 300, 32768, 130),
                                                   (1, 5, 50002, 2), (1, 6000, 16, 3000)])
 def test_copy(gpu, up, pools, pages, bytes_, n):

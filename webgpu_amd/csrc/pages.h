@@ -35,18 +35,22 @@ __device__ __forceinline__ uint32_t pages_scan(uint32_t v, uint32_t *lds, uint32
   return before + s - v;
 }
 
-// Which of the 16 pages p0 .. have `test`, as bits.
-template <class F> __device__ __forceinline__ uint32_t pages_bits(const int32_t *refs, uint32_t pages, uint32_t p0, F &&test) {
+// Pages of a thread at a time: 1, 4 or 16, so that all threads have some; a thread goes through its own one after another.
+__device__ __forceinline__ uint32_t pages_per(uint32_t pages) { return pages <= PAGES_NT ? 1 : pages <= 4 * PAGES_NT ? 4 : 16; }
+// Which of the `per` pages p0 .. have `test`, as bits.
+template <class F> __device__ __forceinline__ uint32_t pages_bits(const int32_t *refs, uint32_t pages, uint32_t p0, uint32_t per, F &&test) {
+  auto four = [&](uint32_t e) {
+    const int4 v = *(const int4 *)(refs + p0 + e);
+    return ((test(v.x) ? 1u : 0u) | (test(v.y) ? 2u : 0u) | (test(v.z) ? 4u : 0u) | (test(v.w) ? 8u : 0u)) << e;
+  };
   uint32_t m = 0;
-  if (p0 + 16 <= pages) {
+  if (per == 16 && p0 + 16 <= pages) {
 #pragma unroll
-    for (uint32_t e = 0; e < 16; e += 4) {
-      const int4 v = *(const int4 *)(refs + p0 + e);
-      m |= (test(p0 + e, v.x) ? 1u : 0u) << e | (test(p0 + e + 1, v.y) ? 2u : 0u) << e | (test(p0 + e + 2, v.z) ? 4u : 0u) << e |
-           (test(p0 + e + 3, v.w) ? 8u : 0u) << e;
-    }
+    for (uint32_t e = 0; e < 16; e += 4) m |= four(e);
+  } else if (per == 4 && p0 + 4 <= pages) {
+    m = four(0);
   } else {
-    for (uint32_t e = 0; p0 + e < pages; e++) m |= (test(p0 + e, refs[p0 + e]) ? 1u : 0u) << e;
+    for (uint32_t e = 0; e < per && p0 + e < pages; e++) m |= (test(refs[p0 + e]) ? 1u : 0u) << e;
   }
   return m;
 }
@@ -56,19 +60,20 @@ template <class F> __device__ __forceinline__ uint32_t pages_bits(const int32_t 
 template <bool GIVE, class F>
 __device__ __forceinline__ uint32_t pages_free(const int32_t *refs, uint32_t pages, uint32_t want, uint32_t *lds, F &&give) {
   uint32_t found = 0;
-  for (uint32_t base = 0; base < pages && found < want; base += 16 * PAGES_NT) {
-    uint32_t m = pages_bits(refs, pages, base + 16 * threadIdx.x, [](uint32_t, int32_t n) { return n <= 0; }), total;
+  const uint32_t per = pages_per(pages);
+  for (uint32_t base = 0; base < pages && found < want; base += per * PAGES_NT) {
+    const uint32_t p0 = base + per * threadIdx.x;
+    uint32_t m = pages_bits(refs, pages, p0, per, [](int32_t n) { return n <= 0; }), total;
     uint32_t rank = found + pages_scan(__popc(m), lds, total);
     if constexpr (GIVE)
-      for (; m && rank < want; m &= m - 1, rank++) give(rank, base + 16 * threadIdx.x + __ffs(m) - 1);
+      for (; m && rank < want; m &= m - 1, rank++) give(rank, p0 + __ffs(m) - 1);
     found += total;
   }
   return min(found, want);
 }
 
 // ------------------------------------------------------------------ places for new tokens
-// A thread per request: what it needs, the sum before it; then the free pages go to the requests in order, a thread per
-// 16 pages. Where pages run short one thread goes through the requests. 6.7 us for 4 tokens of 8 requests and 700 pages, 8.7 for 512 tokens of each.
+// A thread per request: what it needs, the sum before it; then the free pages go to the requests in order. Where pages run short one thread goes through the requests. 4.6 us for 4 tokens of 8 requests and 700 pages, 7.0 for 512 tokens of each.
 struct ExtendLds { uint32_t scan[PAGES_NT / 64 + 1]; uint32_t start[PAGES_NT + 1]; int32_t len[PAGES_NT], added[PAGES_NT]; };
 
 __device__ __forceinline__ void extend_place(const PagesExtendArgs &a, uint32_t i, int32_t before, int32_t added) {
@@ -299,23 +304,25 @@ hipError_t pages_fork(hipStream_t s, const PagesForkArgs &in) {
 // ------------------------------------------------------------------ compaction
 // With `used` pages in use, the free ones below `used` are as many as the used ones from there on: the j-th of
 // these moves to the j-th of those. One workgroup goes through the pages twice, to count and to pair; a hole comes before
-// the page that moves there, so its number is listed when it is asked for. 7.8 us for 128 pages, 13.9 for 4000: loads, scans,
-// and 16 pages a thread one after another.
+// the page that moves there, so its number is listed when it is asked for. 3.4 us for 128 pages, 8.1 for 4000: loads, scans,
+// and four pages a thread one after another (16: 7.8 and 13.9).
 struct CompactLds { uint32_t scan[PAGES_NT / 64 + 1]; };
 __global__ __launch_bounds__(PAGES_NT) void k_pages_compact(PagesCompactArgs a) {
   __shared__ CompactLds L;
-  const uint32_t tid = threadIdx.x;
-  uint32_t used = 0, total;
-  for (uint32_t p0 = 16 * tid; p0 < a.pages; p0 += 16 * PAGES_NT)
-    used += __popc(pages_bits(a.refs, a.pages, p0, [](uint32_t, int32_t n) { return n > 0; }));
+  const uint32_t tid = threadIdx.x, per = pages_per(a.pages);
+  auto bits = [&](uint32_t p0) { return p0 < a.pages ? pages_bits(a.refs, a.pages, p0, per, [](int32_t n) { return n > 0; }) : 0; };
+  uint32_t total;
+  const uint32_t on0 = bits(per * tid);  // (they are read once where that is all)
+  uint32_t used = __popc(on0);
+  for (uint32_t p0 = per * (tid + PAGES_NT); p0 < a.pages; p0 += per * PAGES_NT) used += __popc(bits(p0));
   pages_scan(used, L.scan, total);
   used = total;
   uint32_t holes = 0, moves = 0;
-  for (uint32_t base = 0; base < a.pages; base += 16 * PAGES_NT) {
-    const uint32_t p0 = base + 16 * tid, n = p0 < a.pages ? min(16u, a.pages - p0) : 0;
-    const uint32_t on = n ? pages_bits(a.refs, a.pages, p0, [](uint32_t, int32_t c) { return c > 0; }) : 0;
-    const uint32_t low = used > p0 ? (used - p0 >= 16 ? 0xFFFFu : (1u << (used - p0)) - 1) : 0, all = (1u << n) - 1;
-    uint32_t hole = ~on & all & low, move = on & ~low;
+  for (uint32_t base = 0; base < a.pages; base += per * PAGES_NT) {
+    const uint32_t p0 = base + per * tid, n = p0 < a.pages ? min(per, a.pages - p0) : 0;
+    const uint32_t on = base ? bits(p0) : on0;
+    const uint32_t low = used > p0 ? (1u << min(used - p0, n)) - 1 : 0;  // of those that are there
+    uint32_t hole = ~on & low, move = on & ~low;
     uint32_t h = holes + pages_scan(__popc(hole), L.scan, total);
     holes += total;
     for (; hole; hole &= hole - 1, h++) a.copies[2 + 2 * h] = (int32_t)(p0 + __ffs(hole) - 1);
