@@ -772,10 +772,10 @@ __global__ __launch_bounds__(256) void k_pages_join(PagesK a) {
   float sum = 0.f;
   for (uint32_t i = lane; i < n; i += 64) {
     const float2 s = pair(i);
-    // (a sum of 0 is a part without a finite score: it adds nothing, and its values may be NaN)
-    const float f = s.y < 0.f || s.y == 0.f ? 0.f : s.x == M ? 1.f : exp2f(s.x - M);
+    // (a part that the row sees nothing of has zeros; a weight of 0 is multiplied as any other, so that values that are not finite stay so)
+    const float f = s.y < 0.f ? 0.f : s.x == M ? 1.f : exp2f(s.x - M);
     weight[wv][i] = f;
-    sum += s.y < 0.f || s.y == 0.f ? 0.f : s.y * f;
+    sum += s.y < 0.f ? 0.f : s.y * f;
   }
   sum = wave_sum(sum);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -796,7 +796,7 @@ __global__ __launch_bounds__(256) void k_pages_join(PagesK a) {
         }
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++)
-          if (f[e] != 0.f) acc += v[e] * f[e];
+          if (i0 + e * groups < n) acc += v[e] * f[e];
       }
       for (uint32_t o = per; o < 64; o *= 2)
 #pragma unroll
@@ -806,8 +806,7 @@ __global__ __launch_bounds__(256) void k_pages_join(PagesK a) {
   } else {
     for (uint32_t d = lane; d < a.hd; d += 64) {
       float acc = 0.f;
-      for (uint32_t i = 0; i < n; i++)
-        if (weight[wv][i] != 0.f) acc += a.part[at(i) * a.hd + d] * weight[wv][i];
+      for (uint32_t i = 0; i < n; i++) acc += a.part[at(i) * a.hd + d] * weight[wv][i];
       a.y[(uint64_t)row * a.hd + d] = none ? 0.f : acc / sum;
     }
   }
