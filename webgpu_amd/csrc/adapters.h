@@ -334,14 +334,14 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
           }
         }
       }
-      // the sums of these ranks, over the row's power of two
+      // the sums of these ranks, over the row's power of two (before the scale: the product of both may leave f32's range)
 #pragma unroll
       for (uint32_t b = 0; b < TILES; b++) {
-        float f = scale;
-        if constexpr (sizeof(E) == 2) f *= H.power[16 * b + c];
+        float power = 1.f;
+        if constexpr (sizeof(E) == 2) power = H.power[16 * b + c];
 #pragma unroll
         for (uint32_t m = 0; m < M; m++) {
-          old[m][b] += acc[m][b] * f;
+          old[m][b] += acc[m][b] * power * scale;
           acc[m][b] = ad4{0, 0, 0, 0};
         }
       }
