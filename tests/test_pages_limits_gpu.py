@@ -1,0 +1,102 @@
+"""Attention over pages at the ends of what its arguments can say: ranges of keys on more pages than a workgroup holds the
+numbers of. The sizes of the ranges are worked out here as the launch's plan does, and asserted."""
+import math
+
+import numpy as np
+import pytest
+
+from tests import pages_ref as ref
+from tests.test_attention_pages_gpu import Batch, NO_WINDOW
+from tests.test_pages_gpu import i32, up  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+CUS, IDS = 256, 1024  # page numbers that a workgroup holds at a time
+
+
+class Thin(Batch):
+    """Requests whose tables name the same few pages again and again, so that long ones need little memory."""
+
+    def __init__(self, rng, heads, kvh, hd, page, lengths, tokens=1, counts=None, kv="f32", pages=97):
+        super().__init__(rng, heads, kvh, hd, page, [pages * page], tokens, None, kv=kv, spare=0)
+        self.lengths, self.counts = i32(lengths), None if counts is None else i32(counts)
+        self.table = rng.integers(0, self.pages, (len(lengths), max(ref.held(n, page) for n in lengths))).astype(np.int32)
+        self.q = rng.standard_normal((len(lengths), tokens, heads, hd)).astype(np.float32)
+
+    def want(self, scale, window=NO_WINDOW):
+        """tests/pages_ref.py's formula, the queries of a request and kv head at once."""
+        y = np.zeros(self.q.shape)
+        page, kvh, hd = self.k.shape[1:]
+        group = self.heads // kvh
+        for r, n in enumerate(self.lengths):
+            asked = min(int(n), self.tokens if self.counts is None else max(0, min(int(self.counts[r]), self.tokens)))
+            if not asked:
+                continue
+            j = np.arange(n)
+            ids = self.table[r, j // page]
+            on = (ids >= 0) & (ids < self.pages)
+            pos = int(n) - asked + np.arange(asked)[:, None]
+            sees = ((j <= pos) & (j > pos - window) & on)[:, None]
+            at = np.where(on, ids, 0), j % page
+            for h in range(kvh):
+                k, v = (m[at[0], at[1], h].astype(np.float64) for m in (self.k, self.v))
+                s = self.q[r, :asked, h * group:(h + 1) * group].astype(np.float64) @ k.T * scale
+                s = np.where(sees, s, -np.inf)
+                top = s.max(-1, keepdims=True)
+                p = np.where(sees, np.exp(s - np.where(np.isfinite(top), top, 0)), 0)
+                total = p.sum(-1, keepdims=True)
+                y[r, :asked, h * group:(h + 1) * group] = p @ v / np.where(total > 0, total, 1)
+        return y
+
+
+def longest_range(b, unit, target):
+    """Pages of the longest range of keys of a workgroup: chunks of whole units, as many as `target` makes of the batch."""
+    units = [ref.held(int(n), unit) for n in b.lengths]
+    chunk = math.ceil(sum(units) / target)
+    return max(ref.held(ref.held(u, ref.held(u, chunk)) * unit if u > chunk else int(n), b.page) for u, n in zip(units, b.lengths))
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
+@pytest.mark.parametrize("page,lengths", [(1, [2500, 1025, 1024, 1, 0, 3100, 2049, 700] * 4), (2, [5000, 4097, 3, 2100] * 8)])
+@pytest.mark.parametrize("hd", [8, 64, 20])
+def test_direct_ranges_of_more_pages_than_are_held(gpu, up, hd, page, lengths, kv):  # noqa: F811
+    rng = np.random.default_rng(page + hd)
+    b = Thin(rng, 32, 32, hd, page, lengths, kv=kv)
+    # one row of a kv head: 32 workgroups a chunk, four a CU (head dims of no multiple of 8: tiles of keys that fit 50000 bytes)
+    unit = (32 if kv == "f16" else 16) * 4 if hd % 8 == 0 else 64
+    assert longest_range(b, unit, 4 * CUS // 32) > IDS
+    b.check(b.run(gpu, up, 0.3), 0.3)
+    for window in (1100, 40):
+        b.check(b.run(gpu, up, 0.3, window), 0.3, window)
+    # pages that are none, the first of them behind those that are held first
+    kept = b.table.copy()
+    b.table[0, 1030], b.table[1, b.table.shape[1] - 5], b.table[5 % len(lengths), 1500] = -1, 2 ** 31 - 1, b.pages
+    b.check(b.run(gpu, up, 0.3), 0.3)
+    b.table[0, 7] = -2
+    b.check(b.run(gpu, up, 0.3), 0.3)
+    # a value that is not finite there, which all see
+    b.table = kept
+    b.v[int(b.table[0, 1040]), 0, 3, hd - 1] = np.inf
+    got, want = b.run(gpu, up, 0.3), b.want(0.3)
+    assert np.array_equal(np.isinf(got), np.isinf(want)) and not np.isnan(got).any()
+    fine = np.isfinite(want)
+    assert np.abs(got[fine] - want[fine]).max() <= b.bound(0.3)[2]
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_staged_ranges_of_more_pages_than_are_held(gpu, up, hd):  # noqa: F811
+    rng = np.random.default_rng(hd)
+    heads, tokens = 64, 128
+    lengths, counts = [2300, 1100, 700, 40], [128, 127, 100, 40]
+    b = Thin(rng, heads, heads, hd, 1, lengths, tokens, counts, kv="f16")
+    rows = 64 if hd == 256 else 128
+    wgs = heads * tokens // rows
+    at_once = CUS // wgs
+    target = at_once - 2 if len(lengths) <= at_once else max(1, 2 * CUS // wgs)
+    assert longest_range(b, 128, target) > IDS
+    scale = 1 / math.sqrt(hd)
+    b.check(b.run(gpu, up, scale), scale)
+    b.check(b.run(gpu, up, scale, 1200), scale, 1200)
+    b.table[0, 1100], b.table[1, 1090] = -1, b.pages
+    b.check(b.run(gpu, up, scale), scale)
+    b.table[2, 3] = -7
+    b.check(b.run(gpu, up, scale, 1200), scale, 1200)
