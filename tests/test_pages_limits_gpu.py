@@ -1,5 +1,6 @@
 """Attention over pages at the ends of what its arguments can say: ranges of keys on more pages than a workgroup holds the
-numbers of. The sizes of the ranges are worked out here as the launch's plan does, and asserted."""
+numbers of, and prefixes of more threads than a launch takes. The sizes of the ranges are worked out here as the launch's plan does, and
+asserted."""
 import math
 
 import numpy as np
@@ -7,7 +8,7 @@ import pytest
 
 from tests import pages_ref as ref
 from tests.test_attention_pages_gpu import Batch, NO_WINDOW
-from tests.test_pages_gpu import i32, up  # noqa: F401
+from tests.test_pages_gpu import i32, read, up  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 CUS, IDS = 256, 1024  # page numbers that a workgroup holds at a time
@@ -100,3 +101,28 @@ def test_staged_ranges_of_more_pages_than_are_held(gpu, up, hd):  # noqa: F811
     b.check(b.run(gpu, up, scale), scale)
     b.table[2, 3] = -7
     b.check(b.run(gpu, up, scale, 1200), scale, 1200)
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
+def test_a_prefix_of_more_threads_than_a_launch_takes(gpu, up, kv):  # noqa: F811
+    """2^20 kv heads over a prefix of 16368 pages: parts of fewer than 1024 page numbers would be more than 2^32 threads along x. The
+    prefix is one page again and again, computed apart; the pages behind it hold other values."""
+    heads, hd, shared, tail = 1 << 20, 8, 16368, 3
+    kind, half = (np.float16, True) if kv == "f16" else (np.float32, False)
+    values = np.arange(1, 4, dtype=kind)[:, None] * np.ones(heads * hd, kind)  # page p holds p + 1
+    table = np.zeros((2, shared + tail), np.int32)
+    table[:, shared:] = [[1], [2]]
+    lengths = i32([shared + 1, shared + tail])
+    held = [gpu.buffer(n) for n in (2 * heads * hd * 4, values.nbytes, 2 * heads * hd * 4)]  # zero queries and keys: equal weights
+    try:
+        q, k, y = held
+        for owner in (0, 1):
+            (gpu.attention_pages_f16kv if half else gpu.attention_pages)(q, k, up(values), y, up(table), up(lengths), heads, heads, hd, 1.0, NO_WINDOW, 1,
+                                                                         shared + tail, 3, 2, shared=shared, owner=owner)
+            got = read(gpu, y, (2, heads * hd), np.float32)
+            want = np.array([(shared + 2) / (shared + 1), (shared + 3 * tail) / (shared + tail)])
+            # equal weights: their sums are whole numbers in f32, the values' products with them and the quotient round
+            assert np.abs(got - want[:, None]).max() <= 4 * 2.0 ** -24 * want.max()
+    finally:
+        for b in held:
+            gpu.destroy(b)

@@ -862,8 +862,9 @@ static PagesLaunch pages_launch(const PagesAttnArgs &in) {
     const uint64_t wgs = in.kv_heads * std::max<uint64_t>(1, (prows + p.prows / 4) / p.prows);
     const double held = (double)in.requests * in.tokens * in.heads * in.hd * 8 / 4e6;
     double best = 1e30;
-    // (a launch has at most 65535 blocks of rows along y)
-    for (uint32_t n = 1; p.pblocks <= 65535 && n <= PAGES_PREFIX && (uint64_t)(n - 1) * unit < in.shared; n++) {
+    // (a launch has at most 65535 blocks of rows along y, and fewer than 2^32 threads along x)
+    const uint64_t threads = (uint64_t)in.kv_heads * (p.pstaged ? TREE_STAGED_NT : PAGES_WG);
+    for (uint32_t n = 1; p.pblocks <= 65535 && n <= PAGES_PREFIX && threads * n <= 0xFFFFFFFFull && (uint64_t)(n - 1) * unit < in.shared; n++) {
       const uint32_t per = ((in.shared + n - 1) / n + unit - 1) / unit * unit, parts = (in.shared + per - 1) / per;
       if (parts < n || (p.mfma && per >> in.shift >= PAGES_IDS)) continue;  // (too many parts for that: computed apart)
       const double work = p.mfma ? (in.kv16 ? 2.1 : 3.1) * ((per + block * slices - 1) / (block * slices)) : 0.5 * per;
