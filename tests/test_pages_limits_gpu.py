@@ -1,5 +1,5 @@
 """Attention over pages at the ends of what its arguments can say: ranges of keys on more pages than a workgroup holds the
-numbers of, and prefixes of more threads than a launch takes. The sizes of the ranges are worked out here as the launch's plan does, and
+numbers of, and prefixes of more threads than a launch takes, and what a call allocates. The sizes of the ranges are worked out here as the launch's plan does, and
 asserted."""
 import math
 
@@ -8,7 +8,8 @@ import pytest
 
 from tests import pages_ref as ref
 from tests.test_attention_pages_gpu import Batch, NO_WINDOW
-from tests.test_pages_gpu import i32, read, up  # noqa: F401
+from tests.test_pages_gpu import Held, i32, read, up  # noqa: F401
+from webgpu_amd.gpu import Compute
 
 pytestmark = pytest.mark.gpu
 CUS, IDS = 256, 1024  # page numbers that a workgroup holds at a time
@@ -126,3 +127,21 @@ def test_a_prefix_of_more_threads_than_a_launch_takes(gpu, up, kv):  # noqa: F81
     finally:
         for b in held:
             gpu.destroy(b)
+
+
+@pytest.mark.parametrize("kv,heads,hd,tokens,lengths,mib", [("f32", 128, 8, 512, [512], 10), ("f16", 128, 8, 320, [330, 17, 320, 0], 14), ("f16", 32, 64, 1024, [1024], 26),
+                                                            ("f32", 128, 20, 100, [160, 90, 130], 16)])
+def test_prompts_that_are_not_cut_need_no_scratch(kv, heads, hd, tokens, lengths, mib):
+    """So many blocks of rows that one chunk for each request is all that is wanted: nothing is kept for a join, and a budget that has room
+    for the buffers alone suffices."""
+    gpu = Compute(mib).init()
+    up = Held(gpu)  # noqa: F811
+    try:
+        b = Batch(np.random.default_rng(tokens), heads, heads, hd, 16, lengths, tokens, kv=kv)
+        before = gpu.allocated
+        got = b.run(gpu, up, 0.2)
+        assert gpu.allocated - before == sum(x.size for x in up.held)
+        b.check(got, 0.2)
+    finally:
+        up.free()
+        gpu.dispose()

@@ -874,9 +874,9 @@ static PagesLaunch pages_launch(const PagesAttnArgs &in) {
   }
   return p;
 }
-// Whether some row may have several parts.
+// Whether some row may have several parts: with one chunk wanted each request is one (pages_plan() rounds up).
 static bool pages_joins(const PagesAttnArgs &in, const PagesLaunch &p) {
-  return p.nprefix || ((uint64_t)in.max_pages << in.shift) > (uint64_t)p.unit * p.least;
+  return p.nprefix || (p.target > 1 && ((uint64_t)in.max_pages << in.shift) > (uint64_t)p.unit * p.least);
 }
 
 uint64_t attention_pages_scratch_floats(const PagesAttnArgs &in) {
