@@ -910,9 +910,10 @@ __global__ __launch_bounds__(TREE_STAGED_NT) void k_attn_tree_staged(TreeK a, Tr
 
 // The splits of a row in order, of partial outputs and (max, sum) pairs (tree_pairs), maxima in powers of
 // two. A sum of zero is a split without keys that the row sees (or without a finite score, which adds
-// nothing either); the last split knows padding, by a negative sum. A row always sees itself, so sums
+// nothing but values that are not finite); the last split knows padding, by a negative sum. A row always sees itself, so sums
 // that are all zero mean scores that were all -inf: 0 / 0, as the formula has it.
-// A wavefront per row: the splits' weights go over its lanes and LDS, then (VEC: hd a power of two of 4 to 256) lane groups
+// A wavefront per row: the splits' weights go over its lanes and LDS (a weight of 0 is multiplied as any other, so that values that are not
+// finite stay so; a split that the row sees nothing of has zeros), then (VEC: hd a power of two of 4 to 256) lane groups
 // of hd / 4 (at most 64) lanes take every (64 / group)-th split, 16 bytes a lane and eight loads ahead.
 constexpr uint32_t TREE_SPLITS = 256;
 template <bool VEC>
@@ -958,8 +959,7 @@ __global__ __launch_bounds__(256) void k_attn_tree_join(const float *part, float
             v[e] = z < nsplit ? *(const f32x4 *)(p + z * zs + d) : f32x4{0, 0, 0, 0};
           }
 #pragma unroll
-          for (uint32_t e = 0; e < 8; e++)
-            if (f[e] != 0.f) acc += v[e] * f[e];
+          for (uint32_t e = 0; e < 8; e++) acc += v[e] * f[e];
         }
       for (uint32_t o = width; o < groups * width; o *= 2)  // groups is a power of two where there are several
 #pragma unroll
@@ -970,8 +970,7 @@ __global__ __launch_bounds__(256) void k_attn_tree_join(const float *part, float
   } else {
     for (uint32_t d = lane; d < hd; d += 64) {
       float acc = 0.f;
-      for (uint32_t z = 0; z < nsplit; z++)
-        if (wz[wv][z] != 0.f) acc += p[z * zs + d] * wz[wv][z];
+      for (uint32_t z = 0; z < nsplit; z++) acc += p[z * zs + d] * wz[wv][z];
       if (blockIdx.x * 4 + wv < rows) y[row * hd + d] = pad ? 0.f : acc * inv;
     }
   }
