@@ -299,15 +299,16 @@ int wgd_kv_commit(wgd_context *ctx, wgd_buffer *const *rings, uint32_t count, co
  * and refs[p] (int32[pages]) how many rows of the table hold page p; 0 or less is a free page. Zero-filled buffers are the empty
  * state. A host that keeps pages itself adds to their refs. The page is a power of two up to WGD_PAGE_MAX; requests <=
  * WGD_REQUESTS_MAX; max_pages * page and pages * page are below 2^31. Lengths outside [0, max_pages * page] count as
- * the nearest end. These launches wait for nothing, and their choices do not depend on the order of threads. They
- * allocate nothing once a call of the same sizes has run (WGD_E_STATE where a capture would have to). Buffers that a call writes
- * are others than those that it reads, unless it says so. */
+ * the nearest end (wgd_pages_extend refuses such a request, with -1 in `added`, and leaves its length). These launches
+ * wait for nothing, and their choices do not depend on the order of threads. They allocate nothing once a call of the same
+ * sizes has run (WGD_E_STATE where a capture would have to); captured ones share the context's scratch, so graphs are
+ * replayed in order with its other work. Buffers that a call writes are others than those that it reads, unless it says so. */
 #define WGD_REQUESTS_MAX 1024
 #define WGD_PAGE_MAX 1024
 
 /* Places for counts[r] (int32[requests], in [0, tokens]; NULL: `tokens` each) new tokens of every request: in the
  * order of requests, each takes the lowest free pages that it needs beyond those it has, or where fewer are left none
- * at all: then, and where the tokens do not fit max_pages or counts[r] lies outside, added[r] (int32[requests]) becomes -1
+ * at all: then, and where the tokens do not fit max_pages, or counts[r] or lengths[r] lies outside, added[r] (int32[requests]) becomes -1
  * and the request stays as it was, while later ones may still fit. Else added[r] = counts[r], which is what lengths[r] grows
  * by; positions[r * tokens + t] (for wgd_rope_at) and slots[r * tokens + t] (page * id + place, for wgd_pages_store) are
  * those of its t-th new token, and -1 where there is none (both int32[requests * tokens]). requests * tokens <= 2^24. */

@@ -145,3 +145,22 @@ def test_prompts_that_are_not_cut_need_no_scratch(kv, heads, hd, tokens, lengths
     finally:
         up.free()
         gpu.dispose()
+
+
+def test_lengths_that_are_none(gpu, up):  # noqa: F811
+    """extend refuses such requests whatever their count, fork and attention take the nearest end."""
+    page, width, pages = 4, 3, 12
+    table = i32(np.arange(12).reshape(4, 3))
+    lengths, refs = i32([-1, 13, -2 ** 31, 2 ** 31 - 1]), i32([0, 0, 0, 1, 1, 1, 0, 0, 0, 1, 1, 1])
+    b = [up(x) for x in (table, lengths, refs)]
+    outs = [up(np.full(n, 77, np.int32)) for n in (4, 8, 8)]
+    for counts in ([0] * 4, [1, 0, 2, 1]):
+        gpu.pages_extend(*b, *outs, 4, 2, page, width, pages, counts=up(i32(counts)))
+        for x, want in zip(b + outs, (table, lengths, refs, i32([-1] * 4), i32([-1] * 8), i32([-1] * 8))):
+            assert np.array_equal(read(gpu, x, want.shape), want)
+    copies = up(np.zeros(9, np.int32))
+    gpu.pages_fork(*b, up(i32([0, 0, 3, 3])), copies, 4, page, width, pages)
+    t, n, c, pairs = ref.fork(table, lengths, refs, [0, 0, 3, 3], None, page)
+    assert n.tolist() == [-1, 0, 12, 2 ** 31 - 1] and pairs == []
+    for x, want in zip(b, (t, n, c)):
+        assert np.array_equal(read(gpu, x, want.shape), want)
