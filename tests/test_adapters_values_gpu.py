@@ -62,6 +62,15 @@ def test_adapters_of_large_and_small_inputs(gpu, up, batch, rank, cols, rows, x_
 
 
 @pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("batch,rank", [(40, 65), (25, 128), (3, 300), (40, 1024)])
+def test_adapters_of_many_ranks_round_y_once(gpu, up, batch, rank, half):  # noqa: F811
+    """What is added is far smaller than y: the one rounding of the sum into y is nearly all of the error."""
+    rng = np.random.default_rng(rank)
+    a, b, x, scales = case(rng, batch, 2, rank, 24, 257, half)
+    held(gpu, up, a, b, (x * 1e-5).astype(np.float32), rng.uniform(1, 2, (batch, 257)).astype(np.float32), rng.integers(0, 2, batch), scales)
+
+
+@pytest.mark.parametrize("half", [False, True])
 def test_adapters_whose_scale_and_inner_sums_are_large(gpu, up, half):  # noqa: F811
     """The scale times an inner sum passes f32's range, the scale times B's products with them does not."""
     rng = np.random.default_rng(8)

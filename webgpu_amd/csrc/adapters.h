@@ -253,8 +253,9 @@ __device__ __forceinline__ void adapter_h(const AdaptersArgs &a, AdapterH<E> &H,
 
 // y of `last - first` elements and TILES tiles of 16 rows, M tiles of 16 elements a wavefront at a time. Lane (g, c) has
 // W ranks at W g of element c and of row c; the result's 4 elements at 4 g of row c lie side by side in y. y and the first ranks of B are
-// asked for a step ahead; places that are not there read one that is, and are masked where they are used.
-template <class E, uint32_t M, uint32_t TILES, bool VEC, bool YVEC>
+// asked for a step ahead; places that are not there read one that is, and are masked where they are used. MANY: more than AD_RANKS ranks, whose
+// sums meet before y is added to them once. (With that for all ranks, 4 rows of rank 8 took 9.3 us in place of 7.8, 64 of rank 16 15.9 in place of 13.7.)
+template <class E, uint32_t M, uint32_t TILES, bool VEC, bool YVEC, bool MANY>
 __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &H, uint32_t t0, uint32_t order, uint32_t n, int32_t kind, uint32_t first,
                                             uint32_t last, uint32_t splits) {
   constexpr uint32_t W = 16 / sizeof(E), STEP = 4 * W;
@@ -291,7 +292,7 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
   load(first + 16 * M * wave, ahead, wahead);
   for (uint32_t o0 = first; o0 < last; o0 += 64 * M) {
     const uint32_t o = o0 + 16 * M * wave;
-    ad4 acc[M][TILES] = {};
+    ad4 acc[M][TILES] = {}, sum[M][TILES] = {};
 #pragma unroll
     for (uint32_t m = 0; m < M; m++) {
 #pragma unroll
@@ -300,7 +301,7 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
     }
     load(min(o + 64 * M, last - 1), ahead, wahead);
     for (uint32_t k0 = 0; k0 < a.rank; k0 += AD_RANKS) {
-      if (o0 == first || a.rank > AD_RANKS) {
+      if (o0 == first || MANY) {
         __syncthreads();
         adapter_h<E, TILES>(a, H, t0, order, n, k0, splits);
         __syncthreads();
@@ -334,14 +335,15 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
           }
         }
       }
-      // the sums of these ranks, over the row's power of two (before the scale: the product of both may leave f32's range)
+      // these ranks' sums, over the row's power of two (before the scale: the product of both may leave f32's range)
 #pragma unroll
       for (uint32_t b = 0; b < TILES; b++) {
         float power = 1.f;
         if constexpr (sizeof(E) == 2) power = H.power[16 * b + c];
 #pragma unroll
         for (uint32_t m = 0; m < M; m++) {
-          old[m][b] += acc[m][b] * power * scale;
+          if constexpr (MANY) sum[m][b] += acc[m][b] * power;
+          else old[m][b] += acc[m][b] * power * scale;
           acc[m][b] = ad4{0, 0, 0, 0};
         }
       }
@@ -351,7 +353,8 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
 #pragma unroll
       for (uint32_t b = 0; b < TILES; b++) {
         const uint32_t e = o + 16 * m + 4 * g;
-        const ad4 v = old[m][b];
+        ad4 v = old[m][b];
+        if constexpr (MANY) v += sum[m][b] * scale;
         if constexpr (YVEC) {
           if (16 * b + c < n && e < last) *(ad4 *)(y[b] + e) = v;
         } else {
@@ -364,7 +367,7 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
 }
 
 // The sum into y: `span` elements of the 64 rows' y by one workgroup; 64 or, with 16 rows of an adapter or fewer, 256 of them at a time.
-template <class E, bool VEC, bool YVEC>
+template <class E, bool VEC, bool YVEC, bool MANY>
 __global__ __launch_bounds__(256) void k_adapters_up(AdaptersArgs a, uint32_t chunks, uint32_t splits, uint32_t span) {
   __shared__ AdapterH<E> h;
   const uint32_t t0 = blockIdx.x / chunks * AD_ROWS, first = blockIdx.x % chunks * span, last = min(a.rows, first + span);
@@ -376,8 +379,8 @@ __global__ __launch_bounds__(256) void k_adapters_up(AdaptersArgs a, uint32_t ch
     if (j != next) continue;
     next += gridDim.y;
     const uint32_t n = (uint32_t)__popcll(r.rows), order = adapter_order(r.rows);
-    if (n <= 16) adapter_sum<E, 4, 1, VEC, YVEC>(a, h, t0, order, n, r.w, first, last, splits);
-    else adapter_sum<E, 1, 4, VEC, YVEC>(a, h, t0, order, n, r.w, first, last, splits);
+    if (n <= 16) adapter_sum<E, 4, 1, VEC, YVEC, MANY>(a, h, t0, order, n, r.w, first, last, splits);
+    else adapter_sum<E, 1, 4, VEC, YVEC, MANY>(a, h, t0, order, n, r.w, first, last, splits);
   }
 }
 
@@ -412,7 +415,9 @@ template <class E, bool VEC> static hipError_t launch_adapters(hipStream_t s, co
 }
 template <class E, bool VEC, bool YVEC> static hipError_t launch_adapters_up(hipStream_t s, const AdaptersArgs &a) {
   const AdaptersPlan p = adapters_plan(a);
-  hipLaunchKernelGGL((k_adapters_up<E, VEC, YVEC>), dim3(p.blocks * p.chunks, p.kinds), dim3(256), 0, s, a, p.chunks, p.splits, p.out);
+  const dim3 grid(p.blocks * p.chunks, p.kinds);
+  if (a.rank > AD_RANKS) hipLaunchKernelGGL((k_adapters_up<E, VEC, YVEC, true>), grid, dim3(256), 0, s, a, p.chunks, p.splits, p.out);
+  else hipLaunchKernelGGL((k_adapters_up<E, VEC, YVEC, false>), grid, dim3(256), 0, s, a, p.chunks, p.splits, p.out);
   return hipGetLastError();
 }
 template <class E> static hipError_t launch_adapters_of(hipStream_t s, const AdaptersArgs &a) {
