@@ -254,11 +254,14 @@ __device__ __forceinline__ void adapter_h(const AdaptersArgs &a, AdapterH<E> &H,
 // y of `last - first` elements and TILES tiles of 16 rows, M tiles of 16 elements a wavefront at a time. Lane (g, c) has
 // W ranks at W g of element c and of row c; the result's 4 elements at 4 g of row c lie side by side in y. y and the first ranks of B are
 // asked for a step ahead; places that are not there read one that is, and are masked where they are used. MANY: more than AD_RANKS ranks, whose
-// sums meet before y is added to them once. (With that for all ranks, 4 rows of rank 8 took 9.3 us in place of 7.8, 64 of rank 16 15.9 in place of 13.7.)
+// sums meet before y is added to them, once: f32 ones in the accumulators, others (over a power of two for each AD_RANKS of a row) in `sum`, with the next ranks' B asked for
+// ahead of their h. (With that for all ranks, 4 rows of rank 8 took 9.3 us in place of 7.8. 4 and 64 rows of rank 128, 1024 x 2048: 15.5 and 21.3 f32, 12.6 and 17.5
+// f16; with f32's four steps unrolled 17.4 and 20.9, f16 without B ahead 13.3 and 17.6.)
 template <class E, uint32_t M, uint32_t TILES, bool VEC, bool YVEC, bool MANY>
 __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &H, uint32_t t0, uint32_t order, uint32_t n, int32_t kind, uint32_t first,
                                             uint32_t last, uint32_t splits) {
-  constexpr uint32_t W = 16 / sizeof(E), STEP = 4 * W;
+  constexpr bool AHEAD = MANY && sizeof(E) == 2, CARRY = MANY && sizeof(E) == 4;
+  constexpr uint32_t W = 16 / sizeof(E), STEP = 4 * W, UNROLL = CARRY ? 1 : AD_RANKS / STEP;
   const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float scale = a.scales[kind];
   typedef ad_vec<E, W> wvec;
@@ -301,15 +304,21 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
     }
     load(min(o + 64 * M, last - 1), ahead, wahead);
     for (uint32_t k0 = 0; k0 < a.rank; k0 += AD_RANKS) {
+      if constexpr (AHEAD)
+        if (k0)
+#pragma unroll
+          for (uint32_t m = 0; m < M; m++) wv[m] = get(o + 16 * m, k0);
       if (o0 == first || MANY) {
         __syncthreads();
         adapter_h<E, TILES>(a, H, t0, order, n, k0, splits);
         __syncthreads();
       }
+#pragma unroll UNROLL
       for (uint32_t s = 0; s < AD_RANKS && k0 + s < a.rank; s += STEP) {
-        wvec wn[M];
+        wvec wn[M] = {};
+        if (!AHEAD || s + STEP < AD_RANKS)
 #pragma unroll
-        for (uint32_t m = 0; m < M; m++) wn[m] = get(o + 16 * m, k0 + s + STEP);
+          for (uint32_t m = 0; m < M; m++) wn[m] = get(o + 16 * m, k0 + s + STEP);
         const bool there = !VEC || k0 + s + W * g < a.rank;
         wvec w[M];
 #pragma unroll
@@ -342,6 +351,7 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
         if constexpr (sizeof(E) == 2) power = H.power[16 * b + c];
 #pragma unroll
         for (uint32_t m = 0; m < M; m++) {
+          if constexpr (CARRY) continue;
           if constexpr (MANY) sum[m][b] += acc[m][b] * power;
           else old[m][b] += acc[m][b] * power * scale;
           acc[m][b] = ad4{0, 0, 0, 0};
@@ -354,7 +364,7 @@ __device__ __forceinline__ void adapter_sum(const AdaptersArgs &a, AdapterH<E> &
       for (uint32_t b = 0; b < TILES; b++) {
         const uint32_t e = o + 16 * m + 4 * g;
         ad4 v = old[m][b];
-        if constexpr (MANY) v += sum[m][b] * scale;
+        if constexpr (MANY) v += (CARRY ? acc[m][b] : sum[m][b]) * scale;
         if constexpr (YVEC) {
           if (16 * b + c < n && e < last) *(ad4 *)(y[b] + e) = v;
         } else {
