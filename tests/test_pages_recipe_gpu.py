@@ -48,9 +48,9 @@ def test_the_written_step_runs_and_answers(gpu, up):  # noqa: F811
     def low_rank(name, x, w):
         return 0 if w < 0 else float(scales[w]) * (B[name][w].astype(np.float64) @ (A[name][w].astype(np.float64) @ x))
 
-    def run(counts):
+    def run(counts, requests=requests, tokens=tokens):
         x = rng.standard_normal((requests * tokens, hidden)).astype(np.float32)
-        env.update(x=up(x), counts=up(i32(counts)), which=up(i32(np.repeat(which, tokens))))
+        env.update(x=up(x), counts=up(i32(counts)), which=up(i32(np.repeat(which[:requests], tokens))), requests=requests, tokens=tokens)
         exec(step, env)
         assert read(gpu, env["added"], requests).tolist() == list(counts)
         y = read(gpu, env["y"], (requests, tokens, heads, hd), np.float32)
@@ -78,6 +78,7 @@ def test_the_written_step_runs_and_answers(gpu, up):  # noqa: F811
     run([6, 1, 3, 1])
     run([1, 1, 1, 1])
     env.update(origin=up(i32([0, 0, -1, 3])), keep=up(i32([13, 11, 0, 7])))
+    env.update(requests=requests)
     exec(between, env)
     cached[:] = [cached[0], cached[0][:11], [], cached[3][:7]]
     which[:] = [0, 0, 2, 1]
@@ -85,3 +86,5 @@ def test_the_written_step_runs_and_answers(gpu, up):  # noqa: F811
     assert used[:used.sum()].all()
     run([1, 1, 4, 1])
     run([2, 6, 1, 0])
+    run([6, 3], requests=2)  # those with a chunk are the table's first rows: two batches
+    run([0, 0, 1, 1], tokens=1)
