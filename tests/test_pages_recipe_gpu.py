@@ -1,4 +1,4 @@
-"""The step of a batch as INTEGRATION.md (3d) writes it down: its lines are run as they stand, over prompts, decoded tokens, a fork and
+"""The step of a batch as the guide for hosts writes it down: its lines are run as they stand, over prompts, decoded tokens, a fork and
 a compaction, and every request's attention is held to float64 over its tokens alone."""
 import math
 import os
